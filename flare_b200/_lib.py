@@ -72,6 +72,22 @@ class GatherTensor(ctypes.Structure):
     _fields_ = [("src", vp), ("src_alt", vp), ("dst", vp), ("row_bytes", ctypes.c_int)]
 
 
+ll = ctypes.c_longlong
+
+
+class LookupArgs(ctypes.Structure):
+    _fields_ = [("table", vp), ("scales", vp), ("index", vp), ("weight", vp), ("out", vp), ("rows", ll), ("n", ll),
+                ("table_stride", ll), ("out_stride", ll), ("width", ctypes.c_int), ("table_type", ctypes.c_int),
+                ("index_type", ctypes.c_int), ("out_type", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+class LookupGradArgs(ctypes.Structure):
+    _fields_ = [("dout", vp), ("table", vp), ("index", vp), ("weight", vp), ("dtable", vp), ("dweight", vp),
+                ("workspace", vp), ("rows", ll), ("n", ll), ("dout_stride", ll), ("table_stride", ll),
+                ("workspace_bytes", ll), ("width", ctypes.c_int), ("table_type", ctypes.c_int),
+                ("index_type", ctypes.c_int), ("dout_type", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
 class Stats(ctypes.Structure):
     _fields_ = [("rays", ctypes.c_longlong), ("passes", ctypes.c_longlong), ("hits_composited", ctypes.c_longlong),
                 ("prim_tests", ctypes.c_longlong), ("node_visits", ctypes.c_longlong),
@@ -109,6 +125,11 @@ EXPORTS = {
     "flare_selftest_mlp": (ctypes.c_int, [vp, ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, vp]),
     "flare_render_hits_noalloc": (ctypes.c_int, [ctypes.c_int, vp, vp, vp, vp, vp, ctypes.c_int, vp, vp, vp,
                                                  ctypes.c_int, vp, vp, vp]),
+    "flare_lookup": (ctypes.c_int, [ctypes.POINTER(LookupArgs), vp]),
+    "flare_lookup_workspace": (ll, [ll, ll, ctypes.c_int]),
+    "flare_lookup_backward": (ctypes.c_int, [ctypes.POINTER(LookupGradArgs), vp]),
+    "flare_micro_quantize": (ctypes.c_int, [vp, ctypes.c_int, ll, ctypes.c_int, ll, vp, vp, vp]),
+    "flare_micro_dequantize": (ctypes.c_int, [vp, vp, ll, ctypes.c_int, vp, ctypes.c_int, ll, vp]),
 }
 
 _lib = None

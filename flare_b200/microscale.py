@@ -1,0 +1,83 @@
+"""Matrices held in 4 bits an element with a power-of-two scale per 32 (microscaled 4-bit floats), written and read.
+
+A 96-wide f16 descriptor takes 192 of the 312 bytes that a hit reads; held here it takes 52.  `quantize` makes a `Micro4`
+from a tensor, `Micro4.dequantize` and `embedding.lookup` read it back, the renderer's inference methods take one as
+`conditioning_variable`.  Inference only: none of them has a gradient.  No reference counterpart.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib, _ops
+
+BLOCK = 32  # elements that share a scale
+_FLOATS = tuple(_ops.TYPE_CODE)
+
+
+class Micro4:
+    """A (rows, width) matrix in 4 bits an element.
+
+    codes (rows, 16 * blocks) uint8, blocks = ceil(width / 32): two elements a byte, the even one in the low four
+    bits, each a sign bit and the magnitude 0, .5, 1, 1.5, 2, 3, 4 or 6; zero past `width`.  scales (rows, 4 *
+    ceil(blocks / 4)) uint8: a block's elements are multiplied by 2^(byte - 127), byte 255 stands for NaN; bytes past
+    `blocks` are not used.  Both contiguous.
+    """
+
+    __slots__ = ("codes", "scales", "width")
+
+    def __init__(self, codes, scales, width: int):
+        width = int(width)
+        blocks = -(-width // BLOCK)
+        _ops.need(codes, "codes", (torch.uint8,))
+        _ops.need(scales, "scales", (torch.uint8,), codes.device)
+        if width < 1 or codes.dim() != 2:
+            raise ValueError(f"codes: shape {tuple(codes.shape)} for a width of {width}")
+        _ops.need_shape(codes, "codes", (codes.shape[0], 16 * blocks))
+        _ops.need_shape(scales, "scales", (codes.shape[0], -(-blocks // 4) * 4))
+        for t, name, align in ((codes, "codes", 16), (scales, "scales", 4)):
+            if not t.is_contiguous() or t.data_ptr() % align:
+                raise ValueError(f"{name}: tensor must be contiguous and aligned to {align} bytes")
+        self.codes, self.scales, self.width = codes, scales, width
+
+    @property
+    def shape(self):
+        return self.codes.shape[0], self.width
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype=torch.float16):
+        """The (rows, width) values, rounded to f32, f16 or bf16."""
+        lib = _lib.load()
+        if dtype not in _ops.TYPE_CODE:
+            raise ValueError(f"dtype: {dtype}, expected one of {', '.join(str(d) for d in _FLOATS)}")
+        with _ops.on(self.device):
+            out = torch.empty(self.shape, dtype=dtype, device=self.device)
+            _lib.check(lib.flare_micro_dequantize(_ops.ptr(self.codes), _ops.ptr(self.scales), self.shape[0], self.width,
+                                                  _ops.ptr(out), _ops.TYPE_CODE[dtype], self.width,
+                                                  _ops.stream(self.device)), "dequantize")
+        return out
+
+
+def quantize(x) -> Micro4:
+    """The 4-bit form of a (rows, width) tensor, f32, f16 or bf16, width >= 1; rows may be strided.
+
+    A block's scale is 2^(floor(log2 of its largest magnitude) - 2); elements go to the nearest value, ties to the even
+    code, and to 6 scales at most.  A block that holds an infinity or a NaN becomes NaN.
+    """
+    lib = _lib.load()
+    _ops.need(x, "x", _FLOATS)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x: shape {tuple(x.shape)}, expected (rows, width)")
+    rows, width = x.shape
+    x = _ops.rows(x)
+    blocks = -(-width // BLOCK)
+    with _ops.on(x.device):
+        codes = torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((rows, -(-blocks // 4) * 4), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.flare_micro_quantize(_ops.ptr(x), _ops.TYPE_CODE[x.dtype], rows, width, x.stride(0),
+                                            _ops.ptr(codes), _ops.ptr(scales), _ops.stream(x.device)), "quantize")
+    return Micro4(codes, scales, width)

@@ -12,6 +12,7 @@ Differences from the reference, by design:
   * arguments are checked (CUDA, contiguous, dtype, shapes); violations raise ValueError instead of
     corrupting memory;
   * failures raise FlareError (a RuntimeError) carrying the library's message instead of `throw 0`;
+  * the methods that compute no gradient also take the descriptors as a 4-bit `microscale.Micro4`;
   * the work runs on torch.cuda.current_stream() of the renderer's device without a host sync per
     pass beyond reading the active-ray count.
 """
@@ -22,6 +23,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .microscale import Micro4
 
 F32, F16, I32 = torch.float32, torch.float16, torch.int32
 PASS_SLOTS = 42  # FLARE_PASS_SLOTS: hit slots of an internal traversal pass
@@ -90,7 +92,7 @@ class CPyOptiXFLARERenderer:
     def _stream(self):
         return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
 
-    def _scene(self, m, s, q, RGBA, kappa, dec=None):
+    def _scene(self, m, s, q, RGBA, kappa, dec=None, inference=False):
         n = m.shape[0] if m.dim() == 2 else -1
         dv = self.device
         _need(m, "m", F32, (n, 3), dv)
@@ -105,6 +107,12 @@ class CPyOptiXFLARERenderer:
         sc = _lib.Scene(m=_ptr(m), s=_ptr(s), q=_ptr(q), RGBA=_ptr(RGBA), k=_ptr(kappa), n=n)
         if dec is not None:
             cond, feat, A1, b1, A2, b2, A3, b3 = dec
+            if isinstance(cond, Micro4):
+                if not inference:
+                    raise ValueError("conditioning_variable: 4-bit descriptors have no gradient, training needs f16 ones")
+                if cond.device.index != dv:
+                    raise ValueError(f"conditioning_variable: tensor on {cond.device}, renderer on cuda:{dv}")
+                cond = cond.dequantize(F16)  # read as the f16 rows that the decoder kernels take
             kind = decoder_kind(cond)
             cdim, nfeat = DECODERS[kind]
             _need(cond, "conditioning_variable", F16, (n, cdim), dv)
@@ -122,6 +130,7 @@ class CPyOptiXFLARERenderer:
             sc.cond, sc.features = _ptr(cond), _ptr(feat)
             sc.A1, sc.A2, sc.A3 = _ptr(A1), _ptr(A2), _ptr(A3)
             sc.b1, sc.b2, sc.b3 = _ptr(b1), _ptr(b2), _ptr(b3)
+            sc.held = cond  # the rows of a 4-bit table live until the launch
         return sc
 
     def _rays(self, O, v):
@@ -219,7 +228,8 @@ class CPyOptiXFLARERenderer:
 
     def GetMedianDepth(self, conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3, O, v, m, s, q, RGBA,
                        kappa, T_threshold, depth_and_index):
-        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3))
+        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3),
+                         inference=True)
         self._forward(_lib.FWD_MEDIAN, sc, O, v, None, (0, 0, 0), T_threshold, depth_and_index=(depth_and_index, 2))
 
     def Forward_training(self, conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3, O, v, bitmap,
@@ -232,12 +242,14 @@ class CPyOptiXFLARERenderer:
 
     def Forward_inference(self, conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3, O, v, bitmap,
                           bg_color_R, bg_color_G, bg_color_B, m, s, q, RGBA, kappa, T_threshold):
-        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3))
+        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3),
+                         inference=True)
         self._forward(_lib.FWD_INFERENCE, sc, O, v, bitmap, (bg_color_R, bg_color_G, bg_color_B), T_threshold)
 
     def Forward_pca(self, conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3, override_colors, O, v,
                     bitmap, bg_color_R, bg_color_G, bg_color_B, m, s, q, RGBA, kappa, T_threshold):
-        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3))
+        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3),
+                         inference=True)
         _need(override_colors, "override_colors", F32, (self._n, 3), self.device)
         self._forward(_lib.FWD_PCA, sc, O, v, bitmap, (bg_color_R, bg_color_G, bg_color_B), T_threshold,
                       override_colors=(override_colors, 3))
@@ -245,7 +257,8 @@ class CPyOptiXFLARERenderer:
     def Forward_inference_with_geometry(self, conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3, O,
                                         v, bitmap, normal, alpha, expected_depth_numerator, bg_color_R, bg_color_G,
                                         bg_color_B, m, s, q, RGBA, kappa, T_threshold):
-        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3))
+        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3),
+                         inference=True)
         self._forward(_lib.FWD_INFERENCE_GEOMETRY, sc, O, v, bitmap, (bg_color_R, bg_color_G, bg_color_B), T_threshold,
                       normal=(normal, 3), alpha=(alpha, 1), expected_depth_numerator=(expected_depth_numerator, 1))
 

@@ -51,7 +51,8 @@ class CPyFlareViewerRenderer(CPyOptiXFLARERenderer):
         if A.numel() != n:
             raise ValueError(f"A: {A.numel()} elements, expected {n}")
         RGBA = torch.cat([RGB, A.reshape(n, 1).to(torch.float32)], 1).contiguous()
-        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3))
+        sc = self._scene(m, s, q, RGBA, kappa, (conditioning_variable, features_P_hit_object, A1, b1, A2, b2, A3, b3),
+                         inference=True)
         R = self._rays(O, v)
         mats = _host_table(materials, "materials", 6, _lib.VIEWER_MAX_SPHERES)
         if mats.shape[0] < self._spheres.shape[0]:

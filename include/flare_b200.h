@@ -339,6 +339,79 @@ int flare_render_hits_noalloc(int number_of_sides, const float *m, const float *
 int flare_selftest_mlp(const void *X, int rows, const void *A1, const float *b1, const void *A2,
                        const float *b2, const void *A3, const float *b3, float *Y, void *stream);
 
+/*
+ * ------------------------------------------------------------------------------------------------
+ * Operators for decoders and losses that a caller writes outside the fused render path: the rows of
+ * the hit primitives (lookup), the recurrence that composites them (recurrence), and descriptors and
+ * weights held in 4 bits (micro).  No reference counterpart (the reference decodes and composites
+ * inside its kernels only).  They run on the device that is current at the call and on `stream`, keep
+ * nothing between calls, and can be captured into a CUDA graph.  Every buffer is the caller's.
+ * Element types of the void pointers:
+ */
+#define FLARE_F32 0
+#define FLARE_F16 1
+#define FLARE_BF16 2
+#define FLARE_MICRO 3 /* 4-bit codes with a scale byte per 32 elements, see flare_micro_quantize */
+#define FLARE_I32 0
+#define FLARE_I64 1
+
+/*
+ * Row lookup with scaling: out[i] = scale * weight[i] * table[index[i]], i < n (weight NULL: 1).  An
+ * index outside [0, rows) names no row -- hit lists pad with -1 -- and gives a row of zeros whatever
+ * its weight.  Products are formed in 32 bits and rounded once to out_type.  Strides are in elements
+ * (of 4 bits' values for FLARE_MICRO, whose rows are as flare_micro_quantize lays them out; its
+ * table_stride is ignored).  Types: out may have any of the three float types.
+ */
+typedef struct flare_lookup_args {
+    const void *table;            /* (rows, width) */
+    const unsigned char *scales;  /* FLARE_MICRO: its scale bytes, else NULL */
+    const void *index;            /* (n) */
+    const float *weight;          /* (n) or NULL */
+    void *out;                    /* (n, width), written */
+    long long rows, n, table_stride, out_stride;
+    int width, table_type, index_type, out_type;
+    float scale;
+} flare_lookup_args;
+int flare_lookup(const flare_lookup_args *a, void *stream);
+
+/*
+ * Gradient of the lookup: dtable[p] = scale * sum over the i with index[i] = p of weight[i] * dout[i], in
+ * 32 bits and in a fixed order (the entries are sorted by index, stably), so that results repeat bit for
+ * bit; rows that no entry names get zeros.  dweight[i] = scale * <dout[i], table[index[i]]>, 0 where the
+ * index names no row.  dtable or dweight may be NULL; table is read for dweight only.  workspace:
+ * flare_lookup_workspace bytes, 16-byte aligned, contents irrelevant.  rows < 2^31 - 1, n < 2^31 - 4096.
+ */
+typedef struct flare_lookup_grad_args {
+    const void *dout;             /* (n, width) */
+    const void *table;            /* (rows, width), not FLARE_MICRO */
+    const void *index;            /* (n) */
+    const float *weight;          /* (n) or NULL */
+    float *dtable;                /* (rows, width) contiguous, written */
+    float *dweight;               /* (n), written */
+    void *workspace;
+    long long rows, n, dout_stride, table_stride, workspace_bytes;
+    int width, table_type, index_type, dout_type;
+    float scale;
+} flare_lookup_grad_args;
+long long flare_lookup_workspace(long long rows, long long n, int width);
+int flare_lookup_backward(const flare_lookup_grad_args *a, void *stream);
+
+/*
+ * Microscaled 4-bit storage: blocks of 32 consecutive elements of a row share a power-of-two scale 2^e, e =
+ * floor(log2 of the block's largest magnitude) - 2 clamped to [-127, 127], held as the byte e + 127 (0 for a
+ * block of zeros); each element is the 4-bit float (1 sign, 2 exponent, 1 mantissa bit: 0 .5 1 1.5 2 3 4 6)
+ * nearest to x 2^-e, ties to the even code, magnitudes above 6 to 6.  A block with an infinity or NaN gets
+ * the byte 255, which stands for NaN in all its elements.
+ * codes (rows, 16 * blocks) bytes, blocks = ceil(width / 32), the even element of a pair in the low four bits,
+ * zeros past `width`; scales (rows, 4 * ceil(blocks / 4)) bytes, those past `blocks` are written as 0 and
+ * never used.  Both contiguous, codes 16-byte and scales 4-byte aligned.
+ */
+int flare_micro_quantize(const void *x, int type, long long rows, int width, long long stride, unsigned char *codes,
+                         unsigned char *scales, void *stream);
+/* The values that codes and scales stand for, rounded to `type`. */
+int flare_micro_dequantize(const unsigned char *codes, const unsigned char *scales, long long rows, int width, void *out,
+                           int type, long long stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,33 @@
+"""The ctypes mirrors of the operators' argument structs have the header's layout (CPU only)."""
+import ctypes
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from flare_b200 import _lib, _ops
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PAIRS = {"LookupArgs": "flare_lookup_args", "LookupGradArgs": "flare_lookup_grad_args"}
+VALUES = {"FLARE_F32": 0, "FLARE_F16": 1, "FLARE_BF16": 2, "FLARE_MICRO": _ops.MICRO, "FLARE_I32": 0, "FLARE_I64": 1}
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="needs a C compiler")
+def test_ctypes_structs_match_the_header(tmp_path):
+    lines, expect = ["#include <stddef.h>", "#include <stdio.h>", '#include "flare_b200.h"', "int main(void) {"], []
+    for py, c in PAIRS.items():
+        cls = getattr(_lib, py)
+        lines.append(f'    printf("%zu\\n", sizeof({c}));')
+        expect.append((f"sizeof({c})", ctypes.sizeof(cls)))
+        for name, _ in cls._fields_:
+            lines.append(f'    printf("%zu\\n", offsetof({c}, {name}));')
+            expect.append((f"{c}.{name}", getattr(cls, name).offset))
+    for name, value in VALUES.items():
+        lines.append(f'    printf("%d\\n", {name});')
+        expect.append((name, value))
+    src, exe = tmp_path / "probe.c", tmp_path / "probe"
+    src.write_text("\n".join(lines + ["    return 0;", "}"]) + "\n")
+    subprocess.run(["gcc", "-std=c11", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert [(w, v) for w, v in expect] == [(w, g) for (w, _), g in zip(expect, got)]
