@@ -88,6 +88,19 @@ class LookupGradArgs(ctypes.Structure):
                 ("index_type", ctypes.c_int), ("dout_type", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
+class RecurrenceArgs(ctypes.Structure):
+    _fields_ = [("gate", vp), ("x", vp), ("state", vp), ("offsets", vp), ("h", vp), ("last", vp), ("saved", vp),
+                ("dh", vp), ("dlast", vp), ("dgate", vp), ("dx", vp), ("dstate", vp), ("workspace", vp),
+                ("workspace_bytes", ll), ("seqs", ll), ("steps", ll), ("gate_s", ll), ("gate_t", ll), ("x_s", ll),
+                ("x_t", ll), ("h_s", ll), ("h_t", ll), ("dh_s", ll), ("dh_t", ll), ("dgate_s", ll), ("dgate_t", ll),
+                ("dx_s", ll), ("dx_t", ll), ("width", ctypes.c_int), ("groups", ctypes.c_int),
+                ("gate_type", ctypes.c_int), ("x_type", ctypes.c_int), ("offsets_type", ctypes.c_int),
+                ("reverse", ctypes.c_int)]
+
+
+RECURRENCE_SPAN = 16
+
+
 class Stats(ctypes.Structure):
     _fields_ = [("rays", ctypes.c_longlong), ("passes", ctypes.c_longlong), ("hits_composited", ctypes.c_longlong),
                 ("prim_tests", ctypes.c_longlong), ("node_visits", ctypes.c_longlong),
@@ -128,6 +141,10 @@ EXPORTS = {
     "flare_lookup": (ctypes.c_int, [ctypes.POINTER(LookupArgs), vp]),
     "flare_lookup_workspace": (ll, [ll, ll, ctypes.c_int]),
     "flare_lookup_backward": (ctypes.c_int, [ctypes.POINTER(LookupGradArgs), vp]),
+    "flare_recurrence_saved": (ll, [ll, ll, ctypes.c_int, ctypes.c_int]),
+    "flare_recurrence_workspace": (ll, [ctypes.POINTER(RecurrenceArgs), ctypes.c_int]),
+    "flare_recurrence_forward": (ctypes.c_int, [ctypes.POINTER(RecurrenceArgs), vp]),
+    "flare_recurrence_backward": (ctypes.c_int, [ctypes.POINTER(RecurrenceArgs), vp]),
     "flare_micro_quantize": (ctypes.c_int, [vp, ctypes.c_int, ll, ctypes.c_int, ll, vp, vp, vp]),
     "flare_micro_dequantize": (ctypes.c_int, [vp, vp, ll, ctypes.c_int, vp, ctypes.c_int, ll, vp]),
 }

@@ -397,6 +397,45 @@ long long flare_lookup_workspace(long long rows, long long n, int width);
 int flare_lookup_backward(const flare_lookup_grad_args *a, void *stream);
 
 /*
+ * Gated linear recurrence h_t = gate_t * h_{t-1} + x_t for `seqs` sequences of `width` channels, h before
+ * the first step = state (NULL: 0), in 32 bits.  `groups` gates per step, each shared by width / groups
+ * consecutive channels.  reverse != 0 runs every sequence from its last step to its first (front-to-back
+ * compositing: gate 1 - alpha, x = alpha c, from the last hit).
+ * Dense (offsets NULL): seqs sequences of `steps` steps, strides per sequence (_s) and per step (_t) in
+ * elements; channels and gates of a step are contiguous.  Packed: `steps` rows in all, sequence s the
+ * rows [offsets[s], offsets[s + 1]) (non-decreasing, within [0, steps]); _s strides are ignored; rows of
+ * no sequence are never read as steps and written as zeros.
+ * Forward writes last (seqs, width), the state after the last step, and if not NULL h and saved (what the
+ * backward needs: the state before every FLARE_RECURRENCE_SPAN-th step, flare_recurrence_saved floats).
+ * Backward reads gate, x, state, saved, dh (NULL: 0) and dlast (NULL: 0) and writes dgate, dx and, if not
+ * NULL, dstate.  workspace: flare_recurrence_workspace bytes, 16-byte aligned, contents irrelevant.
+ * A product of gates over a stretch of steps has to stay within the range of a float.
+ */
+#define FLARE_RECURRENCE_SPAN 16
+typedef struct flare_recurrence_args {
+    const void *gate, *x;
+    const float *state;
+    const void *offsets;          /* (seqs + 1) or NULL */
+    void *h;
+    float *last, *saved;
+    const void *dh;
+    const float *dlast;
+    void *dgate, *dx;
+    float *dstate;
+    void *workspace;
+    long long workspace_bytes;
+    long long seqs, steps;
+    long long gate_s, gate_t, x_s, x_t, h_s, h_t, dh_s, dh_t, dgate_s, dgate_t, dx_s, dx_t;
+    int width, groups;
+    int gate_type, x_type;        /* x, h, dh, dx: x_type; gate, dgate: gate_type, either x_type or FLARE_F32 */
+    int offsets_type, reverse;
+} flare_recurrence_args;
+long long flare_recurrence_saved(long long seqs, long long steps, int width, int packed);
+long long flare_recurrence_workspace(const flare_recurrence_args *a, int backward);
+int flare_recurrence_forward(const flare_recurrence_args *a, void *stream);
+int flare_recurrence_backward(const flare_recurrence_args *a, void *stream);
+
+/*
  * Microscaled 4-bit storage: blocks of 32 consecutive elements of a row share a power-of-two scale 2^e, e =
  * floor(log2 of the block's largest magnitude) - 2 clamped to [-127, 127], held as the byte e + 127 (0 for a
  * block of zeros); each element is the 4-bit float (1 sign, 2 exponent, 1 mantissa bit: 0 .5 1 1.5 2 3 4 6)
