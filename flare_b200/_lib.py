@@ -101,6 +101,12 @@ class RecurrenceArgs(ctypes.Structure):
 RECURRENCE_SPAN = 16
 
 
+class ProductArgs(ctypes.Structure):
+    _fields_ = [("a_codes", vp), ("a_scales", vp), ("b_codes", vp), ("b_scales", vp), ("out", vp), ("workspace", vp),
+                ("status", vp), ("m", ll), ("n", ll), ("out_stride", ll), ("workspace_bytes", ll), ("k", ctypes.c_int),
+                ("out_type", ctypes.c_int)]
+
+
 class Stats(ctypes.Structure):
     _fields_ = [("rays", ctypes.c_longlong), ("passes", ctypes.c_longlong), ("hits_composited", ctypes.c_longlong),
                 ("prim_tests", ctypes.c_longlong), ("node_visits", ctypes.c_longlong),
@@ -147,6 +153,8 @@ EXPORTS = {
     "flare_recurrence_backward": (ctypes.c_int, [ctypes.POINTER(RecurrenceArgs), vp]),
     "flare_micro_quantize": (ctypes.c_int, [vp, ctypes.c_int, ll, ctypes.c_int, ll, vp, vp, vp]),
     "flare_micro_dequantize": (ctypes.c_int, [vp, vp, ll, ctypes.c_int, vp, ctypes.c_int, ll, vp]),
+    "flare_micro_product_workspace": (ll, [ll, ll, ctypes.c_int]),
+    "flare_micro_product": (ctypes.c_int, [ctypes.POINTER(ProductArgs), vp]),
 }
 
 _lib = None

@@ -1,8 +1,9 @@
-"""Matrices held in 4 bits an element with a power-of-two scale per 32 (microscaled 4-bit floats), written and read.
+"""Matrices held in 4 bits an element with a power-of-two scale per 32 (microscaled 4-bit floats), and their product.
 
 A 96-wide f16 descriptor takes 192 of the 312 bytes that a hit reads; held here it takes 52.  `quantize` makes a `Micro4`
 from a tensor, `Micro4.dequantize` and `embedding.lookup` read it back, the renderer's inference methods take one as
-`conditioning_variable`.  Inference only: none of them has a gradient.  No reference counterpart.
+`conditioning_variable`, and `product` multiplies two of them on the tensor cores.  Inference only: none of them has a
+gradient.  No reference counterpart.
 """
 from __future__ import annotations
 
@@ -81,3 +82,35 @@ def quantize(x) -> Micro4:
         _lib.check(lib.flare_micro_quantize(_ops.ptr(x), _ops.TYPE_CODE[x.dtype], rows, width, x.stride(0),
                                             _ops.ptr(codes), _ops.ptr(scales), _ops.stream(x.device)), "quantize")
     return Micro4(codes, scales, width)
+
+
+def product(x, w: Micro4, dtype=torch.bfloat16, check=False):
+    """x (m, k) times the transpose of w (n, k): a new (m, n) tensor of f32, f16 or bf16, accumulated in 32 bits.
+
+    x: a `Micro4`, or a tensor that is quantized first.  check: wait for the product and raise FlareError if a wait
+    inside the kernel ran out (without it such a tile is NaN).
+    """
+    lib = _lib.load()
+    if not isinstance(w, Micro4):
+        raise ValueError(f"w: expected a Micro4, got {type(w).__name__}")
+    if not isinstance(x, Micro4):
+        _ops.need(x, "x", _FLOATS, w.device)
+        x = quantize(x)
+    if dtype not in _ops.TYPE_CODE:
+        raise ValueError(f"dtype: {dtype}, expected one of {', '.join(str(d) for d in _FLOATS)}")
+    if x.width != w.width:
+        raise ValueError(f"x has {x.width} columns, w has {w.width}")
+    if x.device != w.device:
+        raise ValueError(f"w: tensor on {w.device}, expected {x.device}")
+    (m, k), n = x.shape, w.shape[0]
+    with _ops.on(x.device):
+        out = torch.empty((m, n), dtype=dtype, device=x.device)
+        ws = _ops.workspace(lib.flare_micro_product_workspace(m, n, k), x.device)
+        status = torch.zeros(1, dtype=torch.int32, device=x.device) if check else None
+        a = _lib.ProductArgs(_ops.ptr(x.codes), _ops.ptr(x.scales), _ops.ptr(w.codes), _ops.ptr(w.scales), _ops.ptr(out),
+                             _ops.ptr(ws), _ops.ptr(status), m, n, n, 0 if ws is None else ws.numel(), k,
+                             _ops.TYPE_CODE[dtype])
+        _lib.check(lib.flare_micro_product(ctypes.byref(a), _ops.stream(x.device)), "product")
+    if check and int(status):
+        raise _lib.FlareError(f"product: device reported error bits 0x{int(status):x} (tensor-core wait timeout)")
+    return out

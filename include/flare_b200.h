@@ -451,6 +451,22 @@ int flare_micro_quantize(const void *x, int type, long long rows, int width, lon
 int flare_micro_dequantize(const unsigned char *codes, const unsigned char *scales, long long rows, int width, void *out,
                            int type, long long stride, void *stream);
 
+/*
+ * out (m, n) = A (m, k) B (n, k)^T of two 4-bit matrices, accumulated in 32 bits on the tensor cores.
+ * workspace: flare_micro_product_workspace bytes, 16-byte aligned, contents irrelevant.  status (optional, a
+ * device int) gets a FLARE error bit OR-ed in if a wait inside the kernel ran out; the tile concerned is NaN.
+ */
+typedef struct flare_product_args {
+    const unsigned char *a_codes, *a_scales, *b_codes, *b_scales;
+    void *out;
+    void *workspace;
+    int *status;
+    long long m, n, out_stride, workspace_bytes;
+    int k, out_type;
+} flare_product_args;
+long long flare_micro_product_workspace(long long m, long long n, int k);
+int flare_micro_product(const flare_product_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

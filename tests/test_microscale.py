@@ -1,4 +1,6 @@
 """Microscaled 4-bit matrices: quantisation, values, lookup and product against a 64-bit restatement (GPU), refusals (CPU)."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -83,6 +85,97 @@ def test_lookup_reads_a_4_bit_table(width, out):
         embedding.lookup_backward(got, q, idx.to(DEV))
 
 
+def _product(m, n, k, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    a, b = ((torch.randn(r, k, generator=g) * torch.exp(spread * torch.randn(r, 1, generator=g))).to(DEV) for r in (m, n))
+    qa, qb = microscale.quantize(a), microscale.quantize(b)
+    va, vb = (ref.values(q.codes.cpu().numpy(), q.scales.cpu().numpy(), k) for q in (qa, qb))
+    # products are exact; an addition may truncate (a whole step of 2^-23) what it adds to sums of magnitudes
+    return qa, qb, va @ vb.T, (k + 2) * 2 * ref.U * (np.abs(va) @ np.abs(vb).T)
+
+
+SIZES = [(1, 1, 1), (1, 1, 33), (3, 5, 64), (128, 128, 256), (129, 64, 96), (1, 300, 500), (300, 1, 4000), (200, 260, 1000),
+         (130, 513, 31), (4, 1000, 4096), (1000, 7, 128), (257, 129, 2049), (5, 2000, 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [F32, F16, BF16])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_product(m, n, k, out):
+    qa, qb, want, err = _product(m, n, k, spread=0.3)
+    got = microscale.product(qa, qb, dtype=out, check=True)
+    assert got.dtype == out
+    ref.close(got, want, err)
+    assert torch.equal(got, microscale.product(qa, qb, dtype=out))
+
+
+@pytest.mark.gpu
+def test_product_of_whole_numbers_is_exact():
+    """Codes and scales whose products and sums are small whole numbers: any order and any place of an element that is
+    taken wrongly shows."""
+    g = torch.Generator().manual_seed(5)
+    for m, n, k in ((300, 280, 520), (2, 700, 1030), (513, 64, 96)):
+        lev = torch.tensor([0.0, 1.0, 2.0, 3.0, 4.0, -1.0, -2.0])
+        a, b = lev[torch.randint(0, 7, (m, k), generator=g)], lev[torch.randint(0, 7, (n, k), generator=g)]
+        for t in (a, b):
+            t[:, ::32] = 4.0  # every block's scale is 1 ...
+            for c in range(0, k, 32):  # ... times a power of two that differs from block to block and row to row
+                t[:, c:c + 32] *= 2.0 ** ((torch.arange(t.shape[0])[:, None] + c // 32) % 3).float()
+        got = microscale.product(a.to(DEV), microscale.quantize(b.to(DEV)), dtype=F32)
+        assert torch.equal(got.cpu(), a @ b.T)
+
+
+@pytest.mark.gpu
+def test_product_of_a_tensor_quantizes_it():
+    g = torch.Generator().manual_seed(3)
+    x, w = torch.randn(50, 70, generator=g).to(DEV).half(), microscale.quantize(torch.randn(30, 70, generator=g).to(DEV))
+    assert torch.equal(microscale.product(x, w), microscale.product(microscale.quantize(x), w))
+    wide = torch.randn(50, 100, generator=g).to(DEV)
+    assert torch.equal(microscale.product(wide[:, 7:77], w), microscale.product(wide[:, 7:77].contiguous(), w))
+
+
+@pytest.mark.gpu
+def test_product_passes_nan_and_range():
+    a, b = torch.randn(140, 96), torch.randn(33, 96)
+    a[3, 40], b[7, 70] = float("nan"), float("inf")
+    got = microscale.product(a.to(DEV), microscale.quantize(b.to(DEV)), dtype=F32).cpu()
+    want = torch.zeros(140, 33, dtype=torch.bool)
+    want[3], want[:, 7] = True, True
+    assert torch.equal(torch.isnan(got), want)
+    big = microscale.quantize(torch.full((2, 32), 2.0 ** 100, device=DEV))
+    assert torch.isinf(microscale.product(big, big, dtype=F32)).all()
+    half = microscale.quantize(torch.full((2, 32), 2.0 ** 10, device=DEV))
+    assert torch.isinf(microscale.product(half, half, dtype=F16)).all()
+    assert (microscale.product(half, half, dtype=F32) == 2.0 ** 25).all()
+
+
+@pytest.mark.gpu
+def test_product_of_nothing():
+    none, some = microscale.quantize(torch.zeros(0, 40, device=DEV)), microscale.quantize(torch.ones(3, 40, device=DEV))
+    assert microscale.product(none, some).shape == (0, 3) and microscale.product(some, none).shape == (3, 0)
+    assert none.dequantize().shape == (0, 40)
+
+
+@pytest.mark.gpu
+def test_on_another_stream_and_in_a_graph():
+    x, w = torch.randn(200, 512, device=DEV).bfloat16(), microscale.quantize(torch.randn(300, 512, device=DEV))
+    want = microscale.product(x, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = microscale.product(x, w)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = microscale.product(x, w)
+        back = microscale.quantize(x).dequantize()
+    x.mul_(2.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want * 2) and torch.equal(back, microscale.quantize(x).dequantize())
+
+
 def test_refusals():
     with pytest.raises(ValueError, match="CUDA"):
         microscale.quantize(torch.zeros(2, 3))
@@ -90,15 +183,18 @@ def test_refusals():
         microscale.quantize(torch.zeros(2, 3, dtype=torch.float64))
     with pytest.raises(ValueError, match="codes"):
         microscale.Micro4(torch.zeros(2, 3), torch.zeros(2, 4), 3)
+    with pytest.raises(ValueError, match="Micro4"):
+        microscale.product(torch.zeros(2, 3), torch.zeros(2, 3))
 
 
 @pytest.mark.gpu
 def test_refusals_on_the_device():
     q = microscale.quantize(torch.ones(4, 40, device=DEV))
+    other = microscale.quantize(torch.ones(4, 41, device=DEV))
     for bad in (lambda: microscale.quantize(torch.ones(4, device=DEV)), lambda: microscale.quantize(torch.ones(4, 0, device=DEV)),
-                lambda: q.dequantize(torch.float64),
+                lambda: q.dequantize(torch.float64), lambda: microscale.product(q, other), lambda: microscale.product(q, q, dtype=torch.int8),
                 lambda: microscale.Micro4(q.codes, q.scales, 65), lambda: microscale.Micro4(q.codes[:2], q.scales, 40),
-                lambda: microscale.Micro4(q.codes[:, :16], q.scales, 32)):
+                lambda: microscale.Micro4(q.codes[:, :16], q.scales, 32), lambda: microscale.product(torch.ones(2, 39, device=DEV), q)):
         with pytest.raises(ValueError):
             bad()
 
@@ -109,3 +205,10 @@ def test_c_entry_refuses_bad_arguments():
     assert lib.flare_micro_quantize(None, 3, 1, 4, 4, None, None, None) == 1 and b"type" in lib.flare_last_error()
     assert lib.flare_micro_dequantize(None, None, 1, 0, None, 0, 4, None) == 1
     assert lib.flare_micro_dequantize(16, 16, 1, 8, 16, 0, 4, None) == 1 and b"overlap" in lib.flare_last_error()
+    assert lib.flare_micro_product(None, None) == 1
+    a = _lib.ProductArgs(m=1, n=1, k=0)
+    assert lib.flare_micro_product(ctypes.byref(a), None) == 1
+    a = _lib.ProductArgs(m=1, n=1, k=32, out_stride=1)
+    assert lib.flare_micro_product(ctypes.byref(a), None) == 1 and b"NULL" in lib.flare_last_error()
+    a = _lib.ProductArgs(m=1, n=1, k=32, out_stride=1, a_codes=8, b_codes=16, a_scales=16, b_scales=16, out=16)
+    assert lib.flare_micro_product(ctypes.byref(a), None) == 1 and b"aligned" in lib.flare_last_error()
