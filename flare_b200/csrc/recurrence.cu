@@ -20,8 +20,9 @@
 namespace flare {
 
 constexpr int SPAN = FLARE_RECURRENCE_SPAN;
-constexpr int MAX_W = 8;        // warps per block along time
-constexpr int MAX_SPLITS = 64;  // blocks along time
+constexpr int WARPS = 8;         // warps per block: W along time times WARPS / W tiles of channels
+constexpr int MAX_SPLITS = 128;  // blocks along time
+constexpr int SUM_STRIDE = 33;   // row stride of a warp's 16 x 32 products, off the banks' 32
 
 struct RecArgs {
     const void *gate, *x, *dh, *offsets;
@@ -30,125 +31,115 @@ struct RecArgs {
     float *last, *saved, *dstate;
     float *agg;      // (splits, 2, seqs * width)
     float *partial;  // (parts, rows, groups): sums over parts of a group's channels
-    long long seqs, steps, rows;
+    long long seqs, rows;
     long long gate_s, gate_t, x_s, x_t, h_s, h_t, dh_s, dh_t, dgate_s, dgate_t, dx_s, dx_t;
-    int width, groups, share;  // share: channels per gate
+    int steps, width, groups;
+    FastDiv share;             // channels per gate
     int off64, reverse, packed;
-    int splits;
-    unsigned units;            // lanes' worth of channels: seqs * width / VE
+    int warps, splits, per;    // W; dense: steps per split
+    unsigned tiles, units;     // units: lanes' worth of channels, seqs * width / VE
     FastDiv upr;               // units per sequence
     int group_units, groups_per_tile, parts;  // backward tiles of whole groups, see Place
-    long long spans;           // dense: spans per sequence
+    int spans;                 // dense: spans per sequence
 };
 
-__device__ __forceinline__ long long offset_at(const RecArgs &a, long long s) {
+__device__ __forceinline__ int offset_at(const RecArgs &a, long long s) {
     const long long o = a.off64 ? __ldg(static_cast<const long long *>(a.offsets) + s) : (long long)__ldg(static_cast<const int *>(a.offsets) + s);
-    return min(max(o, 0ll), a.steps);
+    return (int)min(max(o, 0ll), (long long)a.steps);
 }
 
 // Where a lane's channels lie.  GROUPED: tiles consist of whole groups of channels that share a gate, or of a part of
-// one such group (32 lanes at a time), so that sums over a group need no other block.
+// one such group (32 lanes at a time), so that sums over a group need no other warp.
 template <int VE, bool GROUPED>
 struct Place {
     bool active;
-    long long seq, row0, len;  // row0: first row of the sequence in memory terms (packed), len: its steps
-    int c;                     // first channel
-    long long chain;           // seq * width + c
-    int pos, part;
+    int seq, row0, len;  // row0: the sequence's first row (packed), len: its steps
+    int c;               // first channel
+    unsigned chain;      // seq * width + c
+    int part, leader;    // GROUPED: part of the group, lane of the group's first channel in this warp
     __device__ __forceinline__ Place(const RecArgs &a, unsigned tile) {
         const int lane = threadIdx.x & 31;
         unsigned u;
+        part = 0;
+        leader = 0;
         if (!GROUPED) {
             u = tile * 32 + lane;
-            active = u < a.units;
-            pos = part = 0;
+            active = tile < a.tiles && u < a.units;
         } else if (a.parts == 1) {
             const unsigned g = lane / a.group_units;
-            pos = lane - g * a.group_units;
-            u = (tile * a.groups_per_tile + g) * a.group_units + pos;
-            active = (int)g < a.groups_per_tile && u < a.units;
-            part = 0;
+            leader = g * a.group_units;
+            u = (tile * a.groups_per_tile + g) * a.group_units + lane - leader;
+            active = tile < a.tiles && (int)g < a.groups_per_tile && u < a.units;
         } else {
             part = tile % a.parts;
-            pos = part * 32 + lane;
+            const int pos = part * 32 + lane;
             u = tile / a.parts * a.group_units + pos;
-            active = pos < a.group_units;
+            active = tile < a.tiles && pos < a.group_units;
         }
         if (!active) u = 0;
-        const unsigned s = a.upr.div(u);
-        seq = s;
-        c = (int)(u - s * a.upr.d) * VE;
-        chain = seq * a.width + c;
+        seq = (int)a.upr.div(u);
+        c = (int)(u - seq * a.upr.d) * VE;
+        chain = u * VE;
         row0 = 0;
         len = a.steps;
-        if (a.packed) {
+        if (!active) {
+            len = 0;
+        } else if (a.packed) {
             row0 = offset_at(a, seq);
-            len = max(offset_at(a, seq + 1) - row0, 0ll);
+            len = max(offset_at(a, seq + 1) - row0, 0);
         }
-        if (!active) len = 0;
     }
-    // element offset of step 0's row in a tensor and the distance to the next step's
+    // element offset of the first step's row in a tensor (the next step's is stride_t further on, or before if reversed)
     __device__ __forceinline__ long long first(const RecArgs &a, long long stride_s, long long stride_t) const {
         const long long base = a.packed ? row0 * stride_t : seq * stride_s;
-        return base + (a.reverse ? (len - 1) * stride_t : 0);
+        return a.reverse ? base + (len - 1) * stride_t : base;
     }
     // row of `saved` that holds the state before span k >= 1
-    __device__ __forceinline__ long long saved_row(const RecArgs &a, long long k) const {
-        return a.packed ? row0 / SPAN + seq + k : seq * (a.spans - 1) + k - 1;
+    __device__ __forceinline__ long long saved_row(const RecArgs &a, int k) const {
+        return a.packed ? (long long)row0 / SPAN + seq + k : (long long)seq * (a.spans - 1) + k - 1;
+    }
+    // the steps that block `split` works on, in whole rounds of W spans
+    __device__ __forceinline__ void range(const RecArgs &a, int split, int &t0, int &t1) const {
+        t0 = 0;
+        t1 = len;
+        if (a.splits > 1) {
+            unsigned per = a.per;
+            if (a.packed) {
+                const unsigned round = a.warps * SPAN, rounds = ((unsigned)len + round - 1) / round;
+                per = (rounds + a.splits - 1) / a.splits * round;
+            }
+            t0 = (int)min((long long)len, (long long)split * per);
+            t1 = (int)min((long long)len, (long long)t0 + per);
+        }
     }
 };
-
-// the steps of a lane that block `split` of a.splits works on, in whole rounds of W spans
-__device__ __forceinline__ void split_range(const RecArgs &a, long long len, int W, int split, long long &t0, long long &t1) {
-    const long long round = (long long)W * SPAN;
-    const long long rounds = (len + round - 1) / round;
-    const long long per = (rounds + a.splits - 1) / a.splits * round;
-    t0 = min(len, split * per);
-    t1 = min(len, t0 + per);
-}
-
-__device__ __forceinline__ long long warp_max(long long v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 
 // What a stretch (A, H) makes of the state c.  A state of exactly 0 adds nothing, also where the product of the gates
 // has left the range of a float.
 __device__ __forceinline__ float through(float A, float H, float c) { return c == 0.0f ? H : fmaf(A, c, H); }
 
-// A lane's gates of one span: one per channel, or one for all its channels.
-template <class GT, int VE, bool SHARED>
-struct Gates {
-    static constexpr int N = SHARED ? 1 : VE;
-    Vec<GT, N> g[SPAN];
-    __device__ __forceinline__ void load(const GT *p, long long step, long long n) {
+// SPAN steps of N channels as they lie in memory, the ones past n filled with `rest`.
+template <class T, int N>
+struct Span {
+    Vec<T, N> d[SPAN];
+    // KEEP: others read it again soon
+    template <bool KEEP>
+    __device__ __forceinline__ void load(const T *p, long long step, int n, float rest) {
 #pragma unroll
-        for (int i = 0; i < SPAN; ++i) {
-            if (i < n) g[i].load(p + i * step);
+        for (int i = 0; i < SPAN; ++i, p += step) {
+            if (i < n && KEEP) d[i].load(p);
+            else if (i < n) d[i].load_stream(p);
             else
 #pragma unroll
-                for (int v = 0; v < N; ++v) g[i].set(v, 1.0f);
+                for (int v = 0; v < N; ++v) d[i].set(v, rest);
         }
     }
-    __device__ __forceinline__ float at(int i, int v) const { return g[i].get(SHARED ? 0 : v); }
-};
-
-template <class T, int VE>
-struct Span {
-    Vec<T, VE> d[SPAN];
-    __device__ __forceinline__ void load(const T *p, long long step, long long n) {
-#pragma unroll
-        for (int i = 0; i < SPAN; ++i) {
-            if (i < n) d[i].load(p + i * step);
-            else d[i].zero();
-        }
-    }
+    __device__ __forceinline__ float at(int i, int v) const { return d[i].get(N == 1 ? 0 : v); }
 };
 
 // (A, H) of a span, walked from its first step (forward) or its last (backward, where H collects a_t dh_t)
-template <bool BACK, class T, class GT, int VE, bool SHARED>
-__device__ __forceinline__ void stretch(const Gates<GT, VE, SHARED> &g, const Span<T, VE> &x, float (&A)[VE], float (&H)[VE]) {
+template <bool BACK, class T, class GT, int VE, int GN>
+__device__ __forceinline__ void stretch(const Span<GT, GN> &g, const Span<T, VE> &x, float (&A)[VE], float (&H)[VE]) {
 #pragma unroll
     for (int v = 0; v < VE; ++v) {
         A[v] = 1.0f;
@@ -160,26 +151,33 @@ __device__ __forceinline__ void stretch(const Gates<GT, VE, SHARED> &g, const Sp
 #pragma unroll
         for (int v = 0; v < VE; ++v) {
             const float a = g.at(i, v);
-            H[v] = BACK ? a * (H[v] + x.d[i].get(v)) : fmaf(a, H[v], x.d[i].get(v));
+            H[v] = BACK ? a * (H[v] + x.at(i, v)) : fmaf(a, H[v], x.at(i, v));
             A[v] *= a;
         }
     }
 }
 
-// The state that enters warp w's span, from the state `carry` that enters the round; carry becomes what leaves the round.
-// BACK: warps are passed from the last to the first.  buf: (2, W, 32 VE) floats, not the one of the round before.
+// barrier of the W warps that share a tile
+__device__ __forceinline__ void tile_sync(int W) {
+    const int id = 1 + (threadIdx.x >> 5) / W;
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 * W) : "memory");
+}
+
+// The state that enters warp w's stretch, from the state `carry` that enters all W of them; carry becomes what leaves them.
+// BACK: warps are passed from the last to the first.  buf: (2, W, 32 VE) floats, not the one of the call before.
 template <bool BACK, int VE>
 __device__ __forceinline__ void exchange(float *buf, int W, const float (&A)[VE], const float (&H)[VE], float (&carry)[VE], float (&in)[VE]) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1);
     float *sa = buf, *sh = buf + W * 32 * VE;
 #pragma unroll
     for (int v = 0; v < VE; ++v) {
         sa[(w * VE + v) * 32 + lane] = A[v];
         sh[(w * VE + v) * 32 + lane] = H[v];
     }
-    __syncthreads();
+    tile_sync(W);
 #pragma unroll
     for (int v = 0; v < VE; ++v) in[v] = carry[v];
+#pragma unroll 4
     for (int k = 0; k < W; ++k) {
         const int o = BACK ? W - 1 - k : k;
 #pragma unroll
@@ -190,51 +188,110 @@ __device__ __forceinline__ void exchange(float *buf, int W, const float (&A)[VE]
     }
 }
 
-// state entering block `split`: `c` through the blocks that come before it in the walk
+// The state that enters block `split`: `c` through the blocks before it in the walk.  Each of the W warps joins a
+// part of them, then the parts are passed in order.
 template <bool BACK, int VE>
-__device__ __forceinline__ void fold_splits(const RecArgs &a, long long chain, int split, float (&c)[VE]) {
+__device__ __forceinline__ void fold_splits(const RecArgs &a, unsigned chain, int split, float *buf, float (&c)[VE]) {
     const long long chains = a.seqs * a.width;
+    const int W = a.warps, w = (threadIdx.x >> 5) & (W - 1);
     const int n = BACK ? a.splits - 1 - split : split;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-        const int o = BACK ? a.splits - 1 - k : k;
-        const float *p = a.agg + (long long)o * 2 * chains + chain;
+    if (n == 0) return;
+    // parts in the order of the walk: warp w (BACK: W - 1 - w) has the w-th
+    const int k0 = n * (BACK ? W - 1 - w : w) / W, k1 = n * (BACK ? W - w : w + 1) / W;
+    float A[VE], H[VE], unused[VE];
 #pragma unroll
-        for (int v = 0; v < VE; ++v) c[v] = through(__ldg(p + v), __ldg(p + chains + v), c[v]);
+    for (int v = 0; v < VE; ++v) {
+        A[v] = 1.0f;
+        H[v] = 0.0f;
+    }
+#pragma unroll 4
+    for (int k = k0; k < k1; ++k) {
+        const float *p = a.agg + (long long)(BACK ? a.splits - 1 - k : k) * 2 * chains + chain;
+        Vec<float, VE> pa, ph;
+        pa.load(p);
+        ph.load(p + chains);
+#pragma unroll
+        for (int v = 0; v < VE; ++v) {
+            H[v] = through(pa.get(v), ph.get(v), H[v]);
+            A[v] *= pa.get(v);
+        }
+    }
+    if (W > 1) {
+        exchange<BACK>(buf, W, A, H, c, unused);
+        tile_sync(W);  // the rounds that follow use the buffer again
+    } else {
+#pragma unroll
+        for (int v = 0; v < VE; ++v) c[v] = through(A[v], H[v], c[v]);
     }
 }
 
-// BACK false: (A, H) of x; true: of dh, from the end.  grid (tiles, splits)
+template <int VE>
+__device__ __forceinline__ void load_ends(const float *p, unsigned chain, bool some, float (&f)[VE]) {
+    Vec<float, VE> v;
+    if (p && some) v.load(p + chain);
+    else v.zero();
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = v.get(e);
+}
+template <int VE>
+__device__ __forceinline__ void store_ends(float *p, const float (&f)[VE]) {
+    Vec<float, VE> v;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v.el[e] = f[e];
+    v.store(p);
+}
+
+// zeros in the rows of a packed tensor that belong to no sequence, shared among all blocks
+template <class T>
+__device__ __forceinline__ void clear_rest(const RecArgs &a, void *out, long long stride, int width) {
+    const int tail = offset_at(a, a.seqs), head = min(offset_at(a, 0), tail);
+    const long long n = ((long long)head + a.steps - tail) * width;
+    const long long block = blockIdx.y * (long long)gridDim.x + blockIdx.x, blocks = (long long)gridDim.x * gridDim.y;
+    for (long long i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) {
+        const long long r = i / width;
+        static_cast<T *>(out)[(r < head ? r : tail + r - head) * stride + (i - r * width)] = from_f32<T>(0.0f);
+    }
+}
+
+__device__ __forceinline__ unsigned my_tile(const RecArgs &a) {
+    return blockIdx.x * (WARPS / a.warps) + (threadIdx.x >> 5) / a.warps;
+}
+// a tile's part of the exchange buffers: two of (2, W, 32 VE) floats
+template <int VE>
+__device__ __forceinline__ float *my_buffers(const RecArgs &a, float *smem) {
+    return smem + (threadIdx.x >> 5) / a.warps * (4 * a.warps * 32 * VE);
+}
+__device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// BACK false: (A, H) of x; true: of dh, from the end.  grid (tiles, splits); W > 1
 template <bool BACK, class T, class GT, int VE, bool SHARED>
-__global__ void __launch_bounds__(32 * MAX_W) recurrence_split_kernel(const RecArgs a) {
-    extern __shared__ float smem[];
-    const int W = blockDim.x >> 5, lane = threadIdx.x & 31, w = threadIdx.x >> 5, split = blockIdx.y;
-    const Place<VE, false> me(a, blockIdx.x);
-    long long t0, t1;
-    split_range(a, me.len, W, split, t0, t1);
-    const long long span = warp_max(t1 - t0), round = (long long)W * SPAN;
-    const long long dir = a.reverse ? -1 : 1;
-    const void *src = BACK ? a.dh : a.x;
-    const long long src_s = BACK ? a.dh_s : a.x_s, src_t = BACK ? a.dh_t : a.x_t;
-    const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + me.c / a.share;
-    const T *xp = static_cast<const T *>(src) + me.first(a, src_s, src_t) + me.c;
+__global__ void __launch_bounds__(32 * WARPS) recurrence_split_kernel(const RecArgs a) {
+    extern __shared__ __align__(16) float smem[];
+    const int W = a.warps, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
+    const Place<VE, false> me(a, my_tile(a));
+    int t0, t1;
+    me.range(a, split, t0, t1);
+    float *bufs = my_buffers<VE>(a, smem);
+    const int round = W * SPAN, n = (warp_max(t1 - t0) + round - 1) / round;
+    const T *src = static_cast<const T *>(BACK ? a.dh : a.x);
+    const long long src_t = BACK ? a.dh_t : a.x_t;
+    const long long gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -src_t : src_t;
+    const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + a.share.div(me.c);
+    const T *xp = src + me.first(a, BACK ? a.dh_s : a.x_s, src_t) + me.c;
     float A[VE], H[VE], tA[VE], tH[VE], unused[VE];
 #pragma unroll
     for (int v = 0; v < VE; ++v) {
         tA[v] = 1.0f;
         tH[v] = 0.0f;
     }
-    const long long n = (span + round - 1) / round;
-    for (long long k = 0; k < n; ++k) {
-        const long long r = BACK ? n - 1 - k : k;
-        const long long t = t0 + r * round + w * SPAN, left = t1 - t;
-        Gates<GT, VE, SHARED> g;
+    for (int k = 0; k < n; ++k) {
+        const int t = t0 + (BACK ? n - 1 - k : k) * round + w * SPAN, left = t1 - t;
+        Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x;
-        g.load(gp + t * dir * a.gate_t, dir * a.gate_t, left);
-        if (src) x.load(xp + t * dir * src_t, dir * src_t, left);
-        else x.load(xp, 0, 0);
+        g.template load<true>(gp + t * gs, gs, left, 1.0f);
+        x.template load<true>(xp + t * xs, xs, src ? left : 0, 0.0f);
         stretch<BACK>(g, x, A, H);
-        float *buf = smem + (k & 1) * 2 * W * 32 * VE;
+        float *buf = bufs + (k & 1) * 2 * W * 32 * VE;
         exchange<BACK>(buf, W, A, H, tH, unused);
         // the product of the round's gates, in the same buffer
         for (int o = 0; o < W; ++o)
@@ -244,108 +301,102 @@ __global__ void __launch_bounds__(32 * MAX_W) recurrence_split_kernel(const RecA
     if (w == 0 && me.active) {
         const long long chains = a.seqs * a.width;
         float *p = a.agg + (long long)split * 2 * chains + me.chain;
-#pragma unroll
-        for (int v = 0; v < VE; ++v) {
-            p[v] = tA[v];
-            p[chains + v] = tH[v];
-        }
+        store_ends<VE>(p, tA);
+        store_ends<VE>(p + chains, tH);
     }
 }
 
 template <class T, class GT, int VE, bool SHARED>
-__global__ void __launch_bounds__(32 * MAX_W) recurrence_forward_kernel(const RecArgs a) {
-    extern __shared__ float smem[];
-    const int W = blockDim.x >> 5, w = threadIdx.x >> 5, split = blockIdx.y;
-    const Place<VE, false> me(a, blockIdx.x);
-    long long t0, t1;
-    split_range(a, me.len, W, split, t0, t1);
-    const long long span = warp_max(t1 - t0), round = (long long)W * SPAN;
-    const long long dir = a.reverse ? -1 : 1;
-    const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + me.c / a.share;
+__global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const RecArgs a) {
+    extern __shared__ __align__(16) float smem[];
+    const int W = a.warps, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
+    const Place<VE, false> me(a, my_tile(a));
+    int t0, t1;
+    me.range(a, split, t0, t1);
+    float *bufs = my_buffers<VE>(a, smem);
+    const int round = W * SPAN, n = (warp_max(t1 - t0) + round - 1) / round;
+    const long long gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t, hs = a.reverse ? -a.h_t : a.h_t;
+    const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + a.share.div(me.c);
     const T *xp = static_cast<const T *>(a.x) + me.first(a, a.x_s, a.x_t) + me.c;
-    T *hp = a.h ? static_cast<T *>(a.h) + me.first(a, a.h_s, a.h_t) + me.c : nullptr;
+    T *hp = static_cast<T *>(a.h) + me.first(a, a.h_s, a.h_t) + me.c;
     float carry[VE], h[VE], A[VE], H[VE];
-#pragma unroll
-    for (int v = 0; v < VE; ++v) carry[v] = me.active && a.state ? a.state[me.chain + v] : 0.0f;
-    if (me.active) fold_splits<false, VE>(a, me.chain, split, carry);
-    const long long n = (span + round - 1) / round;
-    for (long long k = 0; k < n; ++k) {
-        const long long t = t0 + k * round + w * SPAN, left = t1 - t;
-        Gates<GT, VE, SHARED> g;
+    load_ends<VE>(a.state, me.chain, me.active, carry);
+    if (a.splits > 1) fold_splits<false, VE>(a, me.chain, split, bufs, carry);
+    for (int k = 0; k < n; ++k) {
+        const int t = t0 + k * round + w * SPAN, left = t1 - t;
+        Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x;
-        g.load(gp + t * dir * a.gate_t, dir * a.gate_t, left);
-        x.load(xp + t * dir * a.x_t, dir * a.x_t, left);
+        g.template load<SHARED>(gp + t * gs, gs, left, 1.0f);
+        x.template load<false>(xp + t * xs, xs, left, 0.0f);
         if (W > 1) {
             stretch<false>(g, x, A, H);
-            exchange<false>(smem + (k & 1) * 2 * W * 32 * VE, W, A, H, carry, h);
+            exchange<false>(bufs + (k & 1) * 2 * W * 32 * VE, W, A, H, carry, h);
         } else {
 #pragma unroll
             for (int v = 0; v < VE; ++v) h[v] = carry[v];
         }
-        if (a.saved && left > 0 && t > 0) {
-            float *p = a.saved + me.saved_row(a, t / SPAN) * a.width + me.c;
+        if (a.saved && left > 0 && t > 0) store_ends<VE>(a.saved + me.saved_row(a, t / SPAN) * a.width + me.c, h);
+        if (a.h) {
+            T *p = hp + t * hs;
 #pragma unroll
-            for (int v = 0; v < VE; ++v) p[v] = h[v];
-        }
+            for (int i = 0; i < SPAN; ++i, p += hs) {
+                Vec<T, VE> o;
 #pragma unroll
-        for (int i = 0; i < SPAN; ++i) {
-            Vec<T, VE> o;
-#pragma unroll
-            for (int v = 0; v < VE; ++v) {
-                h[v] = fmaf(g.at(i, v), h[v], x.d[i].get(v));
-                o.set(v, h[v]);
+                for (int v = 0; v < VE; ++v) {
+                    h[v] = fmaf(g.at(i, v), h[v], x.at(i, v));
+                    o.set(v, h[v]);
+                }
+                if (i < left) o.store_stream(p);
             }
-            if (hp && i < left) o.store(hp + (t + i) * dir * a.h_t);
+        } else {
+#pragma unroll
+            for (int i = 0; i < SPAN; ++i)
+#pragma unroll
+                for (int v = 0; v < VE; ++v) h[v] = fmaf(g.at(i, v), h[v], x.at(i, v));
         }
         if (W == 1)
 #pragma unroll
             for (int v = 0; v < VE; ++v) carry[v] = h[v];
     }
-    if (w == 0 && split == a.splits - 1 && me.active)
-#pragma unroll
-        for (int v = 0; v < VE; ++v) a.last[me.chain + v] = carry[v];
+    if (w == 0 && split == a.splits - 1 && me.active) store_ends<VE>(a.last + me.chain, carry);
+    if (a.packed && a.h) clear_rest<T>(a, a.h, a.h_t, a.width);
 }
 
+// smem: the exchange buffers, then SHARED: 16 x 32 products per warp
 template <class T, class GT, int VE, bool SHARED>
-__global__ void __launch_bounds__(32 * MAX_W) recurrence_backward_kernel(const RecArgs a) {
-    extern __shared__ float smem[];
-    const int W = blockDim.x >> 5, w = threadIdx.x >> 5, split = blockIdx.y;
-    const Place<VE, SHARED> me(a, blockIdx.x);
-    long long t0, t1;
-    split_range(a, me.len, W, split, t0, t1);
-    const long long span = warp_max(t1 - t0), round = (long long)W * SPAN;
-    const long long dir = a.reverse ? -1 : 1;
-    const int gc = me.c / a.share;
+__global__ void __launch_bounds__(32 * WARPS) recurrence_backward_kernel(const RecArgs a) {
+    extern __shared__ __align__(16) float smem[];
+    const int W = a.warps, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
+    const Place<VE, SHARED> me(a, my_tile(a));
+    int t0, t1;
+    me.range(a, split, t0, t1);
+    float *bufs = my_buffers<VE>(a, smem);
+    float *sums = smem + (W > 1 ? 4 * WARPS * 32 * VE : 0) + (threadIdx.x >> 5) * (SPAN * SUM_STRIDE);
+    const int round = W * SPAN, n = (warp_max(t1 - t0) + round - 1) / round;
+    const int gc = (int)a.share.div(me.c);
+    const long long gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t;
+    const long long dhs = a.reverse ? -a.dh_t : a.dh_t, dxs = a.reverse ? -a.dx_t : a.dx_t, dgs = a.reverse ? -a.dgate_t : a.dgate_t;
     const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + gc;
     const T *xp = static_cast<const T *>(a.x) + me.first(a, a.x_s, a.x_t) + me.c;
-    const T *dhp = a.dh ? static_cast<const T *>(a.dh) + me.first(a, a.dh_s, a.dh_t) + me.c : nullptr;
+    const T *dhp = static_cast<const T *>(a.dh) + me.first(a, a.dh_s, a.dh_t) + me.c;
     T *dxp = static_cast<T *>(a.dx) + me.first(a, a.dx_s, a.dx_t) + me.c;
     GT *dgp = static_cast<GT *>(a.dgate) + me.first(a, a.dgate_s, a.dgate_t) + gc;
     float carry[VE], mu[VE], A[VE], H[VE];
-#pragma unroll
-    for (int v = 0; v < VE; ++v) carry[v] = me.active && a.dlast ? a.dlast[me.chain + v] : 0.0f;
-    if (me.active) fold_splits<true, VE>(a, me.chain, split, carry);
-    const long long n = (span + round - 1) / round;
-    for (long long k = 0; k < n; ++k) {
-        const long long t = t0 + (n - 1 - k) * round + w * SPAN, left = t1 - t;
-        Gates<GT, VE, SHARED> g;
+    load_ends<VE>(a.dlast, me.chain, me.active, carry);
+    if (a.splits > 1) fold_splits<true, VE>(a, me.chain, split, bufs, carry);
+    for (int k = 0; k < n; ++k) {
+        const int t = t0 + (n - 1 - k) * round + w * SPAN, left = t1 - t;
+        Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x, dh;
-        g.load(gp + t * dir * a.gate_t, dir * a.gate_t, left);
-        if (dhp) dh.load(dhp + t * dir * a.dh_t, dir * a.dh_t, left);
-        else dh.load(xp, 0, 0);
-        x.load(xp + t * dir * a.x_t, dir * a.x_t, left);
+        g.template load<SHARED>(gp + t * gs, gs, left, 1.0f);
+        dh.template load<false>(dhp + t * dhs, dhs, a.dh ? left : 0, 0.0f);
+        x.template load<false>(xp + t * xs, xs, left, 0.0f);
         float before[SPAN][VE];  // the state before each step
-#pragma unroll
-        for (int v = 0; v < VE; ++v) before[0][v] = 0.0f;
-        if (left > 0) {
-            const float *p = t > 0 ? a.saved + me.saved_row(a, t / SPAN) * a.width + me.c : a.state ? a.state + me.chain : nullptr;
-            if (p)
-#pragma unroll
-                for (int v = 0; v < VE; ++v) before[0][v] = p[v];
-        }
+        if (t > 0) load_ends<VE>(a.saved + me.saved_row(a, t / SPAN) * a.width, me.c, left > 0, before[0]);
+        else load_ends<VE>(a.state, me.chain, left > 0, before[0]);
         if (W > 1) {
             stretch<true>(g, dh, A, H);
-            exchange<true>(smem + (k & 1) * 2 * W * 32 * VE, W, A, H, carry, mu);
+            exchange<true>(bufs + (k & 1) * 2 * W * 32 * VE, W, A, H, carry, mu);
         } else {
 #pragma unroll
             for (int v = 0; v < VE; ++v) mu[v] = carry[v];
@@ -353,74 +404,73 @@ __global__ void __launch_bounds__(32 * MAX_W) recurrence_backward_kernel(const R
 #pragma unroll
         for (int i = 0; i + 1 < SPAN; ++i)
 #pragma unroll
-            for (int v = 0; v < VE; ++v) before[i + 1][v] = fmaf(g.at(i, v), before[i][v], x.d[i].get(v));
+            for (int v = 0; v < VE; ++v) before[i + 1][v] = fmaf(g.at(i, v), before[i][v], x.at(i, v));
+        T *px = dxp + (t + SPAN - 1) * dxs;
+        GT *pg = dgp + (t + SPAN - 1) * dgs;
 #pragma unroll
-        for (int i = SPAN - 1; i >= 0; --i) {
+        for (int i = SPAN - 1; i >= 0; --i, px -= dxs, pg -= dgs) {
             Vec<T, VE> o;
             Vec<GT, SHARED ? 1 : VE> og;
             float sum = 0.0f;
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
-                const float lambda = dh.d[i].get(v) + mu[v];
+                const float lambda = dh.at(i, v) + mu[v];
                 o.set(v, lambda);
-                const float d = lambda * before[i][v];
-                if (SHARED) sum += d;
-                else og.set(v, d);
+                if (SHARED) sum = fmaf(lambda, before[i][v], sum);
+                else og.set(v, lambda * before[i][v]);
                 mu[v] = g.at(i, v) * lambda;
             }
-            if (i < left) o.store(dxp + (t + i) * dir * a.dx_t);
-            if (!SHARED) {
-                if (i < left) og.store(dgp + (t + i) * dir * a.dgate_t);
-            } else {
-                // sum over the group's lanes of this tile; steps past the end and lanes without channels add 0
-                const int units = min(a.group_units - me.part * 32, 32);
-                const int pos = me.pos - me.part * 32;
-                if (!(i < left)) sum = 0.0f;
-                for (int d = 1; d < units; d <<= 1) {
-                    const float other = __shfl_down_sync(0xffffffffu, sum, d);
-                    if (pos + d < units) sum += other;
-                }
-                if (pos == 0 && i < left) {
-                    if (a.parts == 1) {
-                        dgp[(t + i) * dir * a.dgate_t] = from_f32<GT>(sum);
-                    } else {
-                        const long long at = a.reverse ? me.len - 1 - (t + i) : t + i;
-                        const long long row = (a.packed ? me.row0 : me.seq * a.steps) + at;
-                        a.partial[(me.part * a.rows + row) * a.groups + gc] = sum;
-                    }
+            if (i < left) o.store_stream(px);
+            if (SHARED) sums[i * SUM_STRIDE + lane] = sum;
+            else if (i < left) og.store_stream(pg);
+        }
+        if (SHARED) {
+            // (step, group) sums over the group's lanes in this warp, in the lanes' order
+            __syncwarp();
+            const int units = min(a.group_units - me.part * 32, 32), outs = SPAN * a.groups_per_tile;
+            for (int o = lane; o < (outs + 31) / 32 * 32; o += 32) {
+                const int i = o % SPAN, from = o / SPAN * a.group_units;
+                const int src = min(from, 31);
+                // the group's place, from its first lane
+                const int oleft = __shfl_sync(0xffffffffu, left, src), oseq = __shfl_sync(0xffffffffu, me.seq, src);
+                const int orow = __shfl_sync(0xffffffffu, me.row0, src), olen = __shfl_sync(0xffffffffu, me.len, src);
+                const int ogc = __shfl_sync(0xffffffffu, gc, src), ot = __shfl_sync(0xffffffffu, t, src) + i;
+                if (o >= outs || i >= oleft) continue;
+                float sum = 0.0f;
+                for (int l = 0; l < units; ++l) sum += sums[i * SUM_STRIDE + from + l];
+                const long long at = a.reverse ? olen - 1 - ot : ot;
+                if (a.parts == 1) {
+                    static_cast<GT *>(a.dgate)[(a.packed ? orow * a.dgate_t : oseq * a.dgate_s) + at * a.dgate_t + ogc] = from_f32<GT>(sum);
+                } else {
+                    const long long row = (a.packed ? orow : (long long)oseq * a.steps) + at;
+                    a.partial[(me.part * a.rows + row) * a.groups + ogc] = sum;
                 }
             }
+            __syncwarp();
         }
         if (W == 1)
 #pragma unroll
             for (int v = 0; v < VE; ++v) carry[v] = mu[v];
     }
-    if (a.dstate && w == 0 && split == 0 && me.active)
-#pragma unroll
-        for (int v = 0; v < VE; ++v) a.dstate[me.chain + v] = carry[v];
-}
-
-// dgate from the partial sums of its parts, in order
-template <class GT>
-__global__ void recurrence_join_kernel(const RecArgs a) {
-    const long long n = a.rows * a.groups;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        float t = 0.0f;
-        for (int p = 0; p < a.parts; ++p) t += a.partial[p * n + i];
-        const long long row = i / a.groups, g = i - row * a.groups;
-        const long long s = a.packed ? 0 : row / a.steps, at = a.packed ? row : row - s * a.steps;
-        static_cast<GT *>(a.dgate)[s * a.dgate_s + at * a.dgate_t + g] = from_f32<GT>(t);
+    if (a.dstate && w == 0 && split == 0 && me.active) store_ends<VE>(a.dstate + me.chain, carry);
+    if (a.packed) {
+        clear_rest<T>(a, a.dx, a.dx_t, a.width);
+        if (a.parts == 1) clear_rest<GT>(a, a.dgate, a.dgate_t, a.groups);
     }
 }
 
-// zeros in the rows of a packed tensor that belong to no sequence
-template <class T>
-__global__ void recurrence_rest_kernel(const RecArgs a, T *out, long long stride, int width) {
-    const long long head = min(offset_at(a, 0), offset_at(a, a.seqs)), tail = offset_at(a, a.seqs);
-    const long long rows = head + a.steps - tail, n = rows * width;
+// dgate from the partial sums of its parts, in order; zeros in rows of no sequence
+template <class GT>
+__global__ void recurrence_join_kernel(const RecArgs a) {
+    const long long n = a.rows * a.groups;
+    const int tail = a.packed ? offset_at(a, a.seqs) : a.steps, head = a.packed ? min(offset_at(a, 0), tail) : 0;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / width;
-        out[(r < head ? r : tail + r - head) * stride + (i - r * width)] = from_f32<T>(0.0f);
+        const long long row = i / a.groups, g = i - row * a.groups;
+        const long long s = a.packed ? 0 : row / a.steps, at = a.packed ? row : row - s * a.steps;
+        float t = 0.0f;
+        if (!a.packed || (row >= head && row < tail))
+            for (int p = 0; p < a.parts; ++p) t += a.partial[p * n + i];
+        static_cast<GT *>(a.dgate)[s * a.dgate_s + at * a.dgate_t + g] = from_f32<GT>(t);
     }
 }
 
@@ -441,6 +491,8 @@ bool vec_fits(const flare_recurrence_args *a, int ve, bool backward) {
     };
     if (!ok(a->x, a->x_s, a->x_t, xs)) return false;
     if (share == 1 && !ok(a->gate, a->gate_s, a->gate_t, gs)) return false;
+    for (const void *p : {(const void *)a->state, (const void *)a->last, (const void *)a->saved, (const void *)a->dlast, (const void *)a->dstate})
+        if (reinterpret_cast<uintptr_t>(p) % (4 * ve)) return false;
     if (!backward) return ok(a->h, a->h_s, a->h_t, xs);
     return ok(a->dh, a->dh_s, a->dh_t, xs) && ok(a->dx, a->dx_s, a->dx_t, xs) &&
            (share > 1 || ok(a->dgate, a->dgate_s, a->dgate_t, gs));
@@ -451,12 +503,14 @@ RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
     const int share = a->width / a->groups;
     p.shared = share > 1;
     p.rows = a->offsets ? a->steps : a->seqs * a->steps;
-    // 4 bytes a lane make whole 128-byte lines of a warp; wider vectors only where a group of channels then fits a warp
-    p.ve = a->x_type == FLARE_F32 ? 1 : 2;
+    const long long chains = a->seqs * a->width;
+    // the widest vectors that leave the machine enough warps
+    p.ve = 4;
+    while (p.ve > 1 && (!vec_fits(a, p.ve, backward) || chains / p.ve < 32ll * 8 * SMS)) p.ve >>= 1;
+    while (p.ve < 2 && a->x_type != FLARE_F32 && vec_fits(a, 2 * p.ve, backward)) p.ve *= 2;  // 4 bytes a lane at least
+    // sums over a group stay within a warp where wider vectors allow it
     if (backward && p.shared)
-        while (p.ve < 4 && share / p.ve > 32) p.ve *= 2;
-    while (p.ve > 1 && !vec_fits(a, p.ve, backward)) p.ve >>= 1;
-    const long long units = a->seqs * a->width / p.ve;
+        while (p.ve < 4 && share / p.ve > 32 && vec_fits(a, 2 * p.ve, backward)) p.ve *= 2;
     p.group_units = p.parts = p.groups_per_tile = 1;
     if (backward && p.shared) {
         p.group_units = share / p.ve;
@@ -465,21 +519,23 @@ RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
         const long long groups = a->seqs * a->groups;
         p.tiles = p.parts > 1 ? groups * p.parts : (groups + p.groups_per_tile - 1) / p.groups_per_tile;
     } else {
-        p.tiles = (units + 31) / 32;
+        p.tiles = (chains / p.ve + 31) / 32;
     }
-    // time is cut only as far as it takes to fill the machine: W spans a block, then S blocks
+    // time is cut only as far as it takes to fill the machine: W spans at a time, then S blocks
     const long long mean = std::max<long long>(1, a->offsets ? a->steps / std::max<long long>(1, a->seqs) : a->steps);
     const long long spans = (mean + SPAN - 1) / SPAN;
     p.warps = 1;
-    while (p.warps < MAX_W && 2 * p.warps <= spans && p.tiles * p.warps < 12ll * SMS) p.warps *= 2;
+    while (p.warps < WARPS && 2 * p.warps <= spans && p.tiles * p.warps < 16ll * SMS) p.warps *= 2;
+    // packed sequences are uneven: the longest ones finish last, so each gets several warps if the mean one can use them
+    if (a->offsets)
+        while (p.warps < WARPS && 2 * p.warps <= spans) p.warps *= 2;
     p.splits = 1;
-    const long long have = p.tiles * p.warps, want = 8ll * SMS;
-    if (have > 0 && have * 2 <= want) {
+    const long long have = p.tiles * p.warps, want = 24ll * SMS;
+    if (p.warps == WARPS && have > 0 && have * 2 <= want) {
         const long long rounds = (mean + p.warps * SPAN - 1) / (p.warps * SPAN);
-        p.splits = (int)std::min({want / have, rounds, (long long)MAX_SPLITS});
-        if (p.splits < 1) p.splits = 1;
+        p.splits = (int)std::max(1ll, std::min({want / have, rounds, (long long)MAX_SPLITS}));
     }
-    p.agg_bytes = p.splits > 1 ? (8ll * p.splits * a->seqs * a->width + 15) / 16 * 16 : 0;
+    p.agg_bytes = p.splits > 1 ? (8ll * p.splits * chains + 15) / 16 * 16 : 0;
     p.bytes = p.agg_bytes + (p.parts > 1 ? 4ll * p.parts * p.rows * a->groups : 0);
     return p;
 }
@@ -492,16 +548,18 @@ RecArgs rec_args(const flare_recurrence_args *in, const RecPlan &p) {
     a.last = in->last, a.saved = in->saved, a.dstate = in->dstate;
     a.agg = static_cast<float *>(in->workspace);
     a.partial = reinterpret_cast<float *>(static_cast<char *>(in->workspace) + p.agg_bytes);
-    a.seqs = in->seqs, a.steps = in->steps, a.rows = p.rows;
+    a.seqs = in->seqs, a.steps = (int)in->steps, a.rows = p.rows;
     a.gate_s = in->gate_s, a.gate_t = in->gate_t, a.x_s = in->x_s, a.x_t = in->x_t, a.h_s = in->h_s, a.h_t = in->h_t;
     a.dh_s = in->dh_s, a.dh_t = in->dh_t, a.dgate_s = in->dgate_s, a.dgate_t = in->dgate_t, a.dx_s = in->dx_s, a.dx_t = in->dx_t;
-    a.width = in->width, a.groups = in->groups, a.share = in->width / in->groups;
+    a.width = in->width, a.groups = in->groups, a.share = FastDiv((unsigned)(in->width / in->groups));
     a.off64 = in->offsets_type == FLARE_I64, a.reverse = in->reverse != 0, a.packed = in->offsets != nullptr;
-    a.splits = p.splits;
+    a.warps = p.warps, a.splits = p.splits, a.tiles = (unsigned)p.tiles;
+    const long long round = (long long)p.warps * SPAN, rounds = (in->steps + round - 1) / round;
+    a.per = (int)std::min<long long>((rounds + p.splits - 1) / p.splits * round, 0x7fffffff);
     a.units = (unsigned)(in->seqs * in->width / p.ve);
     a.upr = FastDiv((unsigned)(in->width / p.ve));
     a.group_units = p.group_units, a.groups_per_tile = p.groups_per_tile, a.parts = p.parts;
-    a.spans = (in->steps + SPAN - 1) / SPAN;
+    a.spans = (int)((in->steps + SPAN - 1) / SPAN);
     return a;
 }
 
@@ -524,48 +582,38 @@ int rec_dispatch(const flare_recurrence_args *in, const RecPlan &p, F f) {
     });
 }
 
-template <class T>
-void launch_rest(const RecArgs &a, void *out, long long stride, int width, cudaStream_t st) {
-    const unsigned blocks = (unsigned)std::min<long long>((a.steps * width + 255) / 256, 2 * SMS);
-    recurrence_rest_kernel<T><<<blocks, 256, 0, st>>>(a, static_cast<T *>(out), stride, width);
-}
-
 int run_recurrence(const flare_recurrence_args *in, bool backward, cudaStream_t st) {
     const RecPlan p = rec_plan(in, backward);
     const RecArgs a = rec_args(in, p);
-    const dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
-    const int threads = 32 * p.warps;
-    const size_t smem = p.warps > 1 ? sizeof(float) * 4 * p.warps * 32 * p.ve : 0;
-    const char *what = backward ? "flare_recurrence_backward" : "flare_recurrence_forward";
+    const int at_once = WARPS / p.warps;  // tiles per block
+    // a block is launched for rows of no sequence even where there is no sequence
+    const dim3 grid((unsigned)std::max(1ll, (p.tiles + at_once - 1) / at_once), (unsigned)p.splits);
+    const size_t buffers = p.warps > 1 ? sizeof(float) * 4 * WARPS * 32 * p.ve : 0;
     rec_dispatch(in, p, [&](auto t, auto gt, auto ve, auto shared) {
         using T = typename decltype(t)::type;
         using GT = typename decltype(gt)::type;
         constexpr int VE = decltype(ve)::value;
         constexpr bool SH = decltype(shared)::value;
-        if (p.tiles == 0) {  // packed rows without a sequence
-        } else if (p.splits > 1) {
+        if (p.splits > 1) {
             // the split kernel's tiles are plain ones, whatever the main kernel's
-            const dim3 sgrid((a.units + 31) / 32, (unsigned)p.splits);
-            const size_t ss = sizeof(float) * 4 * p.warps * 32 * VE;
-            if (backward) recurrence_split_kernel<true, T, GT, VE, SH><<<sgrid, threads, ss, st>>>(a);
-            else recurrence_split_kernel<false, T, GT, VE, SH><<<sgrid, threads, ss, st>>>(a);
+            RecArgs plain = a;
+            plain.tiles = (a.units + 31) / 32;
+            const dim3 sgrid((plain.tiles + at_once - 1) / at_once, (unsigned)p.splits);
+            if (backward) recurrence_split_kernel<true, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
+            else recurrence_split_kernel<false, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
         }
-        if (p.tiles == 0) {
-        } else if (backward) recurrence_backward_kernel<T, GT, VE, SH><<<grid, threads, smem, st>>>(a);
-        else recurrence_forward_kernel<T, GT, VE, SH><<<grid, threads, smem, st>>>(a);
-        if (p.tiles && backward && p.parts > 1) {
+        if (!backward) {
+            recurrence_forward_kernel<T, GT, VE, SH><<<grid, 32 * WARPS, buffers, st>>>(a);
+            return;
+        }
+        const size_t sums = SH ? sizeof(float) * WARPS * SPAN * SUM_STRIDE : 0;
+        recurrence_backward_kernel<T, GT, VE, SH><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
+        if (p.parts > 1) {
             const long long n = p.rows * in->groups;
             recurrence_join_kernel<GT><<<(unsigned)std::min<long long>((n + 255) / 256, 16 * SMS), 256, 0, st>>>(a);
         }
-        if (a.packed) {
-            if (!backward && a.h) launch_rest<T>(a, a.h, a.h_t, a.width, st);
-            if (backward) {
-                launch_rest<T>(a, a.dx, a.dx_t, a.width, st);
-                launch_rest<GT>(a, a.dgate, a.dgate_t, a.groups, st);
-            }
-        }
     });
-    OPS_LAUNCHED(what);
+    OPS_LAUNCHED(backward ? "flare_recurrence_backward" : "flare_recurrence_forward");
     return FLARE_OK;
 }
 
@@ -576,7 +624,8 @@ int rec_check(const flare_recurrence_args *a, bool backward, const char *what) {
               a->x_type);
     OPS_CHECK(a->seqs >= 0 && a->steps >= 0 && a->width >= 1 && a->groups >= 1 && a->width % a->groups == 0,
               "%s: %lld sequences of %lld steps, %d channels in %d groups", what, a->seqs, a->steps, a->width, a->groups);
-    OPS_CHECK(a->seqs * a->width < 0x40000000ll && a->seqs < 0x40000000ll, "%s: %lld sequences of %d channels", what, a->seqs, a->width);
+    OPS_CHECK(a->seqs < 0x40000000ll && a->seqs * a->width < 0x40000000ll && a->steps < 0x40000000ll,
+              "%s: %lld sequences of %lld steps, %d channels", what, a->seqs, a->steps, a->width);
     OPS_CHECK(a->offsets_type == FLARE_I32 || a->offsets_type == FLARE_I64, "%s: unknown offsets type %d", what, a->offsets_type);
     const bool some = a->seqs > 0, data = (some || a->offsets) && a->steps > 0;
     OPS_CHECK(!data || (a->gate && a->x), "%s: NULL gate or x", what);

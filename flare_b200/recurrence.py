@@ -58,8 +58,9 @@ def _inputs(gate, x, state, offsets):
     if gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or gate.shape[-1] < 1 or x.shape[-1] % gate.shape[-1]:
         raise ValueError(f"gate: shape {tuple(gate.shape)}, expected {tuple(x.shape[:-1])} + (groups,), groups dividing "
                          f"{x.shape[-1]}")
-    if seqs * x.shape[-1] >= 2 ** 30:
-        raise ValueError(f"x: {seqs} sequences of {x.shape[-1]} channels, at most 2^30 channels in all")
+    if seqs * x.shape[-1] >= 2 ** 30 or x.shape[-2] >= 2 ** 30:
+        raise ValueError(f"x: {seqs} sequences of {x.shape[-1]} channels, {x.shape[-2]} steps, at most 2^30 channels in all and "
+                         "2^30 steps")
     _ends(state, "state", seqs, x)
     return _dense(gate), _dense(x), offsets, seqs
 
