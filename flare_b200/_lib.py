@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libflare_b200.so")
@@ -99,6 +100,11 @@ class RecurrenceArgs(ctypes.Structure):
 
 
 RECURRENCE_SPAN = 16
+# The operators' calls are short, so their argument structs are packed in one go: the same members as above.
+PACK_LOOKUP = struct.Struct("@5P4q4if")
+PACK_LOOKUP_GRAD = struct.Struct("@7P5q4if")
+PACK_RECURRENCE = struct.Struct("@13P15q6i")
+PACK_PRODUCT = struct.Struct("@7P4q2i")
 
 
 class ProductArgs(ctypes.Structure):
@@ -144,17 +150,17 @@ EXPORTS = {
     "flare_selftest_mlp": (ctypes.c_int, [vp, ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, vp]),
     "flare_render_hits_noalloc": (ctypes.c_int, [ctypes.c_int, vp, vp, vp, vp, vp, ctypes.c_int, vp, vp, vp,
                                                  ctypes.c_int, vp, vp, vp]),
-    "flare_lookup": (ctypes.c_int, [ctypes.POINTER(LookupArgs), vp]),
+    "flare_lookup": (ctypes.c_int, [vp, vp]),
     "flare_lookup_workspace": (ll, [ll, ll, ctypes.c_int]),
-    "flare_lookup_backward": (ctypes.c_int, [ctypes.POINTER(LookupGradArgs), vp]),
+    "flare_lookup_backward": (ctypes.c_int, [vp, vp]),
     "flare_recurrence_saved": (ll, [ll, ll, ctypes.c_int, ctypes.c_int]),
-    "flare_recurrence_workspace": (ll, [ctypes.POINTER(RecurrenceArgs), ctypes.c_int]),
-    "flare_recurrence_forward": (ctypes.c_int, [ctypes.POINTER(RecurrenceArgs), vp]),
-    "flare_recurrence_backward": (ctypes.c_int, [ctypes.POINTER(RecurrenceArgs), vp]),
+    "flare_recurrence_workspace": (ll, [vp, ctypes.c_int]),
+    "flare_recurrence_forward": (ctypes.c_int, [vp, vp]),
+    "flare_recurrence_backward": (ctypes.c_int, [vp, vp]),
     "flare_micro_quantize": (ctypes.c_int, [vp, ctypes.c_int, ll, ctypes.c_int, ll, vp, vp, vp]),
     "flare_micro_dequantize": (ctypes.c_int, [vp, vp, ll, ctypes.c_int, vp, ctypes.c_int, ll, vp]),
     "flare_micro_product_workspace": (ll, [ll, ll, ctypes.c_int]),
-    "flare_micro_product": (ctypes.c_int, [ctypes.POINTER(ProductArgs), vp]),
+    "flare_micro_product": (ctypes.c_int, [vp, vp]),
 }
 
 _lib = None

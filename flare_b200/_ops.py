@@ -2,7 +2,6 @@
 codes of the C ABI, argument checks in the renderer's manner (ValueError), the stream and device of a call."""
 from __future__ import annotations
 
-import ctypes
 from contextlib import nullcontext
 
 import torch
@@ -12,8 +11,12 @@ MICRO = 3                                                            # FLARE_MIC
 INDEX_CODE = {torch.int32: 0, torch.int64: 1}                        # FLARE_I32, FLARE_I64
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_same_device = nullcontext()
+
+
 def ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def need(t, name, dtypes, device=None):
@@ -30,18 +33,19 @@ def need(t, name, dtypes, device=None):
 
 
 def need_shape(t, name, shape):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     return t
 
 
 def on(device):
     """Makes `device` current for the launches inside."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """The handle of the device's current stream."""
+    return _raw_stream(device.index)
 
 
 def workspace(nbytes, device):

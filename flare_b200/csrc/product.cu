@@ -13,6 +13,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "ops.cuh"
@@ -348,7 +349,14 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, ProductArgs a, 
     int smem = a.stages * Tile::STAGE + 1024;
     if (split > 1) smem = std::max(smem, PT * BN * 4 + 1024);
     auto fn = product_kernel<BN, O>;
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX - SMEM_HEAD);
+    static std::atomic<unsigned long long> set{0};  // devices that this kernel may use all shared memory on
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const unsigned long long bit = 1ull << (device & 63);
+    if (e == cudaSuccess && !(set.load() & bit)) {
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX - SMEM_HEAD);
+        if (e == cudaSuccess) set.fetch_or(bit);
+    }
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)((a.p + PT - 1) / PT), (unsigned)((a.q + BN - 1) / BN), (unsigned)split);

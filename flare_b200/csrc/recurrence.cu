@@ -135,6 +135,12 @@ struct Span {
         }
     }
     __device__ __forceinline__ float at(int i, int v) const { return d[i].get(N == 1 ? 0 : v); }
+    // step i is unpacked to 32 bits here and not before, so that a span waits in its packed form
+    __device__ __forceinline__ void hold(int i) {
+        if constexpr (N * sizeof(T) == 2) asm volatile("" : "+h"(d[i].raw[0]));
+        else if constexpr (N * sizeof(T) == 4) asm volatile("" : "+r"(d[i].raw[0]));
+        else if constexpr (N * sizeof(T) == 8) asm volatile("" : "+r"(d[i].raw[0].x), "+r"(d[i].raw[0].y));
+    }
 };
 
 // (A, H) of a span, walked from its first step (forward) or its last (backward, where H collects a_t dh_t)
@@ -363,8 +369,9 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const Re
 }
 
 // smem: the exchange buffers, then SHARED: 16 x 32 products per warp
-template <class T, class GT, int VE, bool SHARED>
-__global__ void __launch_bounds__(32 * WARPS) recurrence_backward_kernel(const RecArgs a) {
+// DH: whether there is a gradient of every state, not of the last ones alone
+template <class T, class GT, int VE, bool SHARED, bool DH>
+__global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(const RecArgs a) {
     extern __shared__ __align__(16) float smem[];
     const int W = a.warps, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
     const Place<VE, SHARED> me(a, my_tile(a));
@@ -378,7 +385,7 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_backward_kernel(const R
     const long long dhs = a.reverse ? -a.dh_t : a.dh_t, dxs = a.reverse ? -a.dx_t : a.dx_t, dgs = a.reverse ? -a.dgate_t : a.dgate_t;
     const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + gc;
     const T *xp = static_cast<const T *>(a.x) + me.first(a, a.x_s, a.x_t) + me.c;
-    const T *dhp = static_cast<const T *>(a.dh) + me.first(a, a.dh_s, a.dh_t) + me.c;
+    const T *dhp = DH ? static_cast<const T *>(a.dh) + me.first(a, a.dh_s, a.dh_t) + me.c : nullptr;
     T *dxp = static_cast<T *>(a.dx) + me.first(a, a.dx_s, a.dx_t) + me.c;
     GT *dgp = static_cast<GT *>(a.dgate) + me.first(a, a.dgate_s, a.dgate_t) + gc;
     float carry[VE], mu[VE], A[VE], H[VE];
@@ -389,12 +396,13 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_backward_kernel(const R
         Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x, dh;
         g.template load<SHARED>(gp + t * gs, gs, left, 1.0f);
-        dh.template load<false>(dhp + t * dhs, dhs, a.dh ? left : 0, 0.0f);
+        if (DH) dh.template load<false>(dhp + t * dhs, dhs, left, 0.0f);
         x.template load<false>(xp + t * xs, xs, left, 0.0f);
         float before[SPAN][VE];  // the state before each step
         if (t > 0) load_ends<VE>(a.saved + me.saved_row(a, t / SPAN) * a.width, me.c, left > 0, before[0]);
         else load_ends<VE>(a.state, me.chain, left > 0, before[0]);
         if (W > 1) {
+            if (!DH) dh.template load<false>(nullptr, 0, 0, 0.0f);
             stretch<true>(g, dh, A, H);
             exchange<true>(bufs + (k & 1) * 2 * W * 32 * VE, W, A, H, carry, mu);
         } else {
@@ -402,9 +410,11 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_backward_kernel(const R
             for (int v = 0; v < VE; ++v) mu[v] = carry[v];
         }
 #pragma unroll
-        for (int i = 0; i + 1 < SPAN; ++i)
+        for (int i = 0; i + 1 < SPAN; ++i) {
+            x.hold(i);
 #pragma unroll
             for (int v = 0; v < VE; ++v) before[i + 1][v] = fmaf(g.at(i, v), before[i][v], x.at(i, v));
+        }
         T *px = dxp + (t + SPAN - 1) * dxs;
         GT *pg = dgp + (t + SPAN - 1) * dgs;
 #pragma unroll
@@ -412,9 +422,10 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_backward_kernel(const R
             Vec<T, VE> o;
             Vec<GT, SHARED ? 1 : VE> og;
             float sum = 0.0f;
+            if (DH) dh.hold(i);
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
-                const float lambda = dh.at(i, v) + mu[v];
+                const float lambda = DH ? dh.at(i, v) + mu[v] : mu[v];
                 o.set(v, lambda);
                 if (SHARED) sum = fmaf(lambda, before[i][v], sum);
                 else og.set(v, lambda * before[i][v]);
@@ -505,12 +516,14 @@ RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
     p.rows = a->offsets ? a->steps : a->seqs * a->steps;
     const long long chains = a->seqs * a->width;
     // the widest vectors that leave the machine enough warps
-    p.ve = 4;
+    // the gradient holds x, dh, 32-bit states and gates of a span in 128 registers a thread
+    const int widest = !backward ? 4 : (a->x_type == FLARE_F32 ? 1 : 2) * (p.shared ? 2 : 1);
+    p.ve = widest;
     while (p.ve > 1 && (!vec_fits(a, p.ve, backward) || chains / p.ve < 32ll * 8 * SMS)) p.ve >>= 1;
     while (p.ve < 2 && a->x_type != FLARE_F32 && vec_fits(a, 2 * p.ve, backward)) p.ve *= 2;  // 4 bytes a lane at least
     // sums over a group stay within a warp where wider vectors allow it
     if (backward && p.shared)
-        while (p.ve < 4 && share / p.ve > 32 && vec_fits(a, 2 * p.ve, backward)) p.ve *= 2;
+        while (p.ve < widest && share / p.ve > 32 && vec_fits(a, 2 * p.ve, backward)) p.ve *= 2;
     p.group_units = p.parts = p.groups_per_tile = 1;
     if (backward && p.shared) {
         p.group_units = share / p.ve;
@@ -607,7 +620,8 @@ int run_recurrence(const flare_recurrence_args *in, bool backward, cudaStream_t 
             return;
         }
         const size_t sums = SH ? sizeof(float) * WARPS * SPAN * SUM_STRIDE : 0;
-        recurrence_backward_kernel<T, GT, VE, SH><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
+        if (a.dh) recurrence_backward_kernel<T, GT, VE, SH, true><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
+        else recurrence_backward_kernel<T, GT, VE, SH, false><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
         if (p.parts > 1) {
             const long long n = p.rows * in->groups;
             recurrence_join_kernel<GT><<<(unsigned)std::min<long long>((n + 255) / 256, 16 * SMS), 256, 0, st>>>(a);

@@ -13,8 +13,6 @@ No reference counterpart (the reference reads descriptors inside its decoder ker
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib, _ops
@@ -57,12 +55,11 @@ def lookup(table, idx, weight=None, scale=1.0, dtype=None):
     idx, weight = _entries(idx, weight, device)
     with _ops.on(device):
         out = torch.empty(idx.shape + (width,), dtype=dtype, device=device)
-        a = _lib.LookupArgs(_ops.ptr(table.codes if micro else table), _ops.ptr(table.scales) if micro else None,
-                            _ops.ptr(idx), _ops.ptr(weight), _ops.ptr(out), n_rows, idx.numel(),
-                            0 if micro else table.stride(0), width, width,
-                            _ops.MICRO if micro else _ops.TYPE_CODE[table.dtype], _ops.INDEX_CODE[idx.dtype],
-                            _ops.TYPE_CODE[dtype], float(scale))
-        _lib.check(lib.flare_lookup(ctypes.byref(a), _ops.stream(device)), "lookup")
+        a = _lib.PACK_LOOKUP.pack(
+            (table.codes if micro else table).data_ptr(), table.scales.data_ptr() if micro else 0, idx.data_ptr(), _ops.ptr(weight),
+            out.data_ptr(), n_rows, idx.numel(), 0 if micro else table.stride(0), width, width,
+            _ops.MICRO if micro else _ops.TYPE_CODE[table.dtype], _ops.INDEX_CODE[idx.dtype], _ops.TYPE_CODE[dtype], scale)
+        _lib.check(lib.flare_lookup(a, _ops.stream(device)), "lookup")
     return out
 
 
@@ -92,9 +89,9 @@ def lookup_backward(dout, table, idx, weight=None, scale=1.0, need_table=True, n
         dtable = torch.empty((n_rows, width), dtype=torch.float32, device=device) if need_table else None
         dweight = torch.empty(idx.shape, dtype=torch.float32, device=device) if need_weight else None
         ws = _ops.workspace(lib.flare_lookup_workspace(n_rows, n, width) if need_table else 0, device)
-        a = _lib.LookupGradArgs(_ops.ptr(dout), _ops.ptr(table), _ops.ptr(idx), _ops.ptr(weight), _ops.ptr(dtable),
-                                _ops.ptr(dweight), _ops.ptr(ws), n_rows, n, dout.stride(0) if n else width,
-                                table.stride(0), 0 if ws is None else ws.numel(), width, _ops.TYPE_CODE[table.dtype],
-                                _ops.INDEX_CODE[idx.dtype], _ops.TYPE_CODE[dout.dtype], float(scale))
-        _lib.check(lib.flare_lookup_backward(ctypes.byref(a), _ops.stream(device)), "lookup_backward")
+        a = _lib.PACK_LOOKUP_GRAD.pack(
+            dout.data_ptr(), table.data_ptr(), idx.data_ptr(), _ops.ptr(weight), _ops.ptr(dtable), _ops.ptr(dweight), _ops.ptr(ws),
+            n_rows, n, dout.stride(0) if n else width, table.stride(0), 0 if ws is None else ws.numel(), width,
+            _ops.TYPE_CODE[table.dtype], _ops.INDEX_CODE[idx.dtype], _ops.TYPE_CODE[dout.dtype], scale)
+        _lib.check(lib.flare_lookup_backward(a, _ops.stream(device)), "lookup_backward")
     return dtable, dweight

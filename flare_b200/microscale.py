@@ -7,8 +7,6 @@ gradient.  No reference counterpart.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib, _ops
@@ -29,6 +27,7 @@ class Micro4:
     __slots__ = ("codes", "scales", "width")
 
     def __init__(self, codes, scales, width: int):
+        """Checks and keeps the two tensors."""
         width = int(width)
         blocks = -(-width // BLOCK)
         _ops.need(codes, "codes", (torch.uint8,))
@@ -81,7 +80,9 @@ def quantize(x) -> Micro4:
         scales = torch.empty((rows, -(-blocks // 4) * 4), dtype=torch.uint8, device=x.device)
         _lib.check(lib.flare_micro_quantize(_ops.ptr(x), _ops.TYPE_CODE[x.dtype], rows, width, x.stride(0),
                                             _ops.ptr(codes), _ops.ptr(scales), _ops.stream(x.device)), "quantize")
-    return Micro4(codes, scales, width)
+    q = Micro4.__new__(Micro4)  # made here, so there is nothing to check
+    q.codes, q.scales, q.width = codes, scales, width
+    return q
 
 
 def product(x, w: Micro4, dtype=torch.bfloat16, check=False):
@@ -107,10 +108,10 @@ def product(x, w: Micro4, dtype=torch.bfloat16, check=False):
         out = torch.empty((m, n), dtype=dtype, device=x.device)
         ws = _ops.workspace(lib.flare_micro_product_workspace(m, n, k), x.device)
         status = torch.zeros(1, dtype=torch.int32, device=x.device) if check else None
-        a = _lib.ProductArgs(_ops.ptr(x.codes), _ops.ptr(x.scales), _ops.ptr(w.codes), _ops.ptr(w.scales), _ops.ptr(out),
-                             _ops.ptr(ws), _ops.ptr(status), m, n, n, 0 if ws is None else ws.numel(), k,
-                             _ops.TYPE_CODE[dtype])
-        _lib.check(lib.flare_micro_product(ctypes.byref(a), _ops.stream(x.device)), "product")
+        a = _lib.PACK_PRODUCT.pack(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
+                                   _ops.ptr(ws), _ops.ptr(status), m, n, n, 0 if ws is None else ws.numel(), k,
+                                   _ops.TYPE_CODE[dtype])
+        _lib.check(lib.flare_micro_product(a, _ops.stream(x.device)), "product")
     if check and int(status):
         raise _lib.FlareError(f"product: device reported error bits 0x{int(status):x} (tensor-core wait timeout)")
     return out

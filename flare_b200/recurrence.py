@@ -12,8 +12,6 @@ No reference counterpart (the reference composites inside its kernels only).
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib, _ops
@@ -36,7 +34,7 @@ def _like(t, width, dtype):
 
 def _strides(t):
     """(per sequence, per step) in elements."""
-    return (0, 0) if t is None else (t.stride(0), t.stride(1)) if t.dim() == 3 else (0, t.stride(0))
+    return (0, 0) if t is None else t.stride()[:2] if t.dim() == 3 else (0, t.stride(0))
 
 
 def _inputs(gate, x, state, offsets):
@@ -71,24 +69,19 @@ def _ends(t, name, seqs, x):
         _ops.need_shape(t, name, (seqs, x.shape[-1]))
 
 
-def _args(gate, x, offsets, seqs, reverse):
-    a = _lib.RecurrenceArgs()
-    a.gate, a.x, a.offsets = _ops.ptr(gate), _ops.ptr(x), _ops.ptr(offsets)
-    a.gate_s, a.gate_t = _strides(gate)
-    a.x_s, a.x_t = _strides(x)
-    a.seqs, a.steps = seqs, x.shape[-2]
-    a.width, a.groups = x.shape[-1], gate.shape[-1]
-    a.gate_type, a.x_type = _ops.TYPE_CODE[gate.dtype], _ops.TYPE_CODE[x.dtype]
-    a.offsets_type = 0 if offsets is None else _ops.INDEX_CODE[offsets.dtype]
-    a.reverse = 1 if reverse else 0
-    return a
-
-
-def _launch(lib, fn, a, backward, device, what):
-    nbytes = lib.flare_recurrence_workspace(ctypes.byref(a), backward)
-    ws = _ops.workspace(nbytes, device)
-    a.workspace, a.workspace_bytes = _ops.ptr(ws), nbytes
-    _lib.check(fn(ctypes.byref(a), _ops.stream(device)), what)
+def _launch(lib, backward, what, seqs, reverse, gate, x, state, offsets, h=None, last=None, saved=None, dh=None, dlast=None, dgate=None,
+            dx=None, dstate=None):
+    p, dev, steps = _ops.ptr, x.device, x.shape[-2]
+    head = (gate.data_ptr(), x.data_ptr(), p(state), p(offsets), p(h), p(last), p(saved), p(dh), p(dlast), p(dgate), p(dx), p(dstate))
+    tail = (seqs, steps, *_strides(gate), *_strides(x), *_strides(h), *_strides(dh), *_strides(dgate), *_strides(dx), x.shape[-1],
+            gate.shape[-1], _ops.TYPE_CODE[gate.dtype], _ops.TYPE_CODE[x.dtype],
+            0 if offsets is None else _ops.INDEX_CODE[offsets.dtype], 1 if reverse else 0)
+    ws, nbytes = None, 0
+    if backward or steps > _lib.RECURRENCE_SPAN:  # a forward of one span needs none
+        nbytes = lib.flare_recurrence_workspace(_lib.PACK_RECURRENCE.pack(*head, 0, 0, *tail), backward)
+        ws = _ops.workspace(nbytes, dev)
+    a = _lib.PACK_RECURRENCE.pack(*head, p(ws), nbytes, *tail)
+    _lib.check((lib.flare_recurrence_backward if backward else lib.flare_recurrence_forward)(a, _ops.stream(dev)), what)
 
 
 def scan(gate, x, state=None, offsets=None, reverse=False, states=True, training=False):
@@ -108,16 +101,13 @@ def scan(gate, x, state=None, offsets=None, reverse=False, states=True, training
     state = None if state is None else state.contiguous()
     dev, width = x.device, x.shape[-1]
     with _ops.on(dev):
-        a = _args(gate, x, offsets, seqs, reverse)
         h = _like(x, width, x.dtype) if states else None
         last = torch.empty((seqs, width), dtype=torch.float32, device=dev)
         saved = None
         if training:
             n = lib.flare_recurrence_saved(seqs, x.shape[-2], width, 0 if offsets is None else 1)
             saved = torch.empty(n, dtype=torch.float32, device=dev)
-        a.state, a.h, a.last, a.saved = _ops.ptr(state), _ops.ptr(h), _ops.ptr(last), _ops.ptr(saved)
-        a.h_s, a.h_t = _strides(h)
-        _launch(lib, lib.flare_recurrence_forward, a, 0, dev, "scan")
+        _launch(lib, 0, "scan", seqs, reverse, gate, x, state, offsets, h, last, saved)
     return h, last, saved
 
 
@@ -142,15 +132,9 @@ def scan_backward(gate, x, saved, dh=None, dlast=None, state=None, offsets=None,
     _ends(dlast, "dlast", seqs, x)
     dlast = None if dlast is None else dlast.contiguous()
     with _ops.on(dev):
-        a = _args(gate, x, offsets, seqs, reverse)
         dgate, dx = _like(gate, gate.shape[-1], gate.dtype), _like(x, width, x.dtype)
         dstate = None if state is None else torch.empty_like(state)
-        a.state, a.saved, a.dh, a.dlast = _ops.ptr(state), _ops.ptr(saved), _ops.ptr(dh), _ops.ptr(dlast)
-        a.dgate, a.dx, a.dstate = _ops.ptr(dgate), _ops.ptr(dx), _ops.ptr(dstate)
-        a.dh_s, a.dh_t = _strides(dh)
-        a.dgate_s, a.dgate_t = _strides(dgate)
-        a.dx_s, a.dx_t = _strides(dx)
-        _launch(lib, lib.flare_recurrence_backward, a, 1, dev, "scan_backward")
+        _launch(lib, 1, "scan_backward", seqs, reverse, gate, x, state, offsets, None, None, saved, dh, dlast, dgate, dx, dstate)
     return dgate, dx, dstate
 
 
@@ -160,23 +144,28 @@ def step(gate, x, state, out=None):
 
     x: (sequences, width) f32, f16 or bf16; gate: (sequences, groups), of x's type or f32.
     """
-    if not isinstance(x, torch.Tensor) or x.dim() != 2:
-        raise ValueError("x: expected a (sequences, width) tensor")
-    if not isinstance(gate, torch.Tensor) or gate.dim() != 2:
-        raise ValueError("gate: expected a (sequences, groups) tensor")
     lib = _lib.load()
-    gate, x, _, seqs = _inputs(gate[:, None], x[:, None], state, None)
+    _ops.need(x, "x", _FLOATS)
+    dev = x.device
+    _ops.need(gate, "gate", (x.dtype, torch.float32), dev)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x: shape {tuple(x.shape)}, expected (sequences, width)")
+    seqs, width = x.shape
+    if gate.dim() != 2 or gate.shape[0] != seqs or gate.shape[1] < 1 or width % gate.shape[1]:
+        raise ValueError(f"gate: shape {tuple(gate.shape)}, expected ({seqs}, groups), groups dividing {width}")
+    if seqs * width >= 2 ** 30:
+        raise ValueError(f"x: {seqs} sequences of {width} channels, at most 2^30 channels in all")
     out = state if out is None else out
     for t, name in ((state, "state"), (out, "out")):
-        if t is None:
-            raise ValueError(f"{name}: expected a (sequences, width) tensor")
-        _ends(t, name, seqs, x)
+        _ops.need_shape(_ops.need(t, name, _F32, dev), name, x.shape)
         if not t.is_contiguous():
             raise ValueError(f"{name}: tensor must be contiguous")
-    with _ops.on(x.device):
-        a = _args(gate, x, None, seqs, False)
-        h = torch.empty((seqs, x.shape[-1]), dtype=x.dtype, device=x.device)
-        a.state, a.h, a.last = _ops.ptr(state), _ops.ptr(h), _ops.ptr(out)
-        a.h_s = a.h_t = x.shape[-1]
-        _launch(lib, lib.flare_recurrence_forward, a, 0, x.device, "step")
+    gate, x = _dense(gate), _dense(x)
+    with _ops.on(dev):
+        h = torch.empty((seqs, width), dtype=x.dtype, device=dev)
+        # one step of `seqs` sequences: the rows are the sequences
+        a = _lib.PACK_RECURRENCE.pack(gate.data_ptr(), x.data_ptr(), state.data_ptr(), 0, h.data_ptr(), out.data_ptr(), 0, 0, 0, 0, 0, 0,
+                                      0, 0, seqs, 1, gate.stride(0), 0, x.stride(0), 0, width, 0, 0, 0, 0, 0, 0, 0, width,
+                                      gate.shape[1], _ops.TYPE_CODE[gate.dtype], _ops.TYPE_CODE[x.dtype], 0, 0)
+        _lib.check(lib.flare_recurrence_forward(a, _ops.stream(dev)), "step")
     return h

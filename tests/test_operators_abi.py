@@ -33,3 +33,13 @@ def test_ctypes_structs_match_the_header(tmp_path):
     subprocess.run(["gcc", "-std=c11", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert [(w, v) for w, v in expect] == [(w, g) for (w, _), g in zip(expect, got)]
+
+
+def test_packed_arguments_have_the_structs_layout():
+    for pack, cls in ((_lib.PACK_LOOKUP, _lib.LookupArgs), (_lib.PACK_LOOKUP_GRAD, _lib.LookupGradArgs),
+                      (_lib.PACK_RECURRENCE, _lib.RecurrenceArgs), (_lib.PACK_PRODUCT, _lib.ProductArgs)):
+        n = len(cls._fields_)
+        raw = pack.pack(*range(1, n + 1))
+        a = cls.from_buffer_copy(raw.ljust(ctypes.sizeof(cls), b"\0"))
+        got = [getattr(a, name) for name, _ in cls._fields_]
+        assert got == list(range(1, n + 1)) and ctypes.sizeof(cls) - len(raw) < 8
