@@ -159,41 +159,63 @@ int run_lookup(const flare_lookup_args *in, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------------------
 // Stable radix sort of the entries by row; entries that name no row get key `rows` and end behind all others.
-// Per digit: count per tile, scan over tiles, scatter.  A tile is 4096 consecutive entries of one block; warp w
-// ranks entries [512 w, 512 w + 512) of it 32 at a time, so ranks follow the entries' order.
+// Per digit of up to 11 bits: count per tile, scan over tiles, scatter.  A tile is 4096 consecutive entries of one block;
+// warp w ranks entries [512 w, 512 w + 512) of it 32 at a time, so ranks follow the entries' order.  Lanes with equal
+// digits find one another by a ballot per bit (match.any took three times the whole kernel's time).  Up to one tile of
+// entries is sorted by one block in shared memory.
 // ------------------------------------------------------------------------------------------------
 constexpr int RS_THREADS = 256, RS_WARPS = RS_THREADS / 32, RS_ROUNDS = 16, RS_TILE = RS_THREADS * RS_ROUNDS;
-constexpr int RS_MAX_BITS = 8, RS_BINS = 1 << RS_MAX_BITS;
+constexpr int RS_MAX_BITS = 11, RS_BINS = 1 << RS_MAX_BITS, RS_SMALL_BITS = 8;
 
 struct SortArgs {
     const void *index;              // first pass: keys come from the index, values are the entry numbers
-    const unsigned *key_in, *val_in;
-    unsigned *key_out, *val_out, *hist;  // hist: digit-major (bins, tiles)
+    const uint2 *in;                // (key, entry)
+    uint2 *out;
+    unsigned *key_out, *val_out;    // last pass
+    unsigned *hist;                 // digit-major (bins, tiles)
     unsigned *total;                // per digit
+    float *dweight;                 // 0 for entries without a row, or NULL
     long long rows;
     unsigned n, tiles;
-    int shift, bits, index_type, first;
+    int shift, bits, key_bits, index_type, first, last;
 };
 
-__device__ __forceinline__ unsigned sort_key(const SortArgs &a, unsigned i) {
-    if (!a.first) return a.key_in[i];
+__device__ __forceinline__ unsigned index_key(const SortArgs &a, unsigned i) {
     const long long p = a.index_type == FLARE_I64 ? row_of<long long>(a.index, i, a.rows) : row_of<int>(a.index, i, a.rows);
     return p < 0 ? (unsigned)a.rows : (unsigned)p;
+}
+__device__ __forceinline__ uint2 sort_entry(const SortArgs &a, unsigned i) {
+    return a.first ? make_uint2(index_key(a, i), i) : a.in[i];
+}
+
+// lanes of the warp with the same `bits`-bit digit (and the same `in`)
+__device__ __forceinline__ unsigned lanes_with(unsigned digit, int bits, bool in) {
+    const unsigned some = __ballot_sync(0xffffffffu, in);
+    unsigned same = in ? some : ~some;
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (digit >> b) & 1u;
+        const unsigned ones = __ballot_sync(0xffffffffu, one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
 }
 
 __global__ void __launch_bounds__(RS_THREADS) sort_count_kernel(const SortArgs a) {
     __shared__ unsigned h[RS_BINS];
-    const unsigned mask = (1u << a.bits) - 1u;
-    h[threadIdx.x] = 0;
+    const unsigned bins = 1u << a.bits, mask = bins - 1u;
+    for (unsigned b = threadIdx.x; b < bins; b += RS_THREADS) h[b] = 0;
     __syncthreads();
     const unsigned base = blockIdx.x * RS_TILE;
-#pragma unroll 4
+#pragma unroll 8
     for (int r = 0; r < RS_ROUNDS; ++r) {
         const unsigned i = base + r * RS_THREADS + threadIdx.x;
-        if (i < a.n) atomicAdd(&h[(sort_key(a, i) >> a.shift) & mask], 1u);
+        if (i >= a.n) continue;
+        const unsigned key = a.first ? index_key(a, i) : __ldg(&a.in[i].x);
+        atomicAdd(&h[(key >> a.shift) & mask], 1u);
+        if (a.first && a.dweight && key == (unsigned)a.rows) a.dweight[i] = 0.0f;
     }
     __syncthreads();
-    if (threadIdx.x <= mask) a.hist[(size_t)threadIdx.x * a.tiles + blockIdx.x] = h[threadIdx.x];
+    for (unsigned b = threadIdx.x; b < bins; b += RS_THREADS) a.hist[(size_t)b * a.tiles + blockIdx.x] = h[b];
 }
 
 // exclusive sum over the block, `total` gets the sum of all
@@ -209,7 +231,8 @@ __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned *warp_s
     if (lane == 31) warp_sums[w] = inc;
     __syncthreads();
     unsigned before = 0, all = 0;
-    for (int k = 0; k < (int)(blockDim.x >> 5); ++k) {
+#pragma unroll
+    for (int k = 0; k < RS_WARPS; ++k) {
         if (k < w) before += warp_sums[k];
         all += warp_sums[k];
     }
@@ -234,63 +257,126 @@ __global__ void __launch_bounds__(RS_THREADS) sort_scan_kernel(const SortArgs a)
     if (threadIdx.x == 0) a.total[blockIdx.x] = carry;
 }
 
+// counts entry (of digit d) into its warp's counters; its rank among the warp's entries of that digit
+__device__ __forceinline__ unsigned warp_rank(unsigned short *cnt, unsigned d, int bits, bool in) {
+    const int lane = threadIdx.x & 31;
+    const unsigned same = lanes_with(d, bits, in);
+    const unsigned below = __popc(same & ((1u << lane) - 1u));
+    const unsigned before = in ? cnt[d] : 0u;
+    __syncwarp();
+    if (in && below == 0) cnt[d] = (unsigned short)(before + __popc(same));
+    __syncwarp();
+    return before + below;
+}
+
 __global__ void __launch_bounds__(RS_THREADS) sort_scatter_kernel(const SortArgs a) {
-    __shared__ unsigned cnt[RS_WARPS][RS_BINS];
+    extern __shared__ unsigned smem[];
     __shared__ unsigned sums[RS_WARPS];
+    const unsigned bins = 1u << a.bits, mask = bins - 1u;
+    unsigned *at = smem;                                                   // (bins): first position of the tile's entries of a digit
+    unsigned short *cnt = reinterpret_cast<unsigned short *>(smem + bins); // (warps, bins)
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const unsigned mask = (1u << a.bits) - 1u;
-    for (int k = 0; k < RS_WARPS; ++k) cnt[k][threadIdx.x] = 0;
-    __syncthreads();
+    for (unsigned b = threadIdx.x; b < bins * RS_WARPS / 2; b += RS_THREADS) smem[bins + b] = 0;
     const unsigned base = blockIdx.x * RS_TILE + w * (32 * RS_ROUNDS) + lane;
-    unsigned key[RS_ROUNDS], val[RS_ROUNDS], rank[RS_ROUNDS];
+    uint2 e[RS_ROUNDS];
+    unsigned short rank[RS_ROUNDS];
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) {
-        const unsigned i = base + r * 32;
-        key[r] = i < a.n ? sort_key(a, i) : 0u;
-        val[r] = i < a.n ? (a.first ? i : a.val_in[i]) : 0u;
-    }
-#pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) {
-        const bool in = base + r * 32 < a.n;
-        const unsigned d = in ? (key[r] >> a.shift) & mask : RS_BINS;  // lanes past the end match one another only
-        const unsigned same = __match_any_sync(0xffffffffu, d);
-        const unsigned below = __popc(same & ((1u << lane) - 1u));
-        const unsigned before = in ? cnt[w][d] : 0u;
-        rank[r] = before + below;
-        __syncwarp();
-        if (in && below == 0) cnt[w][d] = before + __popc(same);
-        __syncwarp();
-    }
+    for (int r = 0; r < RS_ROUNDS; ++r) e[r] = base + r * 32 < a.n ? sort_entry(a, base + r * 32) : make_uint2(0, 0);
     __syncthreads();
-    {   // counts become first positions: digits before this one, tiles before this one, warps before this one
+#pragma unroll
+    for (int r = 0; r < RS_ROUNDS; ++r)
+        rank[r] = (unsigned short)warp_rank(cnt + w * bins, (e[r].x >> a.shift) & mask, a.bits, base + r * 32 < a.n);
+    __syncthreads();
+    // first positions: digits before this one, tiles before this one; then warps before this one
+    unsigned carry = 0;
+    for (unsigned b0 = 0; b0 < bins; b0 += RS_THREADS) {
+        const unsigned d = b0 + threadIdx.x;
         unsigned all;
-        const unsigned d = threadIdx.x;
-        const unsigned digit = block_exclusive(d <= mask ? a.total[d] : 0u, sums, &all);
-        if (d <= mask) {
-            unsigned at = digit + a.hist[(size_t)d * a.tiles + blockIdx.x];
+        const unsigned digit = block_exclusive(d < bins ? a.total[d] : 0u, sums, &all);
+        if (d < bins) {
+            at[d] = carry + digit + a.hist[(size_t)d * a.tiles + blockIdx.x];
+            unsigned short before = 0;
+#pragma unroll
             for (int k = 0; k < RS_WARPS; ++k) {
-                const unsigned c = cnt[k][d];
-                cnt[k][d] = at;
-                at += c;
+                const unsigned short c = cnt[k * bins + d];
+                cnt[k * bins + d] = before;
+                before += c;
             }
         }
+        carry += all;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RS_ROUNDS; ++r) {
         if (base + r * 32 >= a.n) continue;
-        const unsigned pos = cnt[w][(key[r] >> a.shift) & mask] + rank[r];
-        a.key_out[pos] = key[r];
-        a.val_out[pos] = val[r];
+        const unsigned d = (e[r].x >> a.shift) & mask;
+        const unsigned pos = at[d] + cnt[w * bins + d] + rank[r];
+        if (a.last) {
+            a.key_out[pos] = e[r].x;
+            a.val_out[pos] = e[r].y;
+        } else {
+            a.out[pos] = e[r];
+        }
     }
+}
+
+// at most one tile: all digits by one block, entries in registers between passes through shared memory
+__global__ void __launch_bounds__(RS_THREADS) sort_small_kernel(const SortArgs a) {
+    constexpr unsigned BINS = 1u << RS_SMALL_BITS;
+    __shared__ uint2 entry[RS_TILE];
+    __shared__ unsigned short cnt[RS_WARPS * BINS];
+    __shared__ unsigned at[BINS], sums[RS_WARPS];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const unsigned base = w * (32 * RS_ROUNDS) + lane;
+    uint2 e[RS_ROUNDS];
+    unsigned short rank[RS_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < RS_ROUNDS; ++r) {
+        const unsigned i = base + r * 32;
+        e[r] = i < a.n ? make_uint2(index_key(a, i), i) : make_uint2(0, 0);
+        if (i < a.n && a.dweight && e[r].x == (unsigned)a.rows) a.dweight[i] = 0.0f;
+    }
+    for (int shift = 0; shift < a.key_bits; shift += RS_SMALL_BITS) {
+        for (unsigned b = threadIdx.x; b < BINS * RS_WARPS / 2; b += RS_THREADS) reinterpret_cast<unsigned *>(cnt)[b] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RS_ROUNDS; ++r)
+            rank[r] = (unsigned short)warp_rank(cnt + w * BINS, (e[r].x >> shift) & (BINS - 1), RS_SMALL_BITS, base + r * 32 < a.n);
+        __syncthreads();
+        unsigned all = 0, before = 0;
+#pragma unroll
+        for (int k = 0; k < RS_WARPS; ++k) {
+            const unsigned c = cnt[k * BINS + threadIdx.x];
+            cnt[k * BINS + threadIdx.x] = (unsigned short)before;
+            before += c;
+        }
+        at[threadIdx.x] = block_exclusive(before, sums, &all);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RS_ROUNDS; ++r) {
+            const unsigned d = (e[r].x >> shift) & (BINS - 1);
+            if (base + r * 32 < a.n) entry[at[d] + cnt[w * BINS + d] + rank[r]] = e[r];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RS_ROUNDS; ++r)
+            if (base + r * 32 < a.n) e[r] = entry[base + r * 32];
+    }
+#pragma unroll
+    for (int r = 0; r < RS_ROUNDS; ++r)
+        if (base + r * 32 < a.n) {
+            a.key_out[base + r * 32] = e[r].x;
+            a.val_out[base + r * 32] = e[r].y;
+        }
 }
 
 // ------------------------------------------------------------------------------------------------
 // Sums per row.  A row whose entries fill a whole aligned chunk of LG_CHUNK sorted entries is "long": its chunks are
 // summed by blocks of their own into partial rows, and the partial rows are added in order; all others are added
-// by a group of lanes.
+// by a group of lanes.  Where a lane's one vector covers its share of the columns (DOT), the same pass forms dweight:
+// the entry's dout row is in registers, and the table's row is read once for all its entries.
 // ------------------------------------------------------------------------------------------------
-constexpr int LG_THREADS = 256, LG_CHUNK = 256;
+constexpr int LG_THREADS = 256, LG_WARPS = LG_THREADS / 32, LG_CHUNK = 256;
 
 struct GradArgs {
     const void *dout, *table, *index;
@@ -298,8 +384,8 @@ struct GradArgs {
     float *dtable, *dweight, *partial;  // partial: (2 * chunks, width)
     const unsigned *key, *order;
     long long rows, dout_stride, table_stride;
-    unsigned n;
-    int width, index_type;
+    unsigned n, chunks, chunk_blocks, col_tiles;  // chunk_blocks * col_tiles blocks work on chunks, those behind them on rows
+    int width, index_type, rows_per_warp;
     float scale;
 };
 
@@ -322,11 +408,12 @@ __device__ __forceinline__ bool is_long(unsigned s, unsigned e) {
     return full + LG_CHUNK <= e;
 }
 
-// acc += sum over sorted entries [s, e) of scale * weight * dout, columns col0 + (lane-owned vectors)
-template <class D, int VE, int NV>
+// acc += sum over sorted entries s, s + step, ... below e of scale * weight * dout, columns col, col + col_step, ...
+// DOT: also dweight of those entries, e the table row's columns, summed over the G lanes of `lanes`
+template <class D, int VE, int NV, int G, bool DOT>
 __device__ __forceinline__ void add_entries(const GradArgs &a, unsigned s, unsigned e, unsigned step, int col, int col_step,
-                                            float (&acc)[NV][VE]) {
-    constexpr int U = 4;  // entries in flight
+                                            float (&acc)[NV][VE], const float (&row)[VE], unsigned lanes) {
+    constexpr int U = NV == 1 ? 4 : 2;  // entries in flight
     for (unsigned j = s; j < e; j += step * U) {
         unsigned i[U];
         float f[U];
@@ -345,12 +432,23 @@ __device__ __forceinline__ void add_entries(const GradArgs &a, unsigned s, unsig
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i[u] != 0xffffffffu)
+        for (int u = 0; u < U; ++u) {
+            if (i[u] == 0xffffffffu) break;
+            float dot = 0.0f;
 #pragma unroll
-                for (int q = 0; q < NV; ++q)
+            for (int q = 0; q < NV; ++q)
 #pragma unroll
-                    for (int v = 0; v < VE; ++v) acc[q][v] = fmaf(f[u], d[u][q].get(v), acc[q][v]);
+                for (int v = 0; v < VE; ++v) {
+                    const float x = d[u][q].get(v);
+                    acc[q][v] = fmaf(f[u], x, acc[q][v]);
+                    if (DOT) dot = fmaf(x, row[v], dot);
+                }
+            if (DOT) {
+#pragma unroll
+                for (int o = G / 2; o; o >>= 1) dot += __shfl_xor_sync(lanes, dot, o);
+                if (col == 0) a.dweight[i[u]] = a.scale * dot;
+            }
+        }
     }
 }
 
@@ -359,38 +457,55 @@ __device__ __forceinline__ void store_row(float *p, const float (&acc)[VE]) {
     Vec<float, VE> o;
 #pragma unroll
     for (int v = 0; v < VE; ++v) o.el[v] = acc[v];
-    o.store(p);
+    o.store_stream(p);
 }
 
-// Block c: the part of the rows at chunk c's ends that are long -> partial rows 2c (the row that the chunk begins
-// with) and 2c + 1 (the row that begins inside it).  grid.y: column tiles of 32 VE.
-template <class D, int VE>
-__global__ void __launch_bounds__(LG_THREADS) grad_chunk_kernel(const GradArgs a) {
-    constexpr int W = LG_THREADS / 32;
-    __shared__ float part[W][32 * VE];
-    const unsigned c0 = blockIdx.x * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n);
+template <class T, int VE>
+__device__ __forceinline__ void load_row(const GradArgs &a, long long p, int col, bool some, float (&row)[VE]) {
+    Vec<T, VE> t;
+    if (some && col < a.width) t.load_stream(static_cast<const T *>(a.table) + p * a.table_stride + col);
+    else t.zero();
+#pragma unroll
+    for (int v = 0; v < VE; ++v) row[v] = t.get(v);
+}
+
+// whether the row that chunk c begins with (side 0) or the one that it ends with (1) is long.  The keys are sorted, so
+// equal keys at both ends of a chunk mean that all of it is one row.
+__device__ __forceinline__ bool chunk_long(const GradArgs &a, unsigned c, int side) {
+    const unsigned c0 = c * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n);
     const unsigned first = __ldg(a.key + c0), last = __ldg(a.key + c1 - 1);
+    if ((side ? last : first) >= (unsigned)a.rows) return false;  // entries without a row
+    if (side == 0) return (c0 + LG_CHUNK <= a.n && last == first) || (c0 >= LG_CHUNK && __ldg(a.key + c0 - LG_CHUNK) == first);
+    return last != first && c1 + LG_CHUNK <= a.n && __ldg(a.key + c1 + LG_CHUNK - 1) == last;
+}
+
+// Eight chunks per block: the part of the rows at a chunk's ends that are long -> partial rows 2c (the row that the
+// chunk begins with) and 2c + 1 (the row that begins inside it).  Column tiles of 32 VE.
+template <class D, class T, int VE, bool DOT>
+__device__ __forceinline__ void grad_chunks(const GradArgs &a, unsigned block, unsigned col_tile) {
+    __shared__ float part[LG_WARPS][32 * VE];
+    __shared__ unsigned todo;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int col = (blockIdx.y * 32 + lane) * VE;
-    for (int side = 0; side < 2; ++side) {
-        const unsigned row = side ? last : first;
-        if (side && last == first) break;
-        if (row >= (unsigned)a.rows) break;  // entries without a row
-        // the keys are sorted, so equal keys at both ends of a chunk mean that all of it is this row
-        bool lng;
-        if (side == 0)
-            lng = (c0 + LG_CHUNK <= a.n && last == first) || (c0 >= LG_CHUNK && __ldg(a.key + c0 - LG_CHUNK) == first);
-        else lng = c1 + LG_CHUNK <= a.n && __ldg(a.key + c1 + LG_CHUNK - 1) == last;
-        if (!lng) continue;
+    if (w == 0) {
+        const unsigned c = block * LG_WARPS + (lane >> 1);
+        const unsigned mask = __ballot_sync(0xffffffffu, lane < 2 * LG_WARPS && c < a.chunks && chunk_long(a, c, lane & 1));
+        if (lane == 0) todo = mask;
+    }
+    __syncthreads();
+    const int col = (col_tile * 32 + lane) * VE;
+    for (unsigned left = todo; left; left &= left - 1) {
+        const int bit = __ffs(left) - 1, side = bit & 1;
+        const unsigned c = block * LG_WARPS + (bit >> 1), c0 = c * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n);
+        const unsigned first = __ldg(a.key + c0), last = __ldg(a.key + c1 - 1);
         unsigned s = c0, e = c1;
         if (first != last) {
             const unsigned cut = c0 + lower_bound(a.key + c0, c1 - c0, side ? last : first + 1);
             if (side) s = cut;
             else e = cut;
         }
-        float acc[1][VE] = {};
-        add_entries<D, VE, 1>(a, s + w, e, W, col, 0, acc);
-        __syncthreads();
+        float acc[1][VE] = {}, row[VE];
+        if (DOT) load_row<T, VE>(a, side ? last : first, col, true, row);
+        add_entries<D, VE, 1, 32, DOT>(a, s + w, e, LG_WARPS, col, 0, acc, row, 0xffffffffu);
 #pragma unroll
         for (int v = 0; v < VE; ++v) part[w][lane * VE + v] = acc[0][v];
         __syncthreads();
@@ -398,77 +513,88 @@ __global__ void __launch_bounds__(LG_THREADS) grad_chunk_kernel(const GradArgs a
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
                 float t = 0.0f;
-                for (int k = 0; k < W; ++k) t += part[k][lane * VE + v];
+                for (int k = 0; k < LG_WARPS; ++k) t += part[k][lane * VE + v];
                 acc[0][v] = t;
             }
-            store_row<VE>(a.partial + ((size_t)2 * blockIdx.x + side) * a.width + col, acc[0]);
+            store_row<VE>(a.partial + ((size_t)2 * c + side) * a.width + col, acc[0]);
         }
         __syncthreads();
     }
 }
 
-// Block c: if a long row begins in chunk c, adds its partial rows in order and writes the row.
+// Eight chunks per block: for a long row that begins in one of them, adds its partial rows in order and writes the row.
 template <int VE>
 __global__ void __launch_bounds__(LG_THREADS) grad_join_kernel(const GradArgs a) {
-    constexpr int W = LG_THREADS / 32;
-    __shared__ float part[W][32 * VE];
-    const unsigned c0 = blockIdx.x * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n);
-    const unsigned row = __ldg(a.key + c1 - 1);  // the only row that can begin here and be long
-    if (row >= (unsigned)a.rows) return;
-    const unsigned s = lower_bound(a.key, a.n, row);
-    if (s < c0) return;  // it began before
-    const unsigned e = lower_bound(a.key, a.n, row + 1);
-    if (!is_long(s, e)) return;
+    __shared__ float part[LG_WARPS][32 * VE];
+    __shared__ unsigned todo;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int col = (blockIdx.y * 32 + lane) * VE;
-    const unsigned last = (e - 1) / LG_CHUNK;
-    float acc[VE] = {};
-    if (col < a.width) {
-#pragma unroll 4
-        for (unsigned c = blockIdx.x + w; c <= last; c += W) {
-            // the row's part of its first chunk is side 1 unless the chunk begins with it
-            const unsigned slot = 2 * c + (c == blockIdx.x && s != c0 ? 1 : 0);
-            Vec<float, VE> d;
-            d.load(a.partial + (size_t)slot * a.width + col);
-#pragma unroll
-            for (int v = 0; v < VE; ++v) acc[v] += d.el[v];
+    if (w == 0) {
+        // a long row begins in c if it is what c ends with and c is where it starts: inside c (side 1), or at its first entry
+        const unsigned c = blockIdx.x * LG_WARPS + lane;
+        bool begins = false;
+        if (lane < LG_WARPS && c < a.chunks) {
+            const unsigned c0 = c * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n), first = __ldg(a.key + c0);
+            begins = chunk_long(a, c, 1) || (__ldg(a.key + c1 - 1) == first && chunk_long(a, c, 0) &&
+                                             (c0 == 0 || __ldg(a.key + c0 - 1) != first));
         }
+        const unsigned mask = __ballot_sync(0xffffffffu, begins);
+        if (lane == 0) todo = mask;
     }
-#pragma unroll
-    for (int v = 0; v < VE; ++v) part[w][lane * VE + v] = acc[v];
     __syncthreads();
-    if (w == 0 && col < a.width) {
+    const int col = (blockIdx.y * 32 + lane) * VE;
+    for (unsigned left = todo; left; left &= left - 1) {
+        const unsigned b = blockIdx.x * LG_WARPS + __ffs(left) - 1, c0 = b * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n);
+        const unsigned row = __ldg(a.key + c1 - 1);
+        const bool inside = __ldg(a.key + c0) != row;
+        const unsigned e = c0 + lower_bound(a.key + c0, a.n - c0, row + 1), last = (e - 1) / LG_CHUNK;
+        float acc[VE] = {};
+        if (col < a.width) {
+#pragma unroll 4
+            for (unsigned c = b + w; c <= last; c += LG_WARPS) {
+                const unsigned slot = 2 * c + (c == b && inside ? 1 : 0);
+                Vec<float, VE> d;
+                d.load(a.partial + (size_t)slot * a.width + col);
 #pragma unroll
-        for (int v = 0; v < VE; ++v) {
-            float t = 0.0f;
-            for (int k = 0; k < W; ++k) t += part[k][lane * VE + v];
-            acc[v] = t;
+                for (int v = 0; v < VE; ++v) acc[v] += d.el[v];
+            }
         }
-        store_row<VE>(a.dtable + (size_t)row * a.width + col, acc);
+#pragma unroll
+        for (int v = 0; v < VE; ++v) part[w][lane * VE + v] = acc[v];
+        __syncthreads();
+        if (w == 0 && col < a.width) {
+#pragma unroll
+            for (int v = 0; v < VE; ++v) {
+                float t = 0.0f;
+                for (int k = 0; k < LG_WARPS; ++k) t += part[k][lane * VE + v];
+                acc[v] = t;
+            }
+            store_row<VE>(a.dtable + (size_t)row * a.width + col, acc);
+        }
+        __syncthreads();
     }
 }
 
-// A group of G lanes per row (32 / G rows per warp), each lane NV vectors of VE columns per column tile.
-template <class D, int VE, int NV, int G>
-__global__ void __launch_bounds__(LG_THREADS) grad_rows_kernel(const GradArgs a) {
+// A group of G lanes per row (32 / G rows at a time per warp), each lane NV vectors of VE columns per column tile.
+template <class D, class T, int VE, int NV, int G, bool DOT>
+__device__ __forceinline__ void grad_rows(const GradArgs &a, unsigned block) {
     constexpr int RPW = 32 / G;
     const int lane = threadIdx.x & 31, sub = lane % G;
-    const long long warp = ((long long)blockIdx.x * LG_THREADS + threadIdx.x) >> 5;
-    // the warp's 32 rows: lane k finds where row 32 warp + k begins
-    const long long row0 = warp * 32;
+    const unsigned lanes = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (lane / G * G);
+    const long long warp = (long long)block * LG_WARPS + (threadIdx.x >> 5), row0 = warp * a.rows_per_warp;
     if (row0 >= a.rows) return;
+    // lane k finds where row row0 + k begins; the last lane's row ends where the next one begins
     const unsigned begin = lower_bound(a.key, a.n, (unsigned)min(row0 + lane, a.rows));
-    const unsigned end31 = lower_bound(a.key, a.n, (unsigned)min(row0 + 32, a.rows));
-    for (int r = 0; r < 32; r += RPW) {
+    const unsigned after = lower_bound(a.key, a.n, (unsigned)min(row0 + 32, a.rows));
+    for (int r = 0; r < a.rows_per_warp; r += RPW) {
         const int k = r + lane / G;
-        const unsigned s = __shfl_sync(0xffffffffu, begin, k);
-        const unsigned nxt = __shfl_sync(0xffffffffu, begin, (k + 1) & 31);
-        const unsigned e = k == 31 ? end31 : nxt;
+        const unsigned s = __shfl_sync(0xffffffffu, begin, k & 31), next = __shfl_sync(0xffffffffu, begin, (k + 1) & 31);
+        const unsigned e = k == 31 ? after : next;
         const long long row = row0 + k;
-        if (row >= a.rows || is_long(s, e)) continue;
+        if (row >= a.rows || k >= a.rows_per_warp || is_long(s, e)) continue;
         for (int c0 = 0; c0 < a.width; c0 += G * NV * VE) {
-            float acc[NV][VE] = {};
-            add_entries<D, VE, NV>(a, s, e, 1, c0 + sub * VE, G * VE, acc);
+            float acc[NV][VE] = {}, held[VE];
+            if (DOT) load_row<T, VE>(a, row, c0 + sub * VE, s < e, held);
+            add_entries<D, VE, NV, G, DOT>(a, s, e, 1, c0 + sub * VE, G * VE, acc, held, lanes);
 #pragma unroll
             for (int q = 0; q < NV; ++q) {
                 const int c = c0 + sub * VE + q * G * VE;
@@ -476,6 +602,13 @@ __global__ void __launch_bounds__(LG_THREADS) grad_rows_kernel(const GradArgs a)
             }
         }
     }
+}
+
+template <class D, class T, int VE, int NV, int G, bool DOT>
+__global__ void __launch_bounds__(LG_THREADS) grad_sum_kernel(const GradArgs a) {
+    const unsigned chunk_part = a.chunk_blocks * a.col_tiles;
+    if (blockIdx.x < chunk_part) grad_chunks<D, T, VE, DOT>(a, blockIdx.x % a.chunk_blocks, blockIdx.x / a.chunk_blocks);
+    else grad_rows<D, T, VE, NV, G, DOT>(a, blockIdx.x - chunk_part);
 }
 
 // dweight: a warp per entry.
@@ -506,56 +639,109 @@ __global__ void zero_kernel(float *p, long long n) {
 }
 
 struct GradPlan {
-    long long key[2], val[2], hist, total, partial, bytes;
+    long long entries[2], key, val, hist, total, partial, bytes;
     unsigned tiles, chunks;
+    int bits, passes;
 };
 
-GradPlan grad_plan(long long n, int width) {
+GradPlan grad_plan(long long rows, long long n, int width) {
     GradPlan g{};
     g.tiles = (unsigned)((n + RS_TILE - 1) / RS_TILE);
     g.chunks = (unsigned)((n + LG_CHUNK - 1) / LG_CHUNK);
+    g.bits = 1;
+    while ((rows >> g.bits) != 0) ++g.bits;  // keys are 0 .. rows
+    g.passes = (g.bits + RS_MAX_BITS - 1) / RS_MAX_BITS;
     long long at = 0;
     auto take = [&](long long bytes) {
         const long long p = at;
         at += (bytes + 255) / 256 * 256;
         return p;
     };
-    for (int b = 0; b < 2; ++b) g.key[b] = take(4 * n);
-    for (int b = 0; b < 2; ++b) g.val[b] = take(4 * n);
-    g.hist = take(4ll * RS_BINS * g.tiles);
-    g.total = take(4ll * RS_BINS);
+    g.key = take(4 * n);
+    g.val = take(4 * n);
+    if (g.tiles > 1) {
+        for (int b = 0; b < 2; ++b) g.entries[b] = take(b < g.passes - 1 ? 8 * n : 0);
+        g.hist = take((4ll << (g.bits + g.passes - 1) / g.passes) * g.tiles);
+        g.total = take(4ll * RS_BINS);
+    }
     // only rows that fill a chunk have partial rows
     g.partial = take(n >= LG_CHUNK ? 8ll * g.chunks * width : 0);
     g.bytes = at;
     return g;
 }
 
-template <class D>
-void launch_grad(const GradArgs &a, int ve, unsigned chunks, cudaStream_t st) {
-    auto go = [&](auto tag) {
-        constexpr int VE = decltype(tag)::value;
-        const int vectors = a.width / VE;
-        if (a.n >= LG_CHUNK) {
-            const dim3 grid(chunks, (vectors + 31) / 32);
-            grad_chunk_kernel<D, VE><<<grid, LG_THREADS, 0, st>>>(a);
+int sort_entries(const flare_lookup_grad_args *in, const GradPlan &g, bool dot, cudaStream_t st) {
+    char *ws = static_cast<char *>(in->workspace);
+    auto words = [&](long long at) { return reinterpret_cast<unsigned *>(ws + at); };
+    SortArgs s{};
+    s.index = in->index;
+    s.index_type = in->index_type;
+    s.key_out = words(g.key);
+    s.val_out = words(g.val);
+    s.dweight = dot ? in->dweight : nullptr;
+    s.rows = in->rows;
+    s.n = (unsigned)in->n;
+    s.tiles = g.tiles;
+    s.key_bits = g.bits;
+    if (g.tiles == 1) {
+        sort_small_kernel<<<1, RS_THREADS, 0, st>>>(s);
+    } else {
+        s.hist = words(g.hist);
+        s.total = words(g.total);
+        for (int p = 0; p < g.passes; ++p) {
+            s.first = p == 0;
+            s.last = p == g.passes - 1;
+            s.bits = (g.bits - s.shift + (g.passes - p) - 1) / (g.passes - p);
+            s.in = reinterpret_cast<uint2 *>(ws + g.entries[(p + 1) & 1]);
+            s.out = reinterpret_cast<uint2 *>(ws + g.entries[p & 1]);
+            const size_t smem = (4 + 2 * RS_WARPS) << s.bits;
+            sort_count_kernel<<<g.tiles, RS_THREADS, 0, st>>>(s);
+            sort_scan_kernel<<<1u << s.bits, RS_THREADS, 0, st>>>(s);
+            sort_scatter_kernel<<<g.tiles, RS_THREADS, smem, st>>>(s);
+            s.shift += s.bits;
         }
-        const unsigned blocks = (unsigned)((a.rows + 32 * (LG_THREADS / 32) - 1) / (32 * (LG_THREADS / 32)));
-        if (vectors <= 4) grad_rows_kernel<D, VE, 1, 4><<<blocks, LG_THREADS, 0, st>>>(a);
-        else if (vectors <= 8) grad_rows_kernel<D, VE, 1, 8><<<blocks, LG_THREADS, 0, st>>>(a);
-        else if (vectors <= 16) grad_rows_kernel<D, VE, 1, 16><<<blocks, LG_THREADS, 0, st>>>(a);
-        else if (vectors <= 32) grad_rows_kernel<D, VE, 1, 32><<<blocks, LG_THREADS, 0, st>>>(a);
-        else grad_rows_kernel<D, VE, 4, 32><<<blocks, LG_THREADS, 0, st>>>(a);
-        if (a.n >= LG_CHUNK) {
-            const dim3 grid(chunks, (vectors + 31) / 32);
-            grad_join_kernel<VE><<<grid, LG_THREADS, 0, st>>>(a);
-        }
-    };
-    switch (ve) {
-        case 8: go(std::integral_constant<int, 8>{}); break;
-        case 4: go(std::integral_constant<int, 4>{}); break;
-        case 2: go(std::integral_constant<int, 2>{}); break;
-        default: go(std::integral_constant<int, 1>{}); break;
     }
+    OPS_LAUNCHED("flare_lookup_backward");
+    return FLARE_OK;
+}
+
+template <int VE>
+using Width = std::integral_constant<int, VE>;
+template <class F>
+void with_width(int ve, F f) {
+    switch (ve) {
+        case 8: f(Width<8>{}); break;
+        case 4: f(Width<4>{}); break;
+        case 2: f(Width<2>{}); break;
+        default: f(Width<1>{}); break;
+    }
+}
+
+template <class D, class T, int VE, bool DOT>
+void launch_sums(GradArgs a, cudaStream_t st) {
+    const int vectors = a.width / VE;
+    a.col_tiles = (vectors + 31) / 32;
+    a.chunk_blocks = a.n >= LG_CHUNK ? (a.chunks + LG_WARPS - 1) / LG_WARPS : 0;
+    // 32 rows a warp share a search; fewer where that leaves the machine without warps
+    a.rows_per_warp = 32;
+    while (a.rows_per_warp > 8 && a.rows / a.rows_per_warp < 64 * SMS) a.rows_per_warp /= 2;
+    const long long per_block = (long long)a.rows_per_warp * LG_WARPS;
+    const unsigned grid = a.chunk_blocks * a.col_tiles + (unsigned)((a.rows + per_block - 1) / per_block);
+    if (vectors <= 8) grad_sum_kernel<D, T, VE, 1, 8, DOT><<<grid, LG_THREADS, 0, st>>>(a);
+    else if (vectors <= 16) grad_sum_kernel<D, T, VE, 1, 16, DOT><<<grid, LG_THREADS, 0, st>>>(a);
+    else if (vectors <= 32) grad_sum_kernel<D, T, VE, 1, 32, DOT><<<grid, LG_THREADS, 0, st>>>(a);
+    else if constexpr (!DOT) grad_sum_kernel<D, T, VE, 4, 32, false><<<grid, LG_THREADS, 0, st>>>(a);
+    if (a.chunk_blocks) grad_join_kernel<VE><<<dim3(a.chunk_blocks, a.col_tiles), LG_THREADS, 0, st>>>(a);
+}
+
+// widest vectors that all the given tensors allow
+int grad_vec(const flare_lookup_grad_args *in, bool dtable, bool table) {
+    int ve = 8;
+    while (ve > 1 && !(in->width % ve == 0 && fits_vec(in->dout, in->dout_stride, type_size(in->dout_type), ve) &&
+                       (!dtable || fits_vec(in->dtable, in->width, 4, ve)) &&
+                       (!table || fits_vec(in->table, in->table_stride, type_size(in->table_type), ve))))
+        ve >>= 1;
+    return ve;
 }
 
 int run_lookup_backward(const flare_lookup_grad_args *in, cudaStream_t st) {
@@ -581,63 +767,39 @@ int run_lookup_backward(const flare_lookup_grad_args *in, cudaStream_t st) {
         }
         return FLARE_OK;
     }
-    if (in->dtable && in->rows) {
-        const GradPlan g = grad_plan(in->n, in->width);
+    const bool sums = in->dtable && in->rows;
+    // both gradients in one pass where a row's columns are one vector a lane
+    const int both = sums && in->dweight ? grad_vec(in, true, true) : 0;
+    const bool dot = both && in->width / both <= 32;
+    if (sums) {
+        const GradPlan g = grad_plan(in->rows, in->n, in->width);
         char *ws = static_cast<char *>(in->workspace);
-        SortArgs s{};
-        s.index = in->index;
-        s.index_type = in->index_type;
-        s.hist = reinterpret_cast<unsigned *>(ws + g.hist);
-        s.total = reinterpret_cast<unsigned *>(ws + g.total);
-        s.rows = in->rows;
-        s.n = a.n;
-        s.tiles = g.tiles;
-        int bits = 1;
-        while ((in->rows >> bits) != 0) ++bits;  // keys are 0 .. rows
-        const int passes = (bits + RS_MAX_BITS - 1) / RS_MAX_BITS;
-        for (int p = 0, shift = 0; p < passes; ++p) {
-            s.first = p == 0;
-            s.shift = shift;
-            s.bits = (bits - shift + (passes - p) - 1) / (passes - p);
-            s.key_in = reinterpret_cast<unsigned *>(ws + g.key[(p + 1) & 1]);
-            s.val_in = reinterpret_cast<unsigned *>(ws + g.val[(p + 1) & 1]);
-            s.key_out = reinterpret_cast<unsigned *>(ws + g.key[p & 1]);
-            s.val_out = reinterpret_cast<unsigned *>(ws + g.val[p & 1]);
-            sort_count_kernel<<<g.tiles, RS_THREADS, 0, st>>>(s);
-            sort_scan_kernel<<<1u << s.bits, RS_THREADS, 0, st>>>(s);
-            sort_scatter_kernel<<<g.tiles, RS_THREADS, 0, st>>>(s);
-            OPS_LAUNCHED("flare_lookup_backward");
-            shift += s.bits;
-        }
-        a.key = s.key_out;
-        a.order = s.val_out;
+        const int e = sort_entries(in, g, dot, st);
+        if (e) return e;
+        a.key = reinterpret_cast<unsigned *>(ws + g.key);
+        a.order = reinterpret_cast<unsigned *>(ws + g.val);
         a.partial = reinterpret_cast<float *>(ws + g.partial);
-        int ve = 8;
-        while (ve > 1 && !(in->width % ve == 0 && fits_vec(in->dout, in->dout_stride, type_size(in->dout_type), ve) &&
-                           fits_vec(in->dtable, in->width, 4, ve)))
-            ve >>= 1;
+        a.chunks = g.chunks;
         with_type(in->dout_type, [&](auto d) {
-            launch_grad<typename decltype(d)::type>(a, ve, g.chunks, st);
+            using D = typename decltype(d)::type;
+            if (dot)
+                with_type(in->table_type, [&](auto t) {
+                    with_width(both, [&](auto ve) { launch_sums<D, typename decltype(t)::type, decltype(ve)::value, true>(a, st); });
+                    return 0;
+                });
+            else with_width(grad_vec(in, true, false), [&](auto ve) { launch_sums<D, float, decltype(ve)::value, false>(a, st); });
             return 0;
         });
         OPS_LAUNCHED("flare_lookup_backward");
     }
-    if (in->dweight) {
-        int ve = 8;
-        while (ve > 1 && !(in->width % ve == 0 && fits_vec(in->dout, in->dout_stride, type_size(in->dout_type), ve) &&
-                           fits_vec(in->table, in->table_stride, type_size(in->table_type), ve)))
-            ve >>= 1;
+    if (in->dweight && !dot) {
         const unsigned blocks = (unsigned)std::min<long long>((in->n + 7) / 8, SMS * 64);
         with_type(in->dout_type, [&](auto d) {
             return with_type(in->table_type, [&](auto t) {
-                using D = typename decltype(d)::type;
-                using T = typename decltype(t)::type;
-                switch (ve) {
-                    case 8: grad_weight_kernel<D, T, 8><<<blocks, LG_THREADS, 0, st>>>(a); break;
-                    case 4: grad_weight_kernel<D, T, 4><<<blocks, LG_THREADS, 0, st>>>(a); break;
-                    case 2: grad_weight_kernel<D, T, 2><<<blocks, LG_THREADS, 0, st>>>(a); break;
-                    default: grad_weight_kernel<D, T, 1><<<blocks, LG_THREADS, 0, st>>>(a); break;
-                }
+                with_width(grad_vec(in, false, true), [&](auto ve) {
+                    grad_weight_kernel<typename decltype(d)::type, typename decltype(t)::type, decltype(ve)::value>
+                        <<<blocks, LG_THREADS, 0, st>>>(a);
+                });
                 return 0;
             });
         });
@@ -666,7 +828,7 @@ int flare_lookup(const flare_lookup_args *a, void *stream) {
 }
 
 long long flare_lookup_workspace(long long rows, long long n, int width) {
-    return rows > 0 && n > 0 && width > 0 ? grad_plan(n, width).bytes : 0;
+    return rows > 0 && n > 0 && width > 0 ? grad_plan(rows, n, width).bytes : 0;
 }
 
 int flare_lookup_backward(const flare_lookup_grad_args *a, void *stream) {
