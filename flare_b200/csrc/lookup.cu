@@ -14,7 +14,7 @@
 
 namespace flare {
 
-constexpr int LK_THREADS = 256, LK_ITEMS = 4;
+constexpr int LK_THREADS = 256, LK_BLOCKS = 16;  // per multiprocessor at most
 
 struct LookupArgs {
     const void *table;
@@ -57,54 +57,77 @@ __device__ __forceinline__ void micro_load(const LookupArgs &a, long long p, uns
     }
 }
 
-// One vector of VE elements per item, LK_ITEMS items in flight per thread so that the index loads and then the
-// row loads of several entries overlap.  T = void: a 4-bit table.
+// Items in flight per thread: 16-byte loads need no more than 2 (4: 224 us instead of 193 for 2.56M rows of 96 f16), narrow ones 4.
+template <class T, int VE>
+constexpr int lookup_items() {
+    if constexpr (std::is_void_v<T>) return 2;
+    else return VE * (int)sizeof(T) >= 16 ? 2 : 4;
+}
+
+// One vector of VE elements per item.  A block takes tiles of LK_THREADS * ITEMS items in turn and asks for the next tile's
+// indices while it waits for this tile's rows.  T = void: a 4-bit table.
 template <class T, class O, class I, int VE>
 __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const LookupArgs a) {
-    const unsigned base = blockIdx.x * (LK_THREADS * LK_ITEMS) + threadIdx.x;
-    long long p[LK_ITEMS];
-    unsigned row[LK_ITEMS], v[LK_ITEMS];
-    float f[LK_ITEMS][VE];
+    constexpr int ITEMS = lookup_items<T, VE>();
+    const unsigned tiles = (a.items + LK_THREADS * ITEMS - 1) / (LK_THREADS * ITEMS);
+    long long next[ITEMS];
+    float factor[ITEMS];
+    auto ask = [&](unsigned tile) {
 #pragma unroll
-    for (int k = 0; k < LK_ITEMS; ++k) {
-        const unsigned it = base + k * LK_THREADS;
-        p[k] = -1;
-        row[k] = a.vpr.div(it);
-        v[k] = it - row[k] * a.vpr.d;
-        if (it < a.items) p[k] = row_of<I>(a.index, a.first + row[k], a.rows);
-    }
-#pragma unroll
-    for (int k = 0; k < LK_ITEMS; ++k) {
-        if (p[k] < 0) {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) f[k][e] = 0.0f;
-            continue;
+        for (int k = 0; k < ITEMS; ++k) {
+            const unsigned it = tile * (LK_THREADS * ITEMS) + k * LK_THREADS + threadIdx.x;
+            next[k] = -1;
+            factor[k] = a.scale;
+            if (tile < tiles && it < a.items) {
+                const unsigned row = a.vpr.div(it);
+                next[k] = row_of<I>(a.index, a.first + row, a.rows);
+                if (a.weight) factor[k] = a.scale * __ldg(a.weight + a.first + row);
+            }
         }
-        const float s = a.weight ? a.scale * __ldg(a.weight + a.first + row[k]) : a.scale;
+    };
+    ask(blockIdx.x);
+    for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const unsigned base = tile * (LK_THREADS * ITEMS) + threadIdx.x;
+        long long p[ITEMS];
+        float s[ITEMS], f[ITEMS][VE];
+        unsigned row[ITEMS], v[ITEMS];
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            p[k] = next[k];
+            s[k] = factor[k];
+            row[k] = a.vpr.div(base + k * LK_THREADS);
+            v[k] = base + k * LK_THREADS - row[k] * a.vpr.d;
+        }
         if constexpr (std::is_void_v<T>) {
-            micro_load<VE>(a, p[k], v[k], f[k]);
-        } else {
-            Vec<T, VE> t;
-            t.load(static_cast<const T *>(a.table) + p[k] * a.table_stride + (long long)v[k] * VE);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) f[k][e] = t.get(e);
+            for (int k = 0; k < ITEMS; ++k)
+                if (p[k] >= 0) micro_load<VE>(a, p[k], v[k], f[k]);
+            ask(tile + gridDim.x);
+        } else {
+            Vec<T, VE> t[ITEMS];
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k)
+                if (p[k] >= 0) t[k].load(static_cast<const T *>(a.table) + p[k] * a.table_stride + (long long)v[k] * VE);
+            ask(tile + gridDim.x);
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) f[k][e] = t[k].get(e);
         }
 #pragma unroll
-        for (int e = 0; e < VE; ++e) f[k][e] *= s;
-    }
+        for (int k = 0; k < ITEMS; ++k) {
+            if (base + k * LK_THREADS >= a.items) break;
+            Vec<O, VE> o;
 #pragma unroll
-    for (int k = 0; k < LK_ITEMS; ++k) {
-        if (base + k * LK_THREADS >= a.items) break;
-        Vec<O, VE> o;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) o.set(e, f[k][e]);
-        o.store_stream(static_cast<O *>(a.out) + (a.first + row[k]) * a.out_stride + (long long)v[k] * VE);
+            for (int e = 0; e < VE; ++e) o.set(e, p[k] >= 0 ? f[k][e] * s[k] : 0.0f);
+            o.store_stream(static_cast<O *>(a.out) + (a.first + row[k]) * a.out_stride + (long long)v[k] * VE);
+        }
     }
 }
 
 template <class T, class O, class I>
 void launch_lookup(const LookupArgs &a, int ve, cudaStream_t st) {
-    const unsigned blocks = (a.items + LK_THREADS * LK_ITEMS - 1) / (LK_THREADS * LK_ITEMS);
+    const unsigned blocks = std::min((a.items + LK_THREADS - 1) / LK_THREADS, (unsigned)(LK_BLOCKS * SMS));
     switch (ve) {
         case 8: lookup_kernel<T, O, I, 8><<<blocks, LK_THREADS, 0, st>>>(a); break;
         case 4: lookup_kernel<T, O, I, 4><<<blocks, LK_THREADS, 0, st>>>(a); break;
@@ -159,13 +182,13 @@ int run_lookup(const flare_lookup_args *in, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------------------
 // Stable radix sort of the entries by row; entries that name no row get key `rows` and end behind all others.
-// Per digit of up to 11 bits: count per tile, scan over tiles, scatter.  A tile is 4096 consecutive entries of one block;
-// warp w ranks entries [512 w, 512 w + 512) of it 32 at a time, so ranks follow the entries' order.  Lanes with equal
+// Per digit of up to 10 bits: count per tile, scan over tiles, scatter.  A tile is 4096 consecutive entries of one block;
+// warp w ranks entries [256 w, 256 w + 256) of it 32 at a time, so ranks follow the entries' order.  Lanes with equal
 // digits find one another by a ballot per bit (match.any took three times the whole kernel's time).  Up to one tile of
 // entries is sorted by one block in shared memory.
 // ------------------------------------------------------------------------------------------------
-constexpr int RS_THREADS = 256, RS_WARPS = RS_THREADS / 32, RS_ROUNDS = 16, RS_TILE = RS_THREADS * RS_ROUNDS;
-constexpr int RS_MAX_BITS = 11, RS_BINS = 1 << RS_MAX_BITS, RS_SMALL_BITS = 8;
+constexpr int RS_THREADS = 512, RS_WARPS = RS_THREADS / 32, RS_ROUNDS = 8, RS_TILE = RS_THREADS * RS_ROUNDS;
+constexpr int RS_MAX_BITS = 10, RS_BINS = 1 << RS_MAX_BITS, RS_SMALL_BITS = 8;
 
 struct SortArgs {
     const void *index;              // first pass: keys come from the index, values are the entry numbers
@@ -186,18 +209,6 @@ __device__ __forceinline__ unsigned index_key(const SortArgs &a, unsigned i) {
 }
 __device__ __forceinline__ uint2 sort_entry(const SortArgs &a, unsigned i) {
     return a.first ? make_uint2(index_key(a, i), i) : a.in[i];
-}
-
-// lanes of the warp with the same `bits`-bit digit (and the same `in`)
-__device__ __forceinline__ unsigned lanes_with(unsigned digit, int bits, bool in) {
-    const unsigned some = __ballot_sync(0xffffffffu, in);
-    unsigned same = in ? some : ~some;
-    for (int b = 0; b < bits; ++b) {
-        const bool one = (digit >> b) & 1u;
-        const unsigned ones = __ballot_sync(0xffffffffu, one);
-        same &= one ? ones : ~ones;
-    }
-    return same;
 }
 
 __global__ void __launch_bounds__(RS_THREADS) sort_count_kernel(const SortArgs a) {
@@ -257,20 +268,39 @@ __global__ void __launch_bounds__(RS_THREADS) sort_scan_kernel(const SortArgs a)
     if (threadIdx.x == 0) a.total[blockIdx.x] = carry;
 }
 
-// counts entry (of digit d) into its warp's counters; its rank among the warp's entries of that digit
-__device__ __forceinline__ unsigned warp_rank(unsigned short *cnt, unsigned d, int bits, bool in) {
+// Ranks of a warp's RS_ROUNDS x 32 entries among those of equal digit; cnt (zeroed) ends as the digits' counts.  All ballots
+// come first, as they do not depend on one another; the rounds' counts do.
+__device__ __forceinline__ void warp_ranks(unsigned short *cnt, const uint2 (&e)[RS_ROUNDS], int shift, int bits, unsigned first, unsigned n,
+                                           unsigned short (&rank)[RS_ROUNDS]) {
     const int lane = threadIdx.x & 31;
-    const unsigned same = lanes_with(d, bits, in);
-    const unsigned below = __popc(same & ((1u << lane) - 1u));
-    const unsigned before = in ? cnt[d] : 0u;
-    __syncwarp();
-    if (in && below == 0) cnt[d] = (unsigned short)(before + __popc(same));
-    __syncwarp();
-    return before + below;
+    const unsigned mask = (1u << bits) - 1u;
+    unsigned same[RS_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < RS_ROUNDS; ++r) same[r] = __ballot_sync(0xffffffffu, first + r * 32 < n);
+#pragma unroll
+    for (int r = 0; r < RS_ROUNDS; ++r) same[r] = first + r * 32 < n ? same[r] : ~same[r];
+    for (int b = shift; b < shift + bits; ++b)
+#pragma unroll
+        for (int r = 0; r < RS_ROUNDS; ++r) {
+            const bool one = (e[r].x >> b) & 1u;
+            const unsigned ones = __ballot_sync(0xffffffffu, one);
+            same[r] &= one ? ones : ~ones;
+        }
+#pragma unroll
+    for (int r = 0; r < RS_ROUNDS; ++r) {
+        const bool in = first + r * 32 < n;
+        const unsigned d = (e[r].x >> shift) & mask, below = __popc(same[r] & ((1u << lane) - 1u));
+        const unsigned before = in ? cnt[d] : 0u;
+        __syncwarp();
+        if (in && below == 0) cnt[d] = (unsigned short)(before + __popc(same[r]));
+        __syncwarp();
+        rank[r] = (unsigned short)(before + below);
+    }
 }
 
-__global__ void __launch_bounds__(RS_THREADS) sort_scatter_kernel(const SortArgs a) {
-    extern __shared__ unsigned smem[];
+__global__ void __launch_bounds__(RS_THREADS, 2) sort_scatter_kernel(const SortArgs a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    unsigned *smem = reinterpret_cast<unsigned *>(raw);
     __shared__ unsigned sums[RS_WARPS];
     const unsigned bins = 1u << a.bits, mask = bins - 1u;
     unsigned *at = smem;                                                   // (bins): first position of the tile's entries of a digit
@@ -282,19 +312,27 @@ __global__ void __launch_bounds__(RS_THREADS) sort_scatter_kernel(const SortArgs
     unsigned short rank[RS_ROUNDS];
 #pragma unroll
     for (int r = 0; r < RS_ROUNDS; ++r) e[r] = base + r * 32 < a.n ? sort_entry(a, base + r * 32) : make_uint2(0, 0);
-    __syncthreads();
+    constexpr int PER = RS_BINS / RS_THREADS;
+    unsigned total[PER], hist[PER];  // asked for early, used after the ranks
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r)
-        rank[r] = (unsigned short)warp_rank(cnt + w * bins, (e[r].x >> a.shift) & mask, a.bits, base + r * 32 < a.n);
+    for (int k = 0; k < PER; ++k) {
+        const unsigned d = k * RS_THREADS + threadIdx.x;
+        total[k] = d < bins ? __ldg(a.total + d) : 0u;
+        hist[k] = d < bins ? __ldg(a.hist + (size_t)d * a.tiles + blockIdx.x) : 0u;
+    }
+    __syncthreads();
+    warp_ranks(cnt + w * bins, e, a.shift, a.bits, base, a.n, rank);
     __syncthreads();
     // first positions: digits before this one, tiles before this one; then warps before this one
     unsigned carry = 0;
-    for (unsigned b0 = 0; b0 < bins; b0 += RS_THREADS) {
-        const unsigned d = b0 + threadIdx.x;
+#pragma unroll
+    for (int b = 0; b < PER; ++b) {
+        const unsigned d = b * RS_THREADS + threadIdx.x;
+        if (b * RS_THREADS >= bins) break;
         unsigned all;
-        const unsigned digit = block_exclusive(d < bins ? a.total[d] : 0u, sums, &all);
+        const unsigned digit = block_exclusive(total[b], sums, &all);
         if (d < bins) {
-            at[d] = carry + digit + a.hist[(size_t)d * a.tiles + blockIdx.x];
+            at[d] = carry + digit + hist[b];
             unsigned short before = 0;
 #pragma unroll
             for (int k = 0; k < RS_WARPS; ++k) {
@@ -339,18 +377,18 @@ __global__ void __launch_bounds__(RS_THREADS) sort_small_kernel(const SortArgs a
     for (int shift = 0; shift < a.key_bits; shift += RS_SMALL_BITS) {
         for (unsigned b = threadIdx.x; b < BINS * RS_WARPS / 2; b += RS_THREADS) reinterpret_cast<unsigned *>(cnt)[b] = 0;
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < RS_ROUNDS; ++r)
-            rank[r] = (unsigned short)warp_rank(cnt + w * BINS, (e[r].x >> shift) & (BINS - 1), RS_SMALL_BITS, base + r * 32 < a.n);
+        warp_ranks(cnt + w * BINS, e, shift, RS_SMALL_BITS, base, a.n, rank);
         __syncthreads();
         unsigned all = 0, before = 0;
+        if (threadIdx.x < BINS)
 #pragma unroll
-        for (int k = 0; k < RS_WARPS; ++k) {
-            const unsigned c = cnt[k * BINS + threadIdx.x];
-            cnt[k * BINS + threadIdx.x] = (unsigned short)before;
-            before += c;
-        }
-        at[threadIdx.x] = block_exclusive(before, sums, &all);
+            for (int k = 0; k < RS_WARPS; ++k) {
+                const unsigned c = cnt[k * BINS + threadIdx.x];
+                cnt[k * BINS + threadIdx.x] = (unsigned short)before;
+                before += c;
+            }
+        const unsigned digit = block_exclusive(before, sums, &all);
+        if (threadIdx.x < BINS) at[threadIdx.x] = digit;
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < RS_ROUNDS; ++r) {
@@ -371,21 +409,26 @@ __global__ void __launch_bounds__(RS_THREADS) sort_small_kernel(const SortArgs a
 }
 
 // ------------------------------------------------------------------------------------------------
-// Sums per row.  A row whose entries fill a whole aligned chunk of LG_CHUNK sorted entries is "long": its chunks are
-// summed by blocks of their own into partial rows, and the partial rows are added in order; all others are added
-// by a group of lanes.  Where a lane's one vector covers its share of the columns (DOT), the same pass forms dweight:
-// the entry's dout row is in registers, and the table's row is read once for all its entries.
+// Sums per row.  The sorted entries are cut into ranges of equal length, one per warp (or group of lanes) and column
+// tile, whatever rows they belong to, so a row that many entries name is no special case.  A row inside one range is
+// written at once; the parts of rows that cross a range's border go to partial rows, which are then added in order.
+// Rows that no entry names get zeros from other blocks of the same launch.
+// dout's rows are fetched at random, so what counts is how many are under way: a group of lanes keeps a ring of RING_STAGES x
+// RING_ENTRIES entries in shared memory, filled by asynchronous copies (96 f16 columns: 150 KB under way per multiprocessor).  Where a
+// row is one column tile (DOT), the same pass forms dweight: the table's rows take part in the ring.  Rows that
+// 16-byte copies do not fit, or that are shorter than 64 bytes, go through registers, 4 entries at a time.
 // ------------------------------------------------------------------------------------------------
-constexpr int LG_THREADS = 256, LG_WARPS = LG_THREADS / 32, LG_CHUNK = 256;
+constexpr int LG_THREADS = 256, LG_WARPS = LG_THREADS / 32;
+constexpr int RING_WARPS = 2, RING_ENTRIES = 8, RING_STAGES = 2;  // 3 stages (fewer warps): 317 us where 2 take 244
 
 struct GradArgs {
     const void *dout, *table, *index;
     const float *weight;
-    float *dtable, *dweight, *partial;  // partial: (2 * chunks, width)
+    float *dtable, *dweight, *partial;  // partial: (2 * ranges, width), the rows that a range begins (0) and ends (1) with
     const unsigned *key, *order;
     long long rows, dout_stride, table_stride;
-    unsigned n, chunks, chunk_blocks, col_tiles;  // chunk_blocks * col_tiles blocks work on chunks, those behind them on rows
-    int width, index_type, rows_per_warp;
+    unsigned n, range, ranges, work_blocks;  // entries per range; blocks on entries, before those on rows without any
+    int width, tiles, pieces, index_type;  // column tiles, 16-byte pieces of dout's row in one
     float scale;
 };
 
@@ -403,55 +446,6 @@ __device__ __forceinline__ unsigned lower_bound(const unsigned *key, unsigned n,
     return lo;
 }
 
-__device__ __forceinline__ bool is_long(unsigned s, unsigned e) {
-    const unsigned full = (s + LG_CHUNK - 1) / LG_CHUNK * LG_CHUNK;
-    return full + LG_CHUNK <= e;
-}
-
-// acc += sum over sorted entries s, s + step, ... below e of scale * weight * dout, columns col, col + col_step, ...
-// DOT: also dweight of those entries, e the table row's columns, summed over the G lanes of `lanes`
-template <class D, int VE, int NV, int G, bool DOT>
-__device__ __forceinline__ void add_entries(const GradArgs &a, unsigned s, unsigned e, unsigned step, int col, int col_step,
-                                            float (&acc)[NV][VE], const float (&row)[VE], unsigned lanes) {
-    constexpr int U = NV == 1 ? 4 : 2;  // entries in flight
-    for (unsigned j = s; j < e; j += step * U) {
-        unsigned i[U];
-        float f[U];
-        Vec<D, VE> d[U][NV];
-#pragma unroll
-        for (int u = 0; u < U; ++u) i[u] = j + u * step < e ? __ldg(a.order + j + u * step) : 0xffffffffu;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            f[u] = i[u] == 0xffffffffu ? 0.0f : a.weight ? a.scale * __ldg(a.weight + i[u]) : a.scale;
-#pragma unroll
-            for (int q = 0; q < NV; ++q) {
-                const int c = col + q * col_step;
-                if (i[u] != 0xffffffffu && c < a.width)
-                    d[u][q].load_stream(static_cast<const D *>(a.dout) + (long long)i[u] * a.dout_stride + c);
-                else d[u][q].zero();
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i[u] == 0xffffffffu) break;
-            float dot = 0.0f;
-#pragma unroll
-            for (int q = 0; q < NV; ++q)
-#pragma unroll
-                for (int v = 0; v < VE; ++v) {
-                    const float x = d[u][q].get(v);
-                    acc[q][v] = fmaf(f[u], x, acc[q][v]);
-                    if (DOT) dot = fmaf(x, row[v], dot);
-                }
-            if (DOT) {
-#pragma unroll
-                for (int o = G / 2; o; o >>= 1) dot += __shfl_xor_sync(lanes, dot, o);
-                if (col == 0) a.dweight[i[u]] = a.scale * dot;
-            }
-        }
-    }
-}
-
 template <int VE>
 __device__ __forceinline__ void store_row(float *p, const float (&acc)[VE]) {
     Vec<float, VE> o;
@@ -460,104 +454,365 @@ __device__ __forceinline__ void store_row(float *p, const float (&acc)[VE]) {
     o.store_stream(p);
 }
 
-template <class T, int VE>
-__device__ __forceinline__ void load_row(const GradArgs &a, long long p, int col, bool some, float (&row)[VE]) {
-    Vec<T, VE> t;
-    if (some && col < a.width) t.load_stream(static_cast<const T *>(a.table) + p * a.table_stride + col);
-    else t.zero();
+// The row that a range's stream of entries is in, and its sum so far: NQ vectors of VE columns per lane of G.
+template <int VE, int NQ, int G>
+struct RowSum {
+    float acc[NQ][VE];
+    unsigned row, before;  // before: the row of the entry before the range
+    bool started;
+    __device__ __forceinline__ RowSum(unsigned before_) : row(0xffffffffu), before(before_), started(false) { clear(); }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int v = 0; v < VE; ++v) row[v] = t.get(v);
-}
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int v = 0; v < VE; ++v) acc[q][v] = 0.0f;
+    }
+    // the stream leaves its row; `more`: the row has entries behind the range
+    __device__ __forceinline__ void leave(const GradArgs &a, unsigned range, int col, bool more) {
+        if (!started) return;
+        float *to = row == before ? a.partial + (size_t)2 * range * a.width
+                    : more        ? a.partial + ((size_t)2 * range + 1) * a.width
+                                  : a.dtable + (size_t)row * a.width;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const int c = col + q * G * VE;
+            if (c < a.width) store_row<VE>(to + c, acc[q]);
+        }
+        clear();
+    }
+    __device__ __forceinline__ void enter(const GradArgs &a, unsigned range, int col, unsigned r) {
+        if (r == row) return;
+        leave(a, range, col, false);
+        row = r;
+        started = true;
+    }
+};
 
-// whether the row that chunk c begins with (side 0) or the one that it ends with (1) is long.  The keys are sorted, so
-// equal keys at both ends of a chunk mean that all of it is one row.
-__device__ __forceinline__ bool chunk_long(const GradArgs &a, unsigned c, int side) {
-    const unsigned c0 = c * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n);
-    const unsigned first = __ldg(a.key + c0), last = __ldg(a.key + c1 - 1);
-    if ((side ? last : first) >= (unsigned)a.rows) return false;  // entries without a row
-    if (side == 0) return (c0 + LG_CHUNK <= a.n && last == first) || (c0 >= LG_CHUNK && __ldg(a.key + c0 - LG_CHUNK) == first);
-    return last != first && c1 + LG_CHUNK <= a.n && __ldg(a.key + c1 + LG_CHUNK - 1) == last;
-}
-
-// Eight chunks per block: the part of the rows at a chunk's ends that are long -> partial rows 2c (the row that the
-// chunk begins with) and 2c + 1 (the row that begins inside it).  Column tiles of 32 VE.
-template <class D, class T, int VE, bool DOT>
-__device__ __forceinline__ void grad_chunks(const GradArgs &a, unsigned block, unsigned col_tile) {
-    __shared__ float part[LG_WARPS][32 * VE];
-    __shared__ unsigned todo;
+// 128 rows a warp: zeros in those that no entry names
+__device__ __forceinline__ void grad_empty(const GradArgs &a, unsigned block, unsigned *words) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    if (w == 0) {
-        const unsigned c = block * LG_WARPS + (lane >> 1);
-        const unsigned mask = __ballot_sync(0xffffffffu, lane < 2 * LG_WARPS && c < a.chunks && chunk_long(a, c, lane & 1));
-        if (lane == 0) todo = mask;
-    }
-    __syncthreads();
-    const int col = (col_tile * 32 + lane) * VE;
-    for (unsigned left = todo; left; left &= left - 1) {
-        const int bit = __ffs(left) - 1, side = bit & 1;
-        const unsigned c = block * LG_WARPS + (bit >> 1), c0 = c * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n);
-        const unsigned first = __ldg(a.key + c0), last = __ldg(a.key + c1 - 1);
-        unsigned s = c0, e = c1;
-        if (first != last) {
-            const unsigned cut = c0 + lower_bound(a.key + c0, c1 - c0, side ? last : first + 1);
-            if (side) s = cut;
-            else e = cut;
-        }
-        float acc[1][VE] = {}, row[VE];
-        if (DOT) load_row<T, VE>(a, side ? last : first, col, true, row);
-        add_entries<D, VE, 1, 32, DOT>(a, s + w, e, LG_WARPS, col, 0, acc, row, 0xffffffffu);
-#pragma unroll
-        for (int v = 0; v < VE; ++v) part[w][lane * VE + v] = acc[0][v];
-        __syncthreads();
-        if (w == 0 && col < a.width) {
-#pragma unroll
-            for (int v = 0; v < VE; ++v) {
-                float t = 0.0f;
-                for (int k = 0; k < LG_WARPS; ++k) t += part[k][lane * VE + v];
-                acc[0][v] = t;
+    const long long row0 = ((long long)block * (blockDim.x >> 5) + w) * 128;
+    if (row0 >= a.rows) return;
+    // the entries of the warp's rows: both borders at once, 16 probes a step for each
+    unsigned lo = 0, len = a.n;
+    {
+        const unsigned v = (unsigned)min(row0 + (lane < 16 ? 0 : 128), a.rows);
+        const int p = lane & 15;
+        while (__any_sync(0xffffffffu, len != 0)) {
+            const unsigned at = lo + (unsigned)((unsigned long long)len * (p + 1) / 17);
+            const bool less = len != 0 && __ldg(a.key + at) < v;
+            const unsigned below = __popc((__ballot_sync(0xffffffffu, less) >> (lane & 16)) & 0xffffu);
+            if (len != 0) {
+                const unsigned from = below ? lo + (unsigned)((unsigned long long)len * below / 17) + 1 : lo;
+                const unsigned to = below < 16 ? lo + (unsigned)((unsigned long long)len * (below + 1) / 17) : lo + len;
+                lo = from;
+                len = to - from;
             }
-            store_row<VE>(a.partial + ((size_t)2 * c + side) * a.width + col, acc[0]);
         }
-        __syncthreads();
+    }
+    const unsigned s = __shfl_sync(0xffffffffu, lo, 0), e = __shfl_sync(0xffffffffu, lo, 16);
+    unsigned *named = words + 4 * w;
+    if (lane < 4) named[lane] = 0;
+    __syncwarp();
+    if (e - s < 1024) {
+        for (unsigned j = s + lane; j < e; j += 32) {
+            const unsigned r = __ldg(a.key + j) - (unsigned)row0;
+            atomicOr(&named[r >> 5], 1u << (r & 31));
+        }
+    } else {  // few rows, many entries: look each row up
+        for (int k = 0; k < 4; ++k) {
+            const unsigned r = (unsigned)min(row0 + 32 * k + lane, a.rows);
+            const unsigned at = s + lower_bound(a.key + s, e - s, r);
+            const unsigned m = __ballot_sync(0xffffffffu, at < e && __ldg(a.key + at) == r);
+            if (lane == 0) named[k] = m;
+        }
+    }
+    __syncwarp();
+    const bool four = a.width % 4 == 0 && (reinterpret_cast<uintptr_t>(a.dtable) & 15) == 0;
+    for (int k = 0; k < 4; ++k) {
+        const long long left = a.rows - row0 - 32 * k;
+        unsigned empty = left <= 0 ? 0u : ~named[k] & (left >= 32 ? 0xffffffffu : (1u << left) - 1u);
+        for (; empty; empty &= empty - 1) {
+            float *p = a.dtable + (row0 + 32 * k + __ffs(empty) - 1) * a.width;
+            if (four)
+                for (int c = lane * 4; c < a.width; c += 128) __stcs(reinterpret_cast<float4 *>(p + c), make_float4(0, 0, 0, 0));
+            else
+                for (int c = lane; c < a.width; c += 32) __stcs(p + c, 0.0f);
+        }
     }
 }
 
-// Eight chunks per block: for a long row that begins in one of them, adds its partial rows in order and writes the row.
+__device__ __forceinline__ unsigned shared_addr(const void *p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy8(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(shared_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A lane's 16 bytes of a row of dout and its share of the table's row, per entry; with the stage's keys, entry numbers and
+// weights a group of G lanes has RING_ENTRIES of them in a stage
+template <class D, class T, bool DOT>
+struct RingPiece {
+    static constexpr int VE = 16 / (int)sizeof(D), TB = DOT ? VE * (int)sizeof(T) : 0;
+    // bytes of a stage whose rows have `pieces` of them
+    __host__ __device__ static constexpr int bytes(int pieces) { return RING_ENTRIES * (pieces * (16 + TB) + 3 * 4); }
+};
+
+// A group of G lanes per range and column tile, a lane for every 16 bytes of dout's row.  A lane copies what it will read
+// itself; the lane's piece of entry e is at e * pieces + its number, dout's first, then the table's, then the numbers.
+template <class D, class T, int G, bool DOT>
+__global__ void __launch_bounds__(32 * RING_WARPS) grad_ring_kernel(const GradArgs a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ unsigned words[4 * RING_WARPS];
+    if (blockIdx.x >= a.work_blocks) {
+        grad_empty(a, blockIdx.x - a.work_blocks, words);
+        return;
+    }
+    using Piece = RingPiece<D, T, DOT>;
+    constexpr int VE = Piece::VE, TB = Piece::TB, E = RING_ENTRIES;
+    const int P = a.pieces, stage_bytes = Piece::bytes(P);
+    const int sub = threadIdx.x % G;
+    const unsigned lanes = G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << (threadIdx.x % 32 / G * G);
+    const unsigned item = blockIdx.x * (32 * RING_WARPS / G) + threadIdx.x / G, range = item / a.tiles;
+    if (range >= a.ranges) return;
+    const int col = (int)(item % a.tiles) * (G * VE) + sub * VE;
+    const bool mine = col < a.width;
+    const unsigned j0 = range * a.range, end = min(j0 + a.range, a.n);
+    // entries without a row are the last ones
+    unsigned j1 = end;
+    if (__ldg(a.key + end - 1) >= (unsigned)a.rows) j1 = j0 + lower_bound(a.key + j0, end - j0, (unsigned)a.rows);
+    if (j1 == j0) return;
+    const int count = (int)(j1 - j0), stages = (count + E - 1) / E;
+    unsigned char *ring = raw + (threadIdx.x / G) * (RING_STAGES * stage_bytes);
+    const D *dout = static_cast<const D *>(a.dout) + col;
+    const T *table = static_cast<const T *>(a.table) + col;
+    // lane l < E: entry number and row of entry l of a stage
+    unsigned num = 0, key = 0;
+    auto numbers = [&](int st) {
+        const unsigned j = j0 + st * E + sub;
+        if (sub < E && j < j1) {
+            num = __ldg(a.order + j);
+            key = __ldg(a.key + j);
+        }
+    };
+    auto issue = [&](int st, int slot) {
+        unsigned char *to = ring + slot * stage_bytes;
+        unsigned *meta = reinterpret_cast<unsigned *>(to + E * P * (16 + TB));
+        const int left = count - st * E;
+        if (sub < E && sub < left) {
+            meta[sub] = key;
+            meta[E + sub] = num;
+            if (a.weight) copy4(meta + 2 * E + sub, a.weight + num);
+            else meta[2 * E + sub] = __float_as_uint(1.0f);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const unsigned i = __shfl_sync(lanes, num, e, G), k = __shfl_sync(lanes, key, e, G);
+            if (mine && e < left) {
+                copy16(to + (e * P + sub) * 16, dout + (long long)i * a.dout_stride);
+                if (DOT) {
+                    const char *from = reinterpret_cast<const char *>(table + (long long)k * a.table_stride);
+                    unsigned char *at = to + E * P * 16 + (e * P + sub) * TB;
+                    if (TB == 8) copy8(at, from);
+#pragma unroll
+                    for (int b = 0; b + 16 <= TB; b += 16) copy16(at + b, from + b);
+                }
+            }
+        }
+    };
+    RowSum<VE, 1, G> sum(j0 ? __ldg(a.key + j0 - 1) : 0xffffffffu);
+    numbers(0);
+#pragma unroll
+    for (int st = 0; st < RING_STAGES - 1; ++st) {
+        if (st < stages) issue(st, st);
+        copies_commit();
+        numbers(st + 1);
+    }
+    int slot = 0, fill = RING_STAGES - 1;
+    for (int st = 0; st < stages; ++st) {
+        if (st + RING_STAGES - 1 < stages) issue(st + RING_STAGES - 1, fill);
+        copies_commit();
+        numbers(st + RING_STAGES);
+        copies_wait<RING_STAGES - 1>();
+        __syncwarp(lanes);
+        const unsigned char *from = ring + slot * stage_bytes;
+        const unsigned *meta = reinterpret_cast<const unsigned *>(from + E * P * (16 + TB));
+        // lanes without a piece read the last one's
+        const unsigned char *mine_d = from + min(sub, P - 1) * 16, *mine_t = from + E * P * 16 + min(sub, P - 1) * TB;
+        const int left = count - st * E;
+        auto entries = [&](int e0, int m) {  // m <= 4 entries
+            const uint4 keys = *reinterpret_cast<const uint4 *>(meta + e0);
+            const float4 ws = *reinterpret_cast<const float4 *>(meta + 2 * E + e0);
+            const unsigned k[4] = {keys.x, keys.y, keys.z, keys.w};
+            const float f[4] = {ws.x, ws.y, ws.z, ws.w};
+            float dot[4] = {};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (u >= m) break;
+                sum.enter(a, range, col, k[u]);
+                const float s = a.scale * f[u];
+                Vec<D, VE> d;
+                d.raw[0] = *reinterpret_cast<const uint4 *>(mine_d + (e0 + u) * P * 16);
+                Vec<T, VE> t;
+                if (DOT)
+#pragma unroll
+                    for (int b = 0; b < Vec<T, VE>::R::N; ++b)
+                        t.raw[b] = reinterpret_cast<const typename Vec<T, VE>::R::type *>(mine_t + (e0 + u) * P * TB)[b];
+#pragma unroll
+                for (int v = 0; v < VE; ++v) {
+                    const float x = d.get(v);
+                    sum.acc[0][v] = fmaf(s, x, sum.acc[0][v]);
+                    if (DOT) dot[u] = fmaf(x, t.get(v), dot[u]);
+                }
+                if (DOT && !mine) dot[u] = 0.0f;
+            }
+            if (DOT) {
+                // four sums over the group: two exchanges leave each lane one of them, by two bits of its number
+                const bool hi = sub & (G / 2), mid = sub & (G / 4);
+                const float x = (hi ? dot[2] : dot[0]) + __shfl_xor_sync(lanes, hi ? dot[0] : dot[2], G / 2);
+                const float y = (hi ? dot[3] : dot[1]) + __shfl_xor_sync(lanes, hi ? dot[1] : dot[3], G / 2);
+                float z = (mid ? y : x) + __shfl_xor_sync(lanes, mid ? x : y, G / 4);
+#pragma unroll
+                for (int o = G / 8; o; o >>= 1) z += __shfl_xor_sync(lanes, z, o);
+                const int u = (hi ? 2 : 0) + (mid ? 1 : 0);
+                if (sub % (G / 4) == 0 && u < m) a.dweight[meta[E + e0 + u]] = a.scale * z;
+            }
+        };
+        if (left >= E) {
+#pragma unroll
+            for (int e0 = 0; e0 < E; e0 += 4) entries(e0, 4);
+        } else {
+            for (int e0 = 0; e0 < left; e0 += 4) entries(e0, min(4, left - e0));
+        }
+        __syncwarp(lanes);  // the stage is filled again
+        slot = slot + 1 == RING_STAGES ? 0 : slot + 1;
+        fill = fill + 1 == RING_STAGES ? 0 : fill + 1;
+    }
+    copies_wait<0>();
+    sum.leave(a, range, col, j1 == end && end < a.n && __ldg(a.key + end) == sum.row);
+}
+
+// A group of G lanes per range and column tile, entries through registers.  NQ vectors of VE columns per lane
+template <class D, int VE, int NQ, int G>
+__global__ void __launch_bounds__(LG_THREADS) grad_plain_kernel(const GradArgs a) {
+    __shared__ unsigned words[4 * LG_WARPS];
+    if (blockIdx.x >= a.work_blocks) {
+        grad_empty(a, blockIdx.x - a.work_blocks, words);
+        return;
+    }
+    constexpr int U = 4;
+    const unsigned item = blockIdx.x * (LG_THREADS / G) + threadIdx.x / G, range = item / a.tiles;
+    if (range >= a.ranges) return;
+    const int col = (int)(item % a.tiles) * (G * VE * NQ) + threadIdx.x % G * VE;
+    const unsigned j0 = range * a.range, j1 = min(j0 + a.range, a.n);
+    RowSum<VE, NQ, G> sum(j0 ? __ldg(a.key + j0 - 1) : 0xffffffffu);
+    unsigned i[U], k[U];
+    auto fetch = [&](unsigned j) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            i[u] = j + u < j1 ? __ldg(a.order + j + u) : 0u;
+            k[u] = j + u < j1 ? __ldg(a.key + j + u) : 0xffffffffu;
+        }
+    };
+    fetch(j0);
+    bool over = false;
+    for (unsigned j = j0; j < j1 && !over; j += U) {
+        unsigned ck[U];
+        float f[U];
+        Vec<D, VE> d[U][NQ];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            ck[u] = k[u];
+            const bool in = ck[u] < (unsigned)a.rows;
+            f[u] = in && a.weight ? a.scale * __ldg(a.weight + i[u]) : a.scale;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                const int c = col + q * G * VE;
+                if (in && c < a.width) d[u][q].load_stream(static_cast<const D *>(a.dout) + (long long)i[u] * a.dout_stride + c);
+                else d[u][q].zero();
+            }
+        }
+        fetch(j + U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (ck[u] >= (unsigned)a.rows) {
+                over = true;
+                break;
+            }
+            sum.enter(a, range, col, ck[u]);
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int v = 0; v < VE; ++v) sum.acc[q][v] = fmaf(f[u], d[u][q].get(v), sum.acc[q][v]);
+        }
+    }
+    sum.leave(a, range, col, j1 < a.n && __ldg(a.key + j1) == sum.row);
+}
+
+// A warp per range: if a row begins in it and goes on behind it, adds the row's partial rows in order and writes it.  Rows of
+// more than JOIN_WARP ranges are added by the whole block.  grid.y: tiles of 32 VE columns
+constexpr int JOIN_WARP = 32;
 template <int VE>
 __global__ void __launch_bounds__(LG_THREADS) grad_join_kernel(const GradArgs a) {
     __shared__ float part[LG_WARPS][32 * VE];
-    __shared__ unsigned todo;
+    __shared__ unsigned first_of[LG_WARPS], last_of[LG_WARPS];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    if (w == 0) {
-        // a long row begins in c if it is what c ends with and c is where it starts: inside c (side 1), or at its first entry
-        const unsigned c = blockIdx.x * LG_WARPS + lane;
-        bool begins = false;
-        if (lane < LG_WARPS && c < a.chunks) {
-            const unsigned c0 = c * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n), first = __ldg(a.key + c0);
-            begins = chunk_long(a, c, 1) || (__ldg(a.key + c1 - 1) == first && chunk_long(a, c, 0) &&
-                                             (c0 == 0 || __ldg(a.key + c0 - 1) != first));
-        }
-        const unsigned mask = __ballot_sync(0xffffffffu, begins);
-        if (lane == 0) todo = mask;
-    }
-    __syncthreads();
     const int col = (blockIdx.y * 32 + lane) * VE;
-    for (unsigned left = todo; left; left &= left - 1) {
-        const unsigned b = blockIdx.x * LG_WARPS + __ffs(left) - 1, c0 = b * LG_CHUNK, c1 = min(c0 + LG_CHUNK, a.n);
-        const unsigned row = __ldg(a.key + c1 - 1);
-        const bool inside = __ldg(a.key + c0) != row;
-        const unsigned e = c0 + lower_bound(a.key + c0, a.n - c0, row + 1), last = (e - 1) / LG_CHUNK;
-        float acc[VE] = {};
-        if (col < a.width) {
-#pragma unroll 4
-            for (unsigned c = b + w; c <= last; c += LG_WARPS) {
-                const unsigned slot = 2 * c + (c == b && inside ? 1 : 0);
-                Vec<float, VE> d;
-                d.load(a.partial + (size_t)slot * a.width + col);
+    const unsigned c = blockIdx.x * LG_WARPS + w;
+    auto add = [&](unsigned slot, float (&acc)[VE]) {
+        Vec<float, VE> d;
+        if (col < a.width) d.load(a.partial + (size_t)slot * a.width + col);
+        else d.zero();
 #pragma unroll
-                for (int v = 0; v < VE; ++v) acc[v] += d.el[v];
+        for (int v = 0; v < VE; ++v) acc[v] += d.el[v];
+    };
+    unsigned row = 0, last = 0, slot = 0;
+    bool many = false;
+    if (c + 1 < a.ranges) {  // the last range's row ends there
+        const unsigned c0 = c * a.range, c1 = c0 + a.range;
+        row = __ldg(a.key + c1 - 1);
+        const bool before = c0 && __ldg(a.key + c0 - 1) == row;
+        if (row < (unsigned)a.rows && !before && __ldg(a.key + c1) == row) {
+            slot = 2 * c + 1;  // the row begins in this range
+            // its last range, by growing strides of ranges and then a search
+            unsigned lo = c + 1, step = 1;  // range lo has an entry of the row
+            while (lo + step < a.ranges && __ldg(a.key + (lo + step) * a.range) == row) {
+                lo += step;
+                step *= 2;
+            }
+            for (; step; step >>= 1)
+                if (lo + step < a.ranges && __ldg(a.key + (lo + step) * a.range) == row) lo += step;
+            last = lo;
+            many = last - c > JOIN_WARP;
+            if (!many) {
+                float acc[VE] = {};
+                add(slot, acc);
+#pragma unroll 4
+                for (unsigned r = c + 1; r <= last; ++r) add(2 * r, acc);
+                if (col < a.width) store_row<VE>(a.dtable + (size_t)row * a.width + col, acc);
             }
         }
+    }
+    if (!__syncthreads_or(many)) return;
+    if (lane == 0) {
+        first_of[w] = many ? c : 0xffffffffu;
+        last_of[w] = last;
+    }
+    __syncthreads();
+    for (int k = 0; k < LG_WARPS; ++k) {
+        const unsigned first = first_of[k], end = last_of[k];
+        if (first == 0xffffffffu) continue;
+        float acc[VE] = {};
+        if (w == 0) add(2 * first + 1, acc);
+#pragma unroll 8
+        for (unsigned r = first + 1 + w; r <= end; r += LG_WARPS) add(2 * r, acc);
 #pragma unroll
         for (int v = 0; v < VE; ++v) part[w][lane * VE + v] = acc[v];
         __syncthreads();
@@ -565,50 +820,14 @@ __global__ void __launch_bounds__(LG_THREADS) grad_join_kernel(const GradArgs a)
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
                 float t = 0.0f;
-                for (int k = 0; k < LG_WARPS; ++k) t += part[k][lane * VE + v];
+                for (int o = 0; o < LG_WARPS; ++o) t += part[o][lane * VE + v];
                 acc[v] = t;
             }
-            store_row<VE>(a.dtable + (size_t)row * a.width + col, acc);
+            const unsigned at = __ldg(a.key + (first + 1) * a.range);
+            store_row<VE>(a.dtable + (size_t)at * a.width + col, acc);
         }
         __syncthreads();
     }
-}
-
-// A group of G lanes per row (32 / G rows at a time per warp), each lane NV vectors of VE columns per column tile.
-template <class D, class T, int VE, int NV, int G, bool DOT>
-__device__ __forceinline__ void grad_rows(const GradArgs &a, unsigned block) {
-    constexpr int RPW = 32 / G;
-    const int lane = threadIdx.x & 31, sub = lane % G;
-    const unsigned lanes = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (lane / G * G);
-    const long long warp = (long long)block * LG_WARPS + (threadIdx.x >> 5), row0 = warp * a.rows_per_warp;
-    if (row0 >= a.rows) return;
-    // lane k finds where row row0 + k begins; the last lane's row ends where the next one begins
-    const unsigned begin = lower_bound(a.key, a.n, (unsigned)min(row0 + lane, a.rows));
-    const unsigned after = lower_bound(a.key, a.n, (unsigned)min(row0 + 32, a.rows));
-    for (int r = 0; r < a.rows_per_warp; r += RPW) {
-        const int k = r + lane / G;
-        const unsigned s = __shfl_sync(0xffffffffu, begin, k & 31), next = __shfl_sync(0xffffffffu, begin, (k + 1) & 31);
-        const unsigned e = k == 31 ? after : next;
-        const long long row = row0 + k;
-        if (row >= a.rows || k >= a.rows_per_warp || is_long(s, e)) continue;
-        for (int c0 = 0; c0 < a.width; c0 += G * NV * VE) {
-            float acc[NV][VE] = {}, held[VE];
-            if (DOT) load_row<T, VE>(a, row, c0 + sub * VE, s < e, held);
-            add_entries<D, VE, NV, G, DOT>(a, s, e, 1, c0 + sub * VE, G * VE, acc, held, lanes);
-#pragma unroll
-            for (int q = 0; q < NV; ++q) {
-                const int c = c0 + sub * VE + q * G * VE;
-                if (c < a.width) store_row<VE>(a.dtable + row * a.width + c, acc[q]);
-            }
-        }
-    }
-}
-
-template <class D, class T, int VE, int NV, int G, bool DOT>
-__global__ void __launch_bounds__(LG_THREADS) grad_sum_kernel(const GradArgs a) {
-    const unsigned chunk_part = a.chunk_blocks * a.col_tiles;
-    if (blockIdx.x < chunk_part) grad_chunks<D, T, VE, DOT>(a, blockIdx.x % a.chunk_blocks, blockIdx.x / a.chunk_blocks);
-    else grad_rows<D, T, VE, NV, G, DOT>(a, blockIdx.x - chunk_part);
 }
 
 // dweight: a warp per entry.
@@ -640,14 +859,18 @@ __global__ void zero_kernel(float *p, long long n) {
 
 struct GradPlan {
     long long entries[2], key, val, hist, total, partial, bytes;
-    unsigned tiles, chunks;
+    unsigned tiles, range, ranges;
     int bits, passes;
 };
 
 GradPlan grad_plan(long long rows, long long n, int width) {
     GradPlan g{};
     g.tiles = (unsigned)((n + RS_TILE - 1) / RS_TILE);
-    g.chunks = (unsigned)((n + LG_CHUNK - 1) / LG_CHUNK);
+    // ranges of 256 entries, shorter where that leaves multiprocessors without a warp
+    g.range = 256;
+    const long long col_tiles = (width + 255) / 256;
+    while (g.range > 32 && (n + g.range - 1) / g.range * col_tiles < 16ll * SMS) g.range /= 2;
+    g.ranges = (unsigned)((n + g.range - 1) / g.range);
     g.bits = 1;
     while ((rows >> g.bits) != 0) ++g.bits;  // keys are 0 .. rows
     g.passes = (g.bits + RS_MAX_BITS - 1) / RS_MAX_BITS;
@@ -664,8 +887,7 @@ GradPlan grad_plan(long long rows, long long n, int width) {
         g.hist = take((4ll << (g.bits + g.passes - 1) / g.passes) * g.tiles);
         g.total = take(4ll * RS_BINS);
     }
-    // only rows that fill a chunk have partial rows
-    g.partial = take(n >= LG_CHUNK ? 8ll * g.chunks * width : 0);
+    g.partial = take(g.ranges > 1 ? 8ll * g.ranges * width : 0);
     g.bytes = at;
     return g;
 }
@@ -710,38 +932,66 @@ using Width = std::integral_constant<int, VE>;
 template <class F>
 void with_width(int ve, F f) {
     switch (ve) {
-        case 8: f(Width<8>{}); break;
         case 4: f(Width<4>{}); break;
         case 2: f(Width<2>{}); break;
         default: f(Width<1>{}); break;
     }
 }
 
-template <class D, class T, int VE, bool DOT>
-void launch_sums(GradArgs a, cudaStream_t st) {
-    const int vectors = a.width / VE;
-    a.col_tiles = (vectors + 31) / 32;
-    a.chunk_blocks = a.n >= LG_CHUNK ? (a.chunks + LG_WARPS - 1) / LG_WARPS : 0;
-    // 32 rows a warp share a search; fewer where that leaves the machine without warps
-    a.rows_per_warp = 32;
-    while (a.rows_per_warp > 8 && a.rows / a.rows_per_warp < 64 * SMS) a.rows_per_warp /= 2;
-    const long long per_block = (long long)a.rows_per_warp * LG_WARPS;
-    const unsigned grid = a.chunk_blocks * a.col_tiles + (unsigned)((a.rows + per_block - 1) / per_block);
-    if (vectors <= 8) grad_sum_kernel<D, T, VE, 1, 8, DOT><<<grid, LG_THREADS, 0, st>>>(a);
-    else if (vectors <= 16) grad_sum_kernel<D, T, VE, 1, 16, DOT><<<grid, LG_THREADS, 0, st>>>(a);
-    else if (vectors <= 32) grad_sum_kernel<D, T, VE, 1, 32, DOT><<<grid, LG_THREADS, 0, st>>>(a);
-    else if constexpr (!DOT) grad_sum_kernel<D, T, VE, 4, 32, false><<<grid, LG_THREADS, 0, st>>>(a);
-    if (a.chunk_blocks) grad_join_kernel<VE><<<dim3(a.chunk_blocks, a.col_tiles), LG_THREADS, 0, st>>>(a);
+template <int VE>
+void launch_join(const GradArgs &a, cudaStream_t st) {
+    if (a.ranges > 1)
+        grad_join_kernel<VE><<<dim3((a.ranges + LG_WARPS - 1) / LG_WARPS, (a.width / VE + 31) / 32), LG_THREADS, 0, st>>>(a);
 }
 
-// widest vectors that all the given tensors allow
-int grad_vec(const flare_lookup_grad_args *in, bool dtable, bool table) {
-    int ve = 8;
+template <class D, class T, int G, bool DOT>
+int launch_ring(GradArgs a, cudaStream_t st) {
+    using Piece = RingPiece<D, T, DOT>;
+    constexpr int GROUPS = 32 * RING_WARPS / G;
+    a.pieces = std::min(G, a.width / Piece::VE);
+    a.tiles = (a.width + G * Piece::VE - 1) / (G * Piece::VE);
+    a.work_blocks = (unsigned)(((long long)a.ranges * a.tiles + GROUPS - 1) / GROUPS);
+    const unsigned empty_blocks = (unsigned)((a.rows + 128 * RING_WARPS - 1) / (128 * RING_WARPS));
+    auto fn = grad_ring_kernel<D, T, G, DOT>;
+    const int e = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_lookup_backward");
+    if (e) return e;
+    fn<<<a.work_blocks + empty_blocks, 32 * RING_WARPS, GROUPS * RING_STAGES * Piece::bytes(a.pieces), st>>>(a);
+    launch_join<Piece::VE>(a, st);
+    return FLARE_OK;
+}
+
+template <class D, class T, bool DOT>
+int launch_ring(const GradArgs &a, cudaStream_t st) {
+    const int pieces = a.width * (int)sizeof(D) / 16;
+    if (pieces <= 8) return launch_ring<D, T, 8, DOT>(a, st);
+    if (pieces <= 16) return launch_ring<D, T, 16, DOT>(a, st);
+    return launch_ring<D, T, 32, DOT>(a, st);
+}
+
+template <class D, int VE, int NQ, int G>
+void launch_plain(GradArgs a, cudaStream_t st) {
+    a.tiles = (a.width + G * VE * NQ - 1) / (G * VE * NQ);
+    const unsigned per_block = LG_THREADS / G;
+    a.work_blocks = (unsigned)(((long long)a.ranges * a.tiles + per_block - 1) / per_block);
+    const unsigned empty_blocks = (unsigned)((a.rows + 128 * LG_WARPS - 1) / (128 * LG_WARPS));
+    grad_plain_kernel<D, VE, NQ, G><<<a.work_blocks + empty_blocks, LG_THREADS, 0, st>>>(a);
+    launch_join<VE>(a, st);
+}
+
+// widest vectors, up to 4 elements, that dout and dtable allow (or, without dtable, dout and table)
+int grad_vec(const flare_lookup_grad_args *in, bool dtable) {
+    int ve = 4;
     while (ve > 1 && !(in->width % ve == 0 && fits_vec(in->dout, in->dout_stride, type_size(in->dout_type), ve) &&
-                       (!dtable || fits_vec(in->dtable, in->width, 4, ve)) &&
-                       (!table || fits_vec(in->table, in->table_stride, type_size(in->table_type), ve))))
+                       (dtable ? fits_vec(in->dtable, in->width, 4, ve)
+                               : fits_vec(in->table, in->table_stride, type_size(in->table_type), ve))))
         ve >>= 1;
     return ve;
+}
+
+// whether 16-byte copies fit a matrix's rows
+bool fits_copies(const void *p, long long stride, int width, int type) {
+    const int per = 16 / type_size(type);
+    return width % per == 0 && stride % per == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
 }
 
 int run_lookup_backward(const flare_lookup_grad_args *in, cudaStream_t st) {
@@ -768,35 +1018,47 @@ int run_lookup_backward(const flare_lookup_grad_args *in, cudaStream_t st) {
         return FLARE_OK;
     }
     const bool sums = in->dtable && in->rows;
-    // both gradients in one pass where a row's columns are one vector a lane
-    const int both = sums && in->dweight ? grad_vec(in, true, true) : 0;
-    const bool dot = both && in->width / both <= 32;
+    // rows of at least 64 bytes that 16-byte copies fit pass through the ring, both gradients at once where a row is one tile
+    const bool ring = sums && in->width * type_size(in->dout_type) >= 64 &&
+                      fits_copies(in->dout, in->dout_stride, in->width, in->dout_type) && fits_copies(in->dtable, in->width, in->width, FLARE_F32);
+    const int per_piece = 16 / type_size(in->dout_type);  // columns of a lane
+    const bool dot = ring && in->dweight && in->width <= 32 * per_piece &&
+                     fits_vec(in->table, in->table_stride, type_size(in->table_type), per_piece);
     if (sums) {
         const GradPlan g = grad_plan(in->rows, in->n, in->width);
         char *ws = static_cast<char *>(in->workspace);
-        const int e = sort_entries(in, g, dot, st);
+        int e = sort_entries(in, g, dot, st);
         if (e) return e;
         a.key = reinterpret_cast<unsigned *>(ws + g.key);
         a.order = reinterpret_cast<unsigned *>(ws + g.val);
         a.partial = reinterpret_cast<float *>(ws + g.partial);
-        a.chunks = g.chunks;
-        with_type(in->dout_type, [&](auto d) {
+        a.range = g.range;
+        a.ranges = g.ranges;
+        e = with_type(in->dout_type, [&](auto d) {
             using D = typename decltype(d)::type;
             if (dot)
-                with_type(in->table_type, [&](auto t) {
-                    with_width(both, [&](auto ve) { launch_sums<D, typename decltype(t)::type, decltype(ve)::value, true>(a, st); });
-                    return 0;
+                return with_type(in->table_type, [&](auto t) {
+                    using T = typename decltype(t)::type;
+                    return launch_ring<D, T, true>(a, st);
                 });
-            else with_width(grad_vec(in, true, false), [&](auto ve) { launch_sums<D, float, decltype(ve)::value, false>(a, st); });
-            return 0;
+            if (ring) return launch_ring<D, float, false>(a, st);
+            const int ve = grad_vec(in, true);
+            with_width(ve, [&](auto w) {
+                constexpr int VE = decltype(w)::value;
+                if (in->width / VE <= 8) launch_plain<D, VE, 1, 8>(a, st);
+                else if (in->width / VE <= 32) launch_plain<D, VE, 1, 32>(a, st);
+                else launch_plain<D, VE, 4, 32>(a, st);
+            });
+            return FLARE_OK;
         });
+        if (e) return e;
         OPS_LAUNCHED("flare_lookup_backward");
     }
     if (in->dweight && !dot) {
         const unsigned blocks = (unsigned)std::min<long long>((in->n + 7) / 8, SMS * 64);
         with_type(in->dout_type, [&](auto d) {
             return with_type(in->table_type, [&](auto t) {
-                with_width(grad_vec(in, false, true), [&](auto ve) {
+                with_width(grad_vec(in, false), [&](auto ve) {
                     grad_weight_kernel<typename decltype(d)::type, typename decltype(t)::type, decltype(ve)::value>
                         <<<blocks, LG_THREADS, 0, st>>>(a);
                 });

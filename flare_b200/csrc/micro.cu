@@ -4,10 +4,33 @@
 // 32, 8 elements each, so that a warp's 16-byte loads are contiguous; the block's largest magnitude is exchanged by two
 // shuffles.
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "ops.cuh"
 
 namespace flare {
+
+int allow_shared_memory(const void *kernel, const char *what) {
+    static std::mutex lock;
+    static std::set<std::pair<const void *, int>> allowed;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) {
+        std::lock_guard<std::mutex> hold(lock);
+        if (allowed.count({kernel, device})) return FLARE_OK;
+        cudaFuncAttributes at{};
+        e = cudaFuncGetAttributes(&at, kernel);
+        // 227 KB a block, less what the kernel has already
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)at.sharedSizeBytes);
+        if (e == cudaSuccess) allowed.insert({kernel, device});
+    }
+    if (e == cudaSuccess) return FLARE_OK;
+    set_error("%s: %s", what, cudaGetErrorString(e));
+    return FLARE_E_CUDA;
+}
 
 constexpr int MQ_THREADS = 256;
 

@@ -132,6 +132,9 @@ struct FastDiv {
     __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
 };
 
+// Lets a kernel have all of a multiprocessor's shared memory, once per device.
+int allow_shared_memory(const void *kernel, const char *what);
+
 template <class T>
 struct TypeTag { using type = T; };
 // f(tag) for the C++ type of a FLARE_* float type

@@ -13,7 +13,6 @@
 #include <cuda.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "common.cuh"
 #include "ops.cuh"
@@ -349,28 +348,20 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, ProductArgs a, 
     int smem = a.stages * Tile::STAGE + 1024;
     if (split > 1) smem = std::max(smem, PT * BN * 4 + 1024);
     auto fn = product_kernel<BN, O>;
-    static std::atomic<unsigned long long> set{0};  // devices that this kernel may use all shared memory on
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    const unsigned long long bit = 1ull << (device & 63);
-    if (e == cudaSuccess && !(set.load() & bit)) {
-        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX - SMEM_HEAD);
-        if (e == cudaSuccess) set.fetch_or(bit);
-    }
-    if (e == cudaSuccess) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)((a.p + PT - 1) / PT), (unsigned)((a.q + BN - 1) / BN), (unsigned)split);
-        cfg.blockDim = dim3(PR_THREADS);
-        cfg.dynamicSmemBytes = (size_t)smem;
-        cfg.stream = st;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = attr.val.clusterDim.y = 1;
-        attr.val.clusterDim.z = (unsigned)split;
-        cfg.attrs = &attr;
-        cfg.numAttrs = split > 1 ? 1 : 0;
-        e = cudaLaunchKernelEx(&cfg, fn, pm, qm, a);
-    }
+    const int e0 = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_micro_product");
+    if (e0) return e0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((a.p + PT - 1) / PT), (unsigned)((a.q + BN - 1) / BN), (unsigned)split);
+    cfg.blockDim = dim3(PR_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = (unsigned)split;
+    cfg.attrs = &attr;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, pm, qm, a);
     if (e != cudaSuccess) {
         set_error("flare_micro_product: %s", cudaGetErrorString(e));
         return FLARE_E_CUDA;
