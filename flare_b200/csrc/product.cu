@@ -2,14 +2,17 @@
 //
 // tcgen05.mma kind::mxf4 multiplies 4-bit elements and applies the block scales itself: D (TMEM, f32) += (A * 2^sa)
 // (B * 2^sb)^T for 64 elements of K at a time, two scales per row.  The larger matrix gives the 128 rows of a tile (P), the
-// other its BN columns (Q); where that is B, the tile is stored transposed.  Per 256 elements of K (a stage):
-//   * warp 4 brings the codes, 128 bytes a row, by TMA into 128-byte-swizzled tiles;
-//   * warps 0-3 bring the scales, a word (128 elements of K) per row and half stage, into the order that tcgen05.cp spreads
-//     over TMEM: 32 rows of 16 bytes, row r the words of tile rows r, r + 32, r + 64, r + 96;
-//   * warp 5 copies the scales to TMEM and issues the products; its commit frees the stage.
-// Then warps 0-3 read D from TMEM, a row per thread, and store it rounded once.  Few tiles and a long K: up to 8 blocks of a
-// cluster take a part of K each and add their tiles through distributed shared memory, in order.
-// Every wait is bounded; a block in which one ran out stores NaN and sets a bit of the status word.
+// other its BN columns (Q); where that is B, the tile is stored transposed.  One block per multiprocessor walks over tiles;
+// per 256 elements of K (a stage):
+//   * warp 8 brings the codes, 128 bytes a row, by TMA into 128-byte-swizzled tiles;
+//   * warps 4-7 bring the scales, a word (128 elements of K) per row and half stage, into the order that tcgen05.cp spreads
+//     over TMEM: 32 rows of 16 bytes, row r the words of tile rows r, r + 32, r + 64, r + 96; a thread loads 4 words of a row
+//     at a time and is two such loads ahead (word by word they took 23 of 89 us at 4096 x 4096 x 4096);
+//   * warp 9 copies the scales to TMEM and issues the products; its commit frees the stage.
+// Warps 0-3 read a finished D from TMEM, a row per thread, round it once and store it through shared memory by TMA, while
+// the next tile goes into the other half of TMEM.  Few tiles and a long K: up to 8 blocks of a cluster take a part of K
+// each and add their tiles through distributed shared memory, in order.
+// Every wait is bounded; where one ran out the block's tiles are NaN and a bit of the status word is set.
 #include <cuda.h>
 
 #include <algorithm>
@@ -23,16 +26,21 @@ namespace flare {
 constexpr int PT = 128;          // rows of P per tile
 constexpr int KSTAGE = 256;      // elements of K per stage
 constexpr int KBYTES = KSTAGE / 2;
-constexpr int PR_THREADS = 192;
-constexpr int SMEM_MAX = 227 * 1024, SMEM_HEAD = 1024;
+constexpr int PR_WARPS = 10, PR_THREADS = 32 * PR_WARPS;
+constexpr int SMEM_MAX = 227 * 1024, SMEM_FIXED = 2048;  // static shared memory and alignment
+constexpr int OUT_BYTES = 32 * 128;                      // a warp's piece of the output on its way
+constexpr int TMEM_COLS = 512;
 
 struct ProductArgs {
     const unsigned char *ps, *qs;
     void *out;
     int *status;
     long long p, q, out_stride;
-    int k, blocks, pitch;   // blocks of 32 per row, scale bytes per row
-    int stages, swap, vec;  // vec: 16-byte stores of a row's columns are aligned
+    int k, blocks, pitch;         // blocks of 32 per row, scale bytes per row
+    int stages, swap, vec, bulk;  // vec: 16-byte stores of a row's columns are aligned; bulk: the output has a tensor map
+    int accs;                     // accumulators in TMEM
+    unsigned ptiles, tiles;
+    int wide;                     // scales may be read 16 bytes at a time
 };
 
 // D (+)= A B^T, 64 elements of K; the scales' columns in TMEM, which half of their words in idesc
@@ -64,6 +72,15 @@ __device__ __forceinline__ void tma_rows(void *dst, const CUtensorMap *map, int 
                  "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
                  : "memory");
 }
+// a box of the output from shared memory; what lies outside the output is left out
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, int x, int y, const void *src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+                 "r"(smem_u32(src))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void stores_have_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void arrive(void *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -82,12 +99,15 @@ __device__ __forceinline__ float remote_f32(uint32_t addr, uint32_t rank) {
 template <int BN>
 struct ProductTile {
     static constexpr int QBLOCKS = (BN + 127) / 128;                      // 128-row pieces of Q's scales
+    static constexpr int ROWS = 1 + QBLOCKS;                              // scale rows per thread
     static constexpr int CODES = (PT + BN) * KBYTES;                      // bytes of codes per stage
-    static constexpr int SCALES = 2 * 512 * (1 + QBLOCKS);                // bytes of scales per stage
+    static constexpr int SCALES = 2 * 512 * ROWS;                         // bytes of scales per stage
     static constexpr int STAGE = CODES + SCALES;                          // a multiple of 1024
-    static constexpr int SCOLS = 2 * 4 * (1 + QBLOCKS);                   // TMEM columns of a stage's scales
-    static constexpr int MAX_STAGES = (SMEM_MAX - SMEM_HEAD - 1024) / STAGE > 8 ? 8 : (SMEM_MAX - SMEM_HEAD - 1024) / STAGE;
+    static constexpr int SCOLS = 2 * 4 * ROWS;                            // TMEM columns of a stage's scales
+    static constexpr int FIT = (SMEM_MAX - SMEM_FIXED - 4 * OUT_BYTES) / STAGE;
+    static constexpr int MAX_STAGES = FIT > 8 ? 8 : FIT;
     static_assert(STAGE % 1024 == 0, "tiles start on swizzle atoms");
+    static_assert(2 * BN + MAX_STAGES * SCOLS <= TMEM_COLS, "two accumulators and the scales fit TMEM");
 };
 
 // 16 columns of one row (or, transposed, 16 rows of one column)
@@ -118,139 +138,235 @@ __device__ __forceinline__ void product_store(const ProductArgs &a, long long p,
     }
 }
 
+// The 32 rows of a warp, columns [c, c + 128 bytes) of the accumulator, rounded and laid out as the tensor map's swizzle wants:
+// row r's 16-byte piece b at 128 r + 16 (b ^ (r mod 8)).
+template <class O>
+__device__ __forceinline__ void stage_output(unsigned char *to, uint32_t tmem) {
+    constexpr int COLS = 128 / (int)sizeof(O), N = 16 / (int)sizeof(O);
+    const int lane = threadIdx.x & 31;
+    float f[COLS];
+#pragma unroll
+    for (int c = 0; c < COLS; c += 16) tmem_ld16(tmem + c, f + c);
+    tmem_wait_ld();
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        Vec<O, N> v;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v.set(e, f[b * N + e]);
+        *reinterpret_cast<uint4 *>(to + lane * 128 + ((b ^ (lane & 7)) << 4)) = v.raw[0];
+    }
+}
+
+// stages of K per block of a cluster: an even number, as scales are read two stages at a time
+__host__ __device__ constexpr int part_of_k(int all, int S) { return S == 1 ? all : ((all + S - 1) / S + 1) / 2 * 2; }
+
 template <int BN, class O>
-__global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_constant__ CUtensorMap pmap,
-                                                             const __grid_constant__ CUtensorMap qmap, const ProductArgs a) {
+__global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap qmap,
+                                                             const __grid_constant__ CUtensorMap omap, const ProductArgs a) {
     using Tile = ProductTile<BN>;
+    constexpr int ROWS = Tile::ROWS;
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up, copies;
-    __shared__ __align__(8) uint64_t full[8], empty[8], done;
+    __shared__ __align__(8) uint64_t full[8], empty[8], ready[2], taken[2];
     // tiles need 1024-byte alignment; the block's own offset is the same in all blocks of a cluster
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    unsigned char *outs = smem + a.stages * Tile::STAGE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = gridDim.z, rank = blockIdx.z;
-    const long long p0 = (long long)blockIdx.x * PT, q0 = (long long)blockIdx.y * BN;
-    const int all = (a.k + KSTAGE - 1) / KSTAGE;
-    const int per = (all + S - 1) / S;
+    const int all = (a.k + KSTAGE - 1) / KSTAGE, per = part_of_k(all, S);
     const int s0 = min(rank * per, all), s1 = min(s0 + per, all), steps = s1 - s0;
+    const unsigned mine = blockIdx.x < a.tiles ? (a.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;  // tiles of this block
+    auto tile_p = [&](unsigned n) { return (long long)((blockIdx.x + n * gridDim.x) % a.ptiles) * PT; };
+    auto tile_q = [&](unsigned n) { return (long long)((blockIdx.x + n * gridDim.x) / a.ptiles) * BN; };
     uint32_t cols = 32;
-    while (cols < (uint32_t)(BN + a.stages * Tile::SCOLS)) cols *= 2;
+    while (cols < (uint32_t)(a.accs * BN + a.stages * Tile::SCOLS)) cols *= 2;
 
-    if (warp == 5) tmem_alloc(&tmem_slot, cols);
+    if (warp == 9) tmem_alloc(&tmem_slot, cols);
     if (threadIdx.x == 0) {
-        gave_up = 0;
+        gave_up = copies = 0;
         for (int s = 0; s < a.stages; ++s) {
             mbar_init(&full[s], 1 + 4);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(&done, 1);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&ready[b], 1);
+            mbar_init(&taken[b], 4);
+        }
         fence_mbar_init();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = tmem_slot, scales = tmem + a.accs * BN;
 
-    if (warp == 4) {
+    if (warp == 8) {
         if (lane == 0) {
-            int issued = 0;
-            for (; issued < steps; ++issued) {
-                const int st = issued % a.stages, round = issued / a.stages;
-                if (round && !mbar_wait(&empty[st], (round - 1) & 1)) {
-                    atomicExch(&gave_up, 1);
-                    break;
+            int st = 0, round = 0, issued = 0;
+            bool ok = true;
+            for (unsigned n = 0; n < mine && ok; ++n) {
+                const int y = (int)tile_p(n), z = (int)tile_q(n);
+                for (int i = 0; i < steps; ++i) {
+                    if (round) ok = mbar_wait(&empty[st], (round - 1) & 1);
+                    if (!ok) break;
+                    unsigned char *t = smem + st * Tile::STAGE;
+                    arrive_expect(&full[st], Tile::CODES);
+                    tma_rows(t, &pmap, (s0 + i) * KBYTES, y, &full[st]);
+                    tma_rows(t + PT * KBYTES, &qmap, (s0 + i) * KBYTES, z, &full[st]);
+                    ++issued;
+                    if (++st == a.stages) st = 0, ++round;
                 }
-                unsigned char *t = smem + st * Tile::STAGE;
-                arrive_expect(&full[st], Tile::CODES);
-                tma_rows(t, &pmap, (s0 + issued) * KBYTES, (int)p0, &full[st]);
-                tma_rows(t + PT * KBYTES, &qmap, (s0 + issued) * KBYTES, (int)q0, &full[st]);
             }
             copies = issued;
-        }
-    } else if (warp == 5) {
-        if (lane == 0) {
-            bool ok = true;
-            for (int i = 0; i < steps && ok; ++i) {
-                const int st = i % a.stages;
-                ok = mbar_wait(&full[st], (i / a.stages) & 1);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t t = smem_u32(smem + st * Tile::STAGE), sc = t + Tile::CODES;
-                const uint32_t scol = tmem + BN + st * Tile::SCOLS;
-                // half h of the stage: the word of P's rows, then those of Q's
-#pragma unroll
-                for (int b = 0; b < 2 * (1 + Tile::QBLOCKS); ++b) scales_to_tmem(scol + 4 * b, sdesc(sc + 512 * b, 16, 128));
-                const int left = a.k - (s0 + i) * KSTAGE;
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    if (m * 64 >= left) break;
-                    const uint32_t sa = scol + (m / 2) * 4 * (1 + Tile::QBLOCKS);
-                    mma_mxf4(tmem, desc_sw128(t + m * 32), desc_sw128(t + PT * KBYTES + m * 32), idesc_mxf4(BN, m & 1), sa, sa + 4,
-                             (i | m) != 0);
-                }
-                mma_commit(&empty[st]);
-            }
             if (!ok) atomicExch(&gave_up, 1);
-            mma_commit(&done);
         }
-    } else {
-        // scales: thread r has row r of P and rows r, r + 128 of Q; the words of 4 stages are loaded together, one such group ahead
-        constexpr int G = 4, ROWS = 1 + Tile::QBLOCKS;
-        const unsigned *src[ROWS];
-        src[0] = p0 + threadIdx.x < a.p ? reinterpret_cast<const unsigned *>(a.ps + (p0 + threadIdx.x) * a.pitch) : nullptr;
+    } else if (warp == 9) {
+        if (lane == 0) {
+            int st = 0, round = 0;
+            bool ok = true;
+            for (unsigned n = 0; n < mine && ok; ++n) {
+                const int buf = a.accs == 2 ? n & 1 : 0;
+                const unsigned use = a.accs == 2 ? n >> 1 : n;  // how often the accumulator was used before
+                if (use) ok = mbar_wait(&taken[buf], (use - 1) & 1);
+                const uint32_t d = tmem + buf * BN;
+                for (int i = 0; i < steps && ok; ++i) {
+                    ok = mbar_wait(&full[st], round & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t t = smem_u32(smem + st * Tile::STAGE), sc = t + Tile::CODES, scol = scales + st * Tile::SCOLS;
+                    // half h of the stage: the word of P's rows, then those of Q's
 #pragma unroll
-        for (int b = 0; b < Tile::QBLOCKS; ++b) {
-            const int r = b * 128 + threadIdx.x;
-            src[1 + b] = r < BN && q0 + r < a.q ? reinterpret_cast<const unsigned *>(a.qs + (q0 + r) * a.pitch) : nullptr;
-        }
-        unsigned next[G][ROWS][2], cur[G][ROWS][2];
-        auto fetch = [&](int i0) {
+                    for (int b = 0; b < 2 * ROWS; ++b) scales_to_tmem(scol + 4 * b, sdesc(sc + 512 * b, 16, 128));
+                    const int left = a.k - (s0 + i) * KSTAGE;
 #pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int b = 0; b < ROWS; ++b)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int word = (s0 + i0 + g) * 2 + h, left = a.blocks - word * 4;
-                        unsigned v = 0;
-                        if (src[b] && i0 + g < steps && left > 0) {
-                            v = __ldg(src[b] + word);
-                            if (left < 4) v &= (1u << (8 * left)) - 1u;  // bytes past the last block are not scales
-                        }
-                        next[g][b][h] = v;
+                    for (int m = 0; m < 4; ++m) {
+                        if (m * 64 >= left) break;
+                        const uint32_t sa = scol + (m / 2) * 4 * ROWS;
+                        mma_mxf4(d, desc_sw128(t + m * 32), desc_sw128(t + PT * KBYTES + m * 32), idesc_mxf4(BN, m & 1), sa, sa + 4,
+                                 (i | m) != 0);
                     }
+                    mma_commit(&empty[st]);
+                    if (++st == a.stages) st = 0, ++round;
+                }
+                if (!ok) {  // known before the tile counts as ready
+                    atomicExch(&gave_up, 1);
+                    __threadfence_block();
+                }
+                mma_commit(&ready[buf]);
+            }
+        }
+    } else if (warp >= 4) {
+        // thread r has row r of P and rows r, r + 128 of Q, 4 words (2 stages) at a time: groups (tile, pair of stages), two ahead
+        const int r = threadIdx.x - 128, pairs = (steps + 1) / 2, words = a.pitch / 4;
+        const unsigned groups = mine * (unsigned)pairs;
+        unsigned ftile = 0;
+        int fpair = 0;
+        auto fetch = [&](uint4 (&v)[ROWS]) {
+#pragma unroll
+            for (int b = 0; b < ROWS; ++b) v[b] = make_uint4(0, 0, 0, 0);
+            if (ftile >= mine) return;
+            const int w = (s0 + 2 * fpair) * 2;
+#pragma unroll
+            for (int b = 0; b < ROWS; ++b) {
+                const int o = b ? (b - 1) * 128 + r : r;
+                const long long row = b ? tile_q(ftile) + o : tile_p(ftile) + o;
+                if (row >= (b ? a.q : a.p) || (b && o >= BN)) continue;
+                const unsigned *src = reinterpret_cast<const unsigned *>((b ? a.qs : a.ps) + row * a.pitch) + w;
+                if (a.wide) {
+                    v[b] = __ldg(reinterpret_cast<const uint4 *>(src));
+                } else {
+                    v[b].x = __ldg(src);
+                    if (w + 1 < words) v[b].y = __ldg(src + 1);
+                    if (w + 2 < words) v[b].z = __ldg(src + 2);
+                    if (w + 3 < words) v[b].w = __ldg(src + 3);
+                }
+            }
+            if (++fpair == pairs) fpair = 0, ++ftile;
         };
-        fetch(0);
+        uint4 next[2][ROWS];
+        if (pairs) {
+            fetch(next[0]);
+            fetch(next[1]);
+        }
+        int st = 0, round = 0, pair = 0;
         bool ok = true;
-        for (int i0 = 0; i0 < steps && ok; i0 += G) {
+        const int at = (r & 31) * 4 + (r >> 5);
+        for (unsigned g = 0; g < groups && ok; ++g) {
+            uint4 cur[ROWS];
 #pragma unroll
-            for (int g = 0; g < G; ++g)
+            for (int b = 0; b < ROWS; ++b) {
+                cur[b] = next[0][b];
+                next[0][b] = next[1][b];
+            }
+            fetch(next[1]);
 #pragma unroll
-                for (int b = 0; b < ROWS; ++b)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) cur[g][b][h] = next[g][b][h];
-            if (i0 + G < steps) fetch(i0 + G);
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const int i = i0 + g;
-                if (i >= steps || !ok) break;
-                const int st = i % a.stages, round = i / a.stages;
+            for (int h = 0; h < 2; ++h) {
+                const int i = 2 * pair + h;
+                if (i >= steps) break;
                 if (round) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1));
                 if (!ok) break;
                 unsigned *sc = reinterpret_cast<unsigned *>(smem + st * Tile::STAGE + Tile::CODES);
-                const int at = (threadIdx.x & 31) * 4 + warp;
+                // bytes past the last block are not scales
+                const int left = a.blocks - (s0 + i) * 8;
+                const unsigned lo = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+                const unsigned hi = left >= 8 ? 0xffffffffu : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int b = 0; b < ROWS; ++b) sc[(h * ROWS + b) * 128 + at] = cur[g][b][h];
+                for (int b = 0; b < ROWS; ++b) {
+                    sc[b * 128 + at] = (h ? cur[b].z : cur[b].x) & lo;
+                    sc[(ROWS + b) * 128 + at] = (h ? cur[b].w : cur[b].y) & hi;
+                }
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) arrive(&full[st]);
+                if (++st == a.stages) st = 0, ++round;
             }
+            if (++pair == pairs) pair = 0;
         }
         if (!ok && lane == 0) atomicExch(&gave_up, 1);
-        if (!mbar_wait(&done, 0)) atomicExch(&gave_up, 1);
+    } else if (S == 1) {
+        constexpr int OC = 128 / (int)sizeof(O);  // output columns of 128 bytes
+        unsigned char *out = outs + warp * OUT_BYTES;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        bool ok = true;
+        for (unsigned n = 0; n < mine; ++n) {
+            const int buf = a.accs == 2 ? n & 1 : 0;
+            const unsigned use = a.accs == 2 ? n >> 1 : n;
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&ready[buf], use & 1));
+            // a wait that ran out before this tile's commit shows here
+            if (*(volatile int *)&gave_up) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            const long long p0 = tile_p(n), q0 = tile_q(n);
+            const uint32_t d = tmem + lanes + buf * BN;
+            if (ok && a.bulk && BN >= OC) {
+                for (int c = 0; c < BN && q0 + c < a.q && p0 + warp * 32 < a.p; c += OC) {
+                    if (lane == 0) stores_have_read();
+                    __syncwarp();
+                    stage_output<O>(out, d + c);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tma_store(&omap, (int)(q0 + c), (int)p0 + warp * 32, out);
+                }
+            } else {
+#pragma unroll 2
+                for (int c = 0; c < BN; c += 16) {
+                    float f[16];
+                    tmem_ld16(d + c, f);
+                    tmem_wait_ld();
+                    if (!ok)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(0x7fc00000u);
+                    if (q0 + c < a.q) product_store<O>(a, p0 + threadIdx.x, q0 + c, f);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(&taken[buf]);
+        }
+        if (!ok && lane == 0) atomicExch(&gave_up, 1);
+        if (lane == 0) stores_done();
+    } else {
+        if (!mbar_wait(&ready[0], 0)) atomicExch(&gave_up, 1);
         tc_fence_after();
     }
     __syncthreads();
@@ -260,22 +376,7 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
         for (int i = max(0, copies - a.stages); i < copies; ++i) mbar_wait(&full[i % a.stages], (i / a.stages) & 1);
         if (a.status) atomicOr(a.status, (int)ERR_MBAR);
     }
-    const float nan = __uint_as_float(0x7fc00000u);
-    if (S == 1) {
-        if (warp < 4) {
-            const long long p = p0 + threadIdx.x;
-#pragma unroll 2
-            for (int c = 0; c < BN; c += 16) {
-                float f[16];
-                tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c, f);
-                tmem_wait_ld();
-                if (bad)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) f[i] = nan;
-                if (q0 + c < a.q) product_store<O>(a, p, q0 + c, f);
-            }
-        }
-    } else {
+    if (S > 1) {
         // every block leaves its tile in its shared memory (the stages are free), then adds a share of the columns
         float *part = reinterpret_cast<float *>(smem);
         if (warp < 4) {
@@ -284,18 +385,22 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
                 tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c, f);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) part[(c + i) * PT + threadIdx.x] = bad ? nan : steps ? f[i] : 0.0f;
+                for (int i = 0; i < 16; ++i) part[(c + i) * PT + threadIdx.x] = bad ? __uint_as_float(0x7fc00000u) : steps ? f[i] : 0.0f;
             }
         }
         cluster_sync();
         if (warp < 4) {
-            const long long p = p0 + threadIdx.x;
+            const long long p = tile_p(0) + threadIdx.x, q0 = tile_q(0);
             O *out = static_cast<O *>(a.out);
             for (int c = rank; c < BN; c += S) {
                 const long long q = q0 + c;
                 if (q >= a.q || p >= a.p) continue;
+                float v[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] = r < S ? remote_f32(smem_u32(part + c * PT + threadIdx.x), r) : 0.0f;
                 float t = 0.0f;
-                for (int r = 0; r < S; ++r) t += remote_f32(smem_u32(part + c * PT + threadIdx.x), r);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) t += v[r];
                 out[a.swap ? q * a.out_stride + p : p * a.out_stride + q] = from_f32<O>(t);
             }
         }
@@ -303,7 +408,7 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 5) tmem_dealloc(tmem, cols);
+    if (warp == 9) tmem_dealloc(tmem, cols);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -322,36 +427,46 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-int code_map(CUtensorMap *map, const unsigned char *codes, long long rows, int blocks, int box_rows) {
+// rows of `cols` elements, in boxes of 128 bytes by box_rows
+int matrix_map(CUtensorMap *map, CUtensorMapDataType type, int size, const void *p, long long rows, long long cols, long long stride, int box_rows) {
     const EncodeTiled encode = encode_tiled();
     if (!encode) {
         set_error("flare_micro_product: the driver has no cuTensorMapEncodeTiled");
         return FLARE_E_CUDA;
     }
-    const cuuint64_t dims[2] = {(cuuint64_t)16 * blocks, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)16 * blocks};
-    const cuuint32_t box[2] = {KBYTES, (cuuint32_t)box_rows}, step[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<unsigned char *>(codes), dims, strides, box, step,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(stride * size)};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const CUresult r = encode(map, type, 2, const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        set_error("flare_micro_product: tensor map of %lld rows of %d bytes: error %d", rows, 16 * blocks, (int)r);
+        set_error("flare_micro_product: tensor map of %lld rows of %lld: error %d", rows, cols, (int)r);
         return FLARE_E_CUDA;
     }
     return FLARE_OK;
 }
 
 template <int BN, class O>
-int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, ProductArgs a, int split, cudaStream_t st) {
+int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorMap &om, ProductArgs a, int split, cudaStream_t st) {
     using Tile = ProductTile<BN>;
-    const int steps = (a.k + KSTAGE - 1) / KSTAGE, per = (steps + split - 1) / split;
-    a.stages = std::min(Tile::MAX_STAGES, std::max(per, 1));
-    int smem = a.stages * Tile::STAGE + 1024;
+    const int per = part_of_k((a.k + KSTAGE - 1) / KSTAGE, split);
+    a.ptiles = (unsigned)((a.p + PT - 1) / PT);
+    const long long tiles = (long long)a.ptiles * ((a.q + BN - 1) / BN);
+    if (tiles > 0x7fffffff) {
+        set_error("flare_micro_product: %lld tiles", tiles);
+        return FLARE_E_INVALID;
+    }
+    a.tiles = (unsigned)tiles;
+    const unsigned grid = split > 1 ? a.tiles : (unsigned)std::min<long long>(tiles, SMS);
+    a.accs = grid < a.tiles ? 2 : 1;
+    // no more stages than the block's tiles have
+    a.stages = (int)std::min<long long>(Tile::MAX_STAGES, per * ((tiles + grid - 1) / grid));
+    int smem = a.stages * Tile::STAGE + 4 * OUT_BYTES + 1024;
     if (split > 1) smem = std::max(smem, PT * BN * 4 + 1024);
     auto fn = product_kernel<BN, O>;
     const int e0 = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_micro_product");
     if (e0) return e0;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((a.p + PT - 1) / PT), (unsigned)((a.q + BN - 1) / BN), (unsigned)split);
+    cfg.gridDim = dim3(grid, 1, (unsigned)split);
     cfg.blockDim = dim3(PR_THREADS);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
@@ -361,7 +476,7 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, ProductArgs a, 
     attr.val.clusterDim.z = (unsigned)split;
     cfg.attrs = &attr;
     cfg.numAttrs = split > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, pm, qm, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, pm, qm, om, a);
     if (e != cudaSuccess) {
         set_error("flare_micro_product: %s", cudaGetErrorString(e));
         return FLARE_E_CUDA;
@@ -383,29 +498,38 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     a.k = in->k;
     a.blocks = (in->k + 31) / 32;
     a.pitch = 4 * ((a.blocks + 3) / 4);
-    a.vec = fits_vec(in->out, in->out_stride, type_size(in->out_type), 16 / type_size(in->out_type));
-    // columns per tile: what Q has, at most 256; narrower where that leaves multiprocessors without a tile
+    a.wide = a.pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(a.ps) | reinterpret_cast<uintptr_t>(a.qs)) % 16 == 0;
+    const int size = type_size(in->out_type);
+    a.vec = fits_vec(in->out, in->out_stride, size, 16 / size);
+    // columns per tile: what Q has, at most 192 (two accumulators of 192 and the scales fill TMEM); narrower where that leaves
+    // multiprocessors without a tile
     int bn = 16;
-    while (bn < 256 && bn < a.q) bn *= 2;
+    while (bn < 128 && bn < a.q) bn *= 2;
     const long long ptiles = (a.p + PT - 1) / PT;
     auto tiles = [&](int b) { return ptiles * ((a.q + b - 1) / b); };
+    if (bn < a.q && tiles(192) >= SMS) bn = 192;
     while (bn > 64 && tiles(bn) < SMS) bn /= 2;
     // and then parts of K, at least two stages each
     const int steps = (in->k + KSTAGE - 1) / KSTAGE;
     int split = 1;
     while (split < 8 && tiles(bn) * split * 2 <= SMS && steps >= split * 4) split *= 2;
-    CUtensorMap pm, qm;
-    int e = code_map(&pm, pc, a.p, a.blocks, PT);
-    if (!e) e = code_map(&qm, qc, a.q, a.blocks, bn);
+    // whole 128-byte pieces of output rows go by TMA
+    a.bulk = !a.swap && split == 1 && a.vec && bn * size >= 128;
+    CUtensorMap pm, qm, om{};
+    int e = matrix_map(&pm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pc, a.p, 16ll * a.blocks, 16ll * a.blocks, PT);
+    if (!e) e = matrix_map(&qm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, a.q, 16ll * a.blocks, 16ll * a.blocks, bn);
+    if (!e && a.bulk)
+        e = matrix_map(&om, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, size, in->out, in->m, in->n,
+                       in->out_stride, 32);
     if (e) return e;
     return with_type(in->out_type, [&](auto t) {
         using O = typename decltype(t)::type;
         switch (bn) {
-            case 16: return launch_product<16, O>(pm, qm, a, split, st);
-            case 32: return launch_product<32, O>(pm, qm, a, split, st);
-            case 64: return launch_product<64, O>(pm, qm, a, split, st);
-            case 128: return launch_product<128, O>(pm, qm, a, split, st);
-            default: return launch_product<256, O>(pm, qm, a, split, st);
+            case 16: return launch_product<16, O>(pm, qm, om, a, split, st);
+            case 32: return launch_product<32, O>(pm, qm, om, a, split, st);
+            case 64: return launch_product<64, O>(pm, qm, om, a, split, st);
+            case 128: return launch_product<128, O>(pm, qm, om, a, split, st);
+            default: return launch_product<192, O>(pm, qm, om, a, split, st);
         }
     });
 }
