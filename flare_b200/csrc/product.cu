@@ -412,6 +412,201 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------
+// One stage of K (k <= 256) and one tile of Q: a small layer over very many rows.  Q and its scales stay in shared memory and
+// TMEM; what moves is P, 16 ceil(k / 32) contiguous bytes a row, and the output.  TMA takes such short rows one by one (147
+// us for 1M x 64 x 96), so warps 4-7 copy P's tile by 16-byte asynchronous copies, consecutive threads consecutive pieces, into
+// the swizzled layout, NARROW_AHEAD tiles ahead.  Pieces past a row's end stay zero from the start.
+// ------------------------------------------------------------------------------------------------
+constexpr int NARROW_STAGES = 4, NARROW_AHEAD = 2, NARROW_BLOCKS = 2;  // blocks per multiprocessor
+
+template <int BN>
+struct NarrowTile {
+    static constexpr int P = PT * KBYTES, PS = 2 * 512;              // a stage: codes, scales
+    static constexpr int Q = BN * KBYTES, QS = 2 * 512;
+    static constexpr int ACCS = BN > 64 ? 1 : 2;                     // two blocks share TMEM
+    static constexpr int COLS = ACCS * BN + 8 * NARROW_STAGES + 8 <= 64 ? 64 : ACCS * BN + 8 * NARROW_STAGES + 8 <= 128 ? 128 : 256;
+    static constexpr int SMEM = 1024 + Q + NARROW_STAGES * P + NARROW_STAGES * PS + QS + 4 * OUT_BYTES;
+    static_assert(BN <= 128 && ACCS * BN + 8 * NARROW_STAGES + 8 <= 256, "TMEM of two blocks");
+};
+
+template <int BN, class O>
+__global__ void __launch_bounds__(PR_THREADS, NARROW_BLOCKS) product_narrow_kernel(const __grid_constant__ CUtensorMap omap, const unsigned char *pc,
+                                                                                   const unsigned char *qc, const ProductArgs a) {
+    using Tile = NarrowTile<BN>;
+    constexpr int ST = NARROW_STAGES;
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int gave_up;
+    __shared__ __align__(8) uint64_t full[ST], empty[ST], ready[2], taken[2];
+    unsigned char *qtile = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    unsigned char *ptile = qtile + Tile::Q, *outs = ptile + ST * Tile::P;
+    unsigned char *pscale = outs + 4 * OUT_BYTES, *qscale = pscale + ST * Tile::PS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned mine = blockIdx.x < a.tiles ? (a.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+    auto tile_p = [&](unsigned n) { return (long long)(blockIdx.x + n * gridDim.x) * PT; };
+    // byte of piece b (16 bytes) of row r in a 128-byte-swizzled tile
+    auto place = [](int r, int b) { return r * 128 + ((b ^ (r & 7)) << 4); };
+    // half h of 128 rows' scales: row r's word
+    auto scale_place = [](int r, int h) { return h * 512 + (r & 31) * 16 + (r >> 5) * 4; };
+    auto scale_word = [&](const unsigned char *scales, long long row, int h) {
+        const int left = a.blocks - 4 * h;
+        if (left <= 0) return 0u;
+        const unsigned v = __ldg(reinterpret_cast<const unsigned *>(scales + row * a.pitch) + h);
+        return left < 4 ? v & ((1u << (8 * left)) - 1u) : v;  // bytes past the last block are not scales
+    };
+
+    if (warp == 9) tmem_alloc(&tmem_slot, Tile::COLS);
+    if (threadIdx.x == 0) {
+        gave_up = 0;
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&full[s], 4);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&ready[b], 1);
+            mbar_init(&taken[b], 4);
+        }
+        fence_mbar_init();
+    }
+    // Q, and zeros where P's rows have no pieces
+    for (int c = threadIdx.x; c < BN * 8; c += PR_THREADS) {
+        const int r = c >> 3, b = c & 7;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (b < a.blocks && r < a.q) v = __ldg(reinterpret_cast<const uint4 *>(qc + (long long)r * 16 * a.blocks) + b);
+        *reinterpret_cast<uint4 *>(qtile + place(r, b)) = v;
+    }
+    for (int c = threadIdx.x; c < 256; c += PR_THREADS) {
+        const int r = c & 127, h = c >> 7;
+        *reinterpret_cast<unsigned *>(qscale + scale_place(r, h)) = r < BN && r < a.q ? scale_word(a.qs, r, h) : 0u;
+    }
+    for (int c = threadIdx.x; c < ST * PT * 8; c += PR_THREADS)
+        if ((c & 7) >= a.blocks) *reinterpret_cast<uint4 *>(ptile + (c >> 10) * Tile::P + place((c >> 3) & 127, c & 7)) = make_uint4(0, 0, 0, 0);
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot, pscol = tmem + Tile::ACCS * BN, qscol = pscol + 8 * ST;
+
+    if (warp == 9) {
+        if (lane == 0) {
+            bool ok = true;
+            for (int h = 0; h < 2; ++h) scales_to_tmem(qscol + 4 * h, sdesc(smem_u32(qscale) + 512 * h, 16, 128));
+            for (unsigned n = 0; n < mine && ok; ++n) {
+                const int st = n % ST, buf = n % Tile::ACCS;
+                const unsigned use = n / Tile::ACCS;
+                if (use) ok = mbar_wait(&taken[buf], (use - 1) & 1);
+                if (ok) ok = mbar_wait(&full[st], (n / ST) & 1);
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t t = smem_u32(ptile + st * Tile::P), sc = smem_u32(pscale + st * Tile::PS), scol = pscol + 8 * st;
+                    for (int h = 0; h < 2; ++h) scales_to_tmem(scol + 4 * h, sdesc(sc + 512 * h, 16, 128));
+                    for (int m = 0; m * 64 < a.k; ++m)
+                        mma_mxf4(tmem + buf * BN, desc_sw128(t + m * 32), desc_sw128(smem_u32(qtile) + m * 32), idesc_mxf4(BN, m & 1),
+                                 scol + (m / 2) * 4, qscol + (m / 2) * 4, m != 0);
+                    mma_commit(&empty[st]);
+                } else {
+                    atomicExch(&gave_up, 1);
+                    __threadfence_block();
+                }
+                mma_commit(&ready[buf]);
+            }
+        }
+    } else if (warp >= 4 && warp < 8) {
+        const int r = threadIdx.x - 128;
+        // this thread's pieces of a tile, at most 8: piece c of the tile's contiguous bytes
+        int to[8], row[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = j * 128 + r;
+            row[j] = j < a.blocks ? c / a.blocks : 0;
+            to[j] = j < a.blocks ? place(row[j], c - row[j] * a.blocks) : 0;
+        }
+        bool ok = true;
+        unsigned w0 = 0, w1 = 0;
+        auto words = [&](unsigned n) {
+            w0 = w1 = 0;
+            if (n < mine && tile_p(n) + r < a.p) {
+                w0 = scale_word(a.ps, tile_p(n) + r, 0);
+                w1 = scale_word(a.ps, tile_p(n) + r, 1);
+            }
+        };
+        words(0);
+        for (unsigned n = 0; n < mine + NARROW_AHEAD && ok; ++n) {
+            if (n < mine) {
+                const int st = n % ST;
+                if (n >= ST) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (n / ST - 1) & 1));
+                if (!ok) break;
+                const long long p0 = tile_p(n);
+                const unsigned char *from = pc + p0 * 16 * a.blocks + r * 16;
+                const uint32_t at = smem_u32(ptile + st * Tile::P);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    // rows past the last are left as they are: their outputs are not stored
+                    if (j < a.blocks && p0 + row[j] < a.p)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + to[j]), "l"(from + j * 2048) : "memory");
+                unsigned char *sc = pscale + st * Tile::PS;
+                *reinterpret_cast<unsigned *>(sc + scale_place(r, 0)) = w0;
+                *reinterpret_cast<unsigned *>(sc + scale_place(r, 1)) = w1;
+                words(n + 1);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (n >= NARROW_AHEAD) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(NARROW_AHEAD) : "memory");
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) arrive(&full[(n - NARROW_AHEAD) % ST]);
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!ok && lane == 0) atomicExch(&gave_up, 1);
+    } else if (warp < 4) {
+        constexpr int OC = 128 / (int)sizeof(O);
+        unsigned char *out = outs + warp * OUT_BYTES;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        bool ok = true;
+        for (unsigned n = 0; n < mine; ++n) {
+            const int buf = n % Tile::ACCS;
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&ready[buf], (n / Tile::ACCS) & 1));
+            if (*(volatile int *)&gave_up) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            const long long p0 = tile_p(n);
+            const uint32_t d = tmem + lanes + buf * BN;
+            if (ok && a.bulk && BN >= OC) {
+                for (int c = 0; c < BN && c < a.q && p0 + warp * 32 < a.p; c += OC) {
+                    if (lane == 0) stores_have_read();
+                    __syncwarp();
+                    stage_output<O>(out, d + c);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tma_store(&omap, c, (int)p0 + warp * 32, out);
+                }
+            } else {
+#pragma unroll 2
+                for (int c = 0; c < BN; c += 16) {
+                    float f[16];
+                    tmem_ld16(d + c, f);
+                    tmem_wait_ld();
+                    if (!ok)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(0x7fc00000u);
+                    if (c < a.q) product_store<O>(a, p0 + threadIdx.x, c, f);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(&taken[buf]);
+        }
+        if (!ok && lane == 0) atomicExch(&gave_up, 1);
+        if (lane == 0) stores_done();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *(volatile int *)&gave_up && a.status) atomicOr(a.status, (int)ERR_MBAR);
+    if (warp == 9) tmem_dealloc(tmem, Tile::COLS);
+}
+
+// ------------------------------------------------------------------------------------------------
 
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -484,6 +679,17 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorM
     return FLARE_OK;
 }
 
+template <int BN, class O>
+int launch_narrow(const CUtensorMap &om, const unsigned char *pc, const unsigned char *qc, ProductArgs a, cudaStream_t st) {
+    a.tiles = (unsigned)((a.p + PT - 1) / PT);
+    auto fn = product_narrow_kernel<BN, O>;
+    const int e = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_micro_product");
+    if (e) return e;
+    fn<<<std::min(a.tiles, (unsigned)(NARROW_BLOCKS * SMS)), PR_THREADS, NarrowTile<BN>::SMEM, st>>>(om, pc, qc, a);
+    OPS_LAUNCHED("flare_micro_product");
+    return FLARE_OK;
+}
+
 int run_product(const flare_product_args *in, cudaStream_t st) {
     ProductArgs a{};
     a.swap = in->m < in->n;  // the larger matrix gives the tiles' 128 rows
@@ -501,6 +707,26 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     a.wide = a.pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(a.ps) | reinterpret_cast<uintptr_t>(a.qs)) % 16 == 0;
     const int size = type_size(in->out_type);
     a.vec = fits_vec(in->out, in->out_stride, size, 16 / size);
+    const CUtensorMapDataType out_map = size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    CUtensorMap pm, qm, om{};
+    int e = FLARE_OK;
+    // one stage of K and one tile of Q, over at least two tiles a multiprocessor
+    if (in->k <= KSTAGE && a.q <= 128 && a.p >= 2ll * SMS * PT) {
+        int bn = 16;
+        while (bn < a.q) bn *= 2;
+        a.bulk = !a.swap && a.vec && bn * size >= 128;
+        if (a.bulk) e = matrix_map(&om, out_map, size, in->out, in->m, in->n, in->out_stride, 32);
+        if (e) return e;
+        return with_type(in->out_type, [&](auto t) {
+            using O = typename decltype(t)::type;
+            switch (bn) {
+                case 16: return launch_narrow<16, O>(om, pc, qc, a, st);
+                case 32: return launch_narrow<32, O>(om, pc, qc, a, st);
+                case 64: return launch_narrow<64, O>(om, pc, qc, a, st);
+                default: return launch_narrow<128, O>(om, pc, qc, a, st);
+            }
+        });
+    }
     // columns per tile: what Q has, at most 192 (two accumulators of 192 and the scales fill TMEM); narrower where that leaves
     // multiprocessors without a tile
     int bn = 16;
@@ -515,12 +741,10 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     while (split < 8 && tiles(bn) * split * 2 <= SMS && steps >= split * 4) split *= 2;
     // whole 128-byte pieces of output rows go by TMA
     a.bulk = !a.swap && split == 1 && a.vec && bn * size >= 128;
-    CUtensorMap pm, qm, om{};
-    int e = matrix_map(&pm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pc, a.p, 16ll * a.blocks, 16ll * a.blocks, PT);
+    e = matrix_map(&pm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pc, a.p, 16ll * a.blocks, 16ll * a.blocks, PT);
     if (!e) e = matrix_map(&qm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, a.q, 16ll * a.blocks, 16ll * a.blocks, bn);
     if (!e && a.bulk)
-        e = matrix_map(&om, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, size, in->out, in->m, in->n,
-                       in->out_stride, 32);
+        e = matrix_map(&om, out_map, size, in->out, in->m, in->n, in->out_stride, 32);
     if (e) return e;
     return with_type(in->out_type, [&](auto t) {
         using O = typename decltype(t)::type;

@@ -114,7 +114,8 @@ def test_product_of_whole_numbers_is_exact():
     """Codes and scales whose products and sums are small whole numbers: any order and any place of an element that is
     taken wrongly shows."""
     g = torch.Generator().manual_seed(5)
-    for m, n, k in ((300, 280, 520), (2, 700, 1030), (513, 64, 96), (4500, 2100, 1290), (2100, 4481, 2600), (70_000, 50, 96)):
+    for m, n, k in ((300, 280, 520), (2, 700, 1030), (513, 64, 96), (4500, 2100, 1290), (2100, 4481, 2600), (70_000, 50, 96),
+                    (90_001, 64, 96), (45_000, 128, 250), (12, 60_003, 31), (76_000, 17, 129)):
         lev = torch.tensor([0.0, 1.0, 2.0, 3.0, 4.0, -1.0, -2.0])
         a, b = lev[torch.randint(0, 7, (m, k), generator=g)], lev[torch.randint(0, 7, (n, k), generator=g)]
         for t in (a, b):
