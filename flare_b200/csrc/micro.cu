@@ -1,8 +1,9 @@
 // micro.cu -- microscaled 4-bit floats: to codes and scales and back (the format is described in the header).
 //
-// Both directions are bound by memory: 2.03 (16-bit input) to 4.53 bytes (f32) an element.  Four lanes share a block of
-// 32, 8 elements each, so that a warp's 16-byte loads are contiguous; the block's largest magnitude is exchanged by two
-// shuffles.
+// Both directions are bound by memory: 2.53 (16-bit values) to 4.53 bytes (f32) an element.  Where rows allow it a lane
+// has 16 consecutive elements, half a block, and reads or writes 32 bytes at a time; the block's largest magnitude takes one
+// exchange.  With 8 elements a lane the instructions per element bound it (3M x 96 f16: 207 us to codes and 150 us back).
+// Other rows go by 8 elements a lane, four lanes to a block.
 #include <algorithm>
 #include <mutex>
 #include <set>
@@ -40,9 +41,9 @@ struct MicroArgs {
     unsigned char *codes, *scales;
     const unsigned char *codes_in, *scales_in;
     long long stride, first;  // first: first row of this launch
-    unsigned items;           // 8-element pieces of this launch
+    unsigned items;           // 8- or 16-element pieces of this launch
     int width, blocks, pitch;
-    FastDiv ppr;              // pieces per row: 4 * blocks
+    FastDiv ppr;              // pieces per row: 4 or 2 per block
 };
 
 template <class T, bool VEC>
@@ -119,13 +120,142 @@ __global__ void __launch_bounds__(MQ_THREADS) micro_dequantize_kernel(const Micr
     }
 }
 
+// 32 bytes, aligned to as many
+__device__ __forceinline__ void load32(const void *p, unsigned (&w)[8]) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void store32(void *p, const unsigned (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) {
+    unsigned d;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// 16 elements of T in 32-byte words, and the largest magnitude's bits as a float's
+template <class T>
+struct Sixteen {
+    static constexpr int N = (int)sizeof(T) / 2;  // 32-byte pieces
+    unsigned w[N][8];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) load32(reinterpret_cast<const char *>(p) + 32 * i, w[i]);
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[i][k] = 0;
+    }
+    __device__ __forceinline__ float2 pair(int k) const {  // elements 2k, 2k + 1
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[k / 4][2 * k % 8]), __uint_as_float(w[k / 4][2 * k % 8 + 1]));
+        else if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2 *>(&w[0][k]));
+        else return make_float2(__uint_as_float(w[0][k] << 16), __uint_as_float(w[0][k] & 0xffff0000u));
+    }
+    // magnitudes compare as their bits do; infinities and NaN are the largest
+    __device__ __forceinline__ unsigned most() const {
+        unsigned m = 0;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) m = max(m, w[i][k] & 0x7fffffffu);
+            return m;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) m = max_u16x2(m, w[0][k] & 0x7fff7fffu);
+            m = max(m & 0xffffu, m >> 16);
+            if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+            else return m << 16;
+        }
+    }
+};
+
+// A lane per 16 elements of a row, two lanes per block
+template <class T>
+__global__ void __launch_bounds__(MQ_THREADS) micro_quantize16_kernel(const MicroArgs a) {
+    const unsigned it = blockIdx.x * MQ_THREADS + threadIdx.x;
+    const unsigned r = a.ppr.div(it), piece = it - r * a.ppr.d;
+    const long long row = a.first + r;
+    const bool in = it < a.items;
+    Sixteen<T> x;
+    if (in && (int)piece * 16 < a.width) x.load(static_cast<const T *>(a.x) + row * a.stride + piece * 16);
+    else x.zero();
+    unsigned most = x.most();
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    unsigned byte = 255, lo = 0, hi = 0;
+    if (most < 0x7f800000u) {
+        // floor(log2) of the largest is its exponent field - 127; below 2^-125 (subnormal ones too) the clamp decides
+        const int e = max((int)(most >> 23) - 127 - 2, -127);
+        byte = (unsigned)(e + 127);
+        const float inv = __uint_as_float((unsigned)(127 - e) << 23);  // 2^-e, e in [-127, 125]
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float2 v = x.pair(k);
+            const unsigned c = micro_code_pair(v.x * inv, v.y * inv);
+            if (k < 4) lo |= c << (8 * k);
+            else hi |= c << (8 * (k - 4));
+        }
+    }
+    if (!in) return;
+    __stcs(reinterpret_cast<uint2 *>(a.codes + row * (16ll * a.blocks)) + piece, make_uint2(lo, hi));
+    if ((piece & 1) == 0) {
+        unsigned char *s = a.scales + row * a.pitch;
+        const int b = (int)piece >> 1;
+        s[b] = (unsigned char)byte;
+        if (b == a.blocks - 1)
+            for (int k = a.blocks; k < a.pitch; ++k) s[k] = 0;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(MQ_THREADS) micro_dequantize16_kernel(const MicroArgs a) {
+    const unsigned it = blockIdx.x * MQ_THREADS + threadIdx.x;
+    if (it >= a.items) return;
+    const unsigned r = a.ppr.div(it), piece = it - r * a.ppr.d;
+    const long long row = a.first + r;
+    if ((int)piece * 16 >= a.width) return;
+    const uint2 c = __ldcs(reinterpret_cast<const uint2 *>(a.codes_in + row * (16ll * a.blocks)) + piece);
+    const unsigned byte = __ldg(a.scales_in + row * a.pitch + (piece >> 1));
+    const float s = micro_scale(byte);
+    unsigned w[(int)sizeof(T) / 2][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float2 t = micro_pair(((k < 4 ? c.x : c.y) >> (8 * (k & 3))) & 255u);
+        const float x = t.x * s, y = t.y * s;
+        if constexpr (sizeof(T) == 4) {
+            w[k / 4][2 * k % 8] = __float_as_uint(x);
+            w[k / 4][2 * k % 8 + 1] = __float_as_uint(y);
+        } else if constexpr (std::is_same_v<T, __half>) {
+            const __half2 h = __floats2half2_rn(x, y);
+            w[0][k] = *reinterpret_cast<const unsigned *>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+            w[0][k] = *reinterpret_cast<const unsigned *>(&h);
+        }
+    }
+    T *o = static_cast<T *>(a.out) + row * a.stride + piece * 16;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) store32(reinterpret_cast<char *>(o) + 32 * i, w[i]);
+}
+
+// whether rows allow 32-byte accesses of 16 elements
+inline bool fits_sixteen(const void *p, long long stride, int width, int size) {
+    return width % 16 == 0 && stride * size % 32 == 0 && reinterpret_cast<uintptr_t>(p) % 32 == 0;
+}
+
 // runs f(args) over launches whose piece numbers stay below 2^31
 template <class F>
-int micro_launches(MicroArgs &a, long long rows, int width, F f) {
+int micro_launches(MicroArgs &a, long long rows, int width, int per_block, F f) {
     a.width = width;
     a.blocks = (width + 31) / 32;
     a.pitch = 4 * ((a.blocks + 3) / 4);
-    const unsigned ppr = 4u * (unsigned)a.blocks;
+    const unsigned ppr = (unsigned)per_block * (unsigned)a.blocks;  // pieces per block and row
     a.ppr = FastDiv(ppr);
     const long long per_launch = std::max<long long>(1, (1ll << 30) / ppr);
     for (a.first = 0; a.first < rows; a.first += per_launch) {
@@ -154,12 +284,13 @@ int flare_micro_quantize(const void *x, int type, long long rows, int width, lon
     a.codes = codes;
     a.scales = scales;
     a.stride = stride;
-    const bool vec = width % 8 == 0 && fits_vec(x, stride, type_size(type), 8);
+    const bool vec = width % 8 == 0 && fits_vec(x, stride, type_size(type), 8), wide = fits_sixteen(x, stride, width, type_size(type));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        return micro_launches(a, rows, width, [&](unsigned blocks) {
-            if (vec) micro_quantize_kernel<T, true><<<blocks, MQ_THREADS, 0, st>>>(a);
+        return micro_launches(a, rows, width, wide ? 2 : 4, [&](unsigned blocks) {
+            if (wide) micro_quantize16_kernel<T><<<blocks, MQ_THREADS, 0, st>>>(a);
+            else if (vec) micro_quantize_kernel<T, true><<<blocks, MQ_THREADS, 0, st>>>(a);
             else micro_quantize_kernel<T, false><<<blocks, MQ_THREADS, 0, st>>>(a);
         });
     });
@@ -181,12 +312,13 @@ int flare_micro_dequantize(const unsigned char *codes, const unsigned char *scal
     a.codes_in = codes;
     a.scales_in = scales;
     a.stride = stride;
-    const bool vec = width % 8 == 0 && fits_vec(out, stride, type_size(type), 8);
+    const bool vec = width % 8 == 0 && fits_vec(out, stride, type_size(type), 8), wide = fits_sixteen(out, stride, width, type_size(type));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        return micro_launches(a, rows, width, [&](unsigned blocks) {
-            if (vec) micro_dequantize_kernel<T, true><<<blocks, MQ_THREADS, 0, st>>>(a);
+        return micro_launches(a, rows, width, wide ? 2 : 4, [&](unsigned blocks) {
+            if (wide) micro_dequantize16_kernel<T><<<blocks, MQ_THREADS, 0, st>>>(a);
+            else if (vec) micro_dequantize_kernel<T, true><<<blocks, MQ_THREADS, 0, st>>>(a);
             else micro_dequantize_kernel<T, false><<<blocks, MQ_THREADS, 0, st>>>(a);
         });
     });

@@ -19,7 +19,7 @@ def _same(got, want):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,width,pad", [(1, 1, 0), (3, 31, 0), (5, 32, 0), (7, 33, 0), (100, 96, 0), (9, 129, 0), (4, 1000, 0), (6, 96, 8),
-                                            (6, 40, 3)])
+                                            (6, 40, 3), (5, 16, 0), (5, 48, 0), (9, 80, 16), (3, 1008, 0)])
 @pytest.mark.parametrize("x", [F32, F16, BF16])
 def test_quantize(rows, width, pad, x):
     g = torch.Generator().manual_seed(width)
