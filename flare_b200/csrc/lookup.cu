@@ -429,6 +429,7 @@ struct GradArgs {
     long long rows, dout_stride, table_stride;
     unsigned n, range, ranges, work_blocks;  // entries per range; blocks on entries, before those on rows without any
     int width, tiles, pieces, index_type;  // column tiles, 16-byte pieces of dout's row in one
+    int empty_rows;
     float scale;
 };
 
@@ -488,15 +489,15 @@ struct RowSum {
     }
 };
 
-// 128 rows a warp: zeros in those that no entry names
+// a.empty_rows (at most 128) rows a warp: zeros in those that no entry names
 __device__ __forceinline__ void grad_empty(const GradArgs &a, unsigned block, unsigned *words) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const long long row0 = ((long long)block * (blockDim.x >> 5) + w) * 128;
+    const long long row0 = ((long long)block * (blockDim.x >> 5) + w) * a.empty_rows, row1 = min(row0 + a.empty_rows, a.rows);
     if (row0 >= a.rows) return;
     // the entries of the warp's rows: both borders at once, 16 probes a step for each
     unsigned lo = 0, len = a.n;
     {
-        const unsigned v = (unsigned)min(row0 + (lane < 16 ? 0 : 128), a.rows);
+        const unsigned v = (unsigned)(lane < 16 ? row0 : row1);
         const int p = lane & 15;
         while (__any_sync(0xffffffffu, len != 0)) {
             const unsigned at = lo + (unsigned)((unsigned long long)len * (p + 1) / 17);
@@ -521,25 +522,39 @@ __device__ __forceinline__ void grad_empty(const GradArgs &a, unsigned block, un
         }
     } else {  // few rows, many entries: look each row up
         for (int k = 0; k < 4; ++k) {
-            const unsigned r = (unsigned)min(row0 + 32 * k + lane, a.rows);
+            const unsigned r = (unsigned)min(row0 + 32 * k + lane, row1);
             const unsigned at = s + lower_bound(a.key + s, e - s, r);
             const unsigned m = __ballot_sync(0xffffffffu, at < e && __ldg(a.key + at) == r);
             if (lane == 0) named[k] = m;
         }
     }
     __syncwarp();
-    const bool four = a.width % 4 == 0 && (reinterpret_cast<uintptr_t>(a.dtable) & 15) == 0;
     for (int k = 0; k < 4; ++k) {
-        const long long left = a.rows - row0 - 32 * k;
+        const long long left = row1 - row0 - 32 * k;
         unsigned empty = left <= 0 ? 0u : ~named[k] & (left >= 32 ? 0xffffffffu : (1u << left) - 1u);
-        for (; empty; empty &= empty - 1) {
-            float *p = a.dtable + (row0 + 32 * k + __ffs(empty) - 1) * a.width;
-            if (four)
-                for (int c = lane * 4; c < a.width; c += 128) __stcs(reinterpret_cast<float4 *>(p + c), make_float4(0, 0, 0, 0));
-            else
-                for (int c = lane; c < a.width; c += 32) __stcs(p + c, 0.0f);
+        while (empty) {
+            // a run of empty rows is one stretch of memory: 16 bytes at a time between its unaligned ends
+            const int first = __ffs(empty) - 1;
+            const unsigned after = ~(empty >> first);
+            const int run = min(after ? __ffs(after) - 1 : 32, 32 - first);
+            empty &= run + first >= 32 ? (1u << first) - 1u : ~(((1u << run) - 1u) << first);
+            float *p = a.dtable + (row0 + 32 * k + first) * a.width;
+            const long long n = (long long)run * a.width;
+            const int head = (int)min(n, (long long)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / 4);
+            const long long body = (n - head) / 4;
+            if (lane < head) p[lane] = 0.0f;
+            float4 *q = reinterpret_cast<float4 *>(p + head);
+            for (long long c = lane; c < body; c += 32) __stcs(q + c, make_float4(0, 0, 0, 0));
+            if (lane < n - head - 4 * body) p[head + 4 * body + lane] = 0.0f;
         }
     }
+}
+
+// rows per warp there: 128 share a search, fewer where that leaves the machine without warps
+inline int empty_rows(long long rows) {
+    int r = 128;
+    while (r > 8 && rows / r < 24ll * SMS) r /= 2;
+    return r;
 }
 
 __device__ __forceinline__ unsigned shared_addr(const void *p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
@@ -951,7 +966,8 @@ int launch_ring(GradArgs a, cudaStream_t st) {
     a.pieces = std::min(G, a.width / Piece::VE);
     a.tiles = (a.width + G * Piece::VE - 1) / (G * Piece::VE);
     a.work_blocks = (unsigned)(((long long)a.ranges * a.tiles + GROUPS - 1) / GROUPS);
-    const unsigned empty_blocks = (unsigned)((a.rows + 128 * RING_WARPS - 1) / (128 * RING_WARPS));
+    a.empty_rows = empty_rows(a.rows);
+    const unsigned empty_blocks = (unsigned)((a.rows + a.empty_rows * RING_WARPS - 1) / (a.empty_rows * RING_WARPS));
     auto fn = grad_ring_kernel<D, T, G, DOT>;
     const int e = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_lookup_backward");
     if (e) return e;
@@ -973,7 +989,8 @@ void launch_plain(GradArgs a, cudaStream_t st) {
     a.tiles = (a.width + G * VE * NQ - 1) / (G * VE * NQ);
     const unsigned per_block = LG_THREADS / G;
     a.work_blocks = (unsigned)(((long long)a.ranges * a.tiles + per_block - 1) / per_block);
-    const unsigned empty_blocks = (unsigned)((a.rows + 128 * LG_WARPS - 1) / (128 * LG_WARPS));
+    a.empty_rows = empty_rows(a.rows);
+    const unsigned empty_blocks = (unsigned)((a.rows + a.empty_rows * LG_WARPS - 1) / (a.empty_rows * LG_WARPS));
     grad_plain_kernel<D, VE, NQ, G><<<a.work_blocks + empty_blocks, LG_THREADS, 0, st>>>(a);
     launch_join<VE>(a, st);
 }

@@ -14,12 +14,14 @@
 // before every span (1/16 of a float per element), not read from rounded outputs.
 // Bound by memory: gate, x (dh) in, h (dx, dgate) out.  State, products and sums are 32-bit floats.
 #include <algorithm>
+#include <cstdlib>
 
 #include "ops.cuh"
 
 namespace flare {
 
 constexpr int SPAN = FLARE_RECURRENCE_SPAN;
+static_assert(SPAN == 16, "shifts by 4");
 constexpr int WARPS = 8;         // warps per block: W along time times WARPS / W tiles of channels
 constexpr int MAX_SPLITS = 128;  // blocks along time
 constexpr int SUM_STRIDE = 33;   // row stride of a warp's 16 x 32 products, off the banks' 32
@@ -32,14 +34,16 @@ struct RecArgs {
     float *agg;      // (splits, 2, seqs * width)
     float *partial;  // (parts, rows, groups): sums over parts of a group's channels
     long long seqs, rows;
-    long long gate_s, gate_t, x_s, x_t, h_s, h_t, dh_s, dh_t, dgate_s, dgate_t, dx_s, dx_t;
+    long long gate_s, x_s, h_s, dh_s, dgate_s, dx_s;   // elements
+    int gate_t, x_t, h_t, dh_t, dgate_t, dx_t;         // elements; less than 2^31 bytes
     int steps, width, groups;
     FastDiv share;             // channels per gate
     int off64, reverse, packed;
-    int warps, splits, per;    // W; dense: steps per split
+    int wlog, splits, per;     // log2 W; dense: steps per split
     unsigned tiles, units;     // units: lanes' worth of channels, seqs * width / VE
     FastDiv upr;               // units per sequence
     int group_units, groups_per_tile, parts;  // backward tiles of whole groups, see Place
+    FastDiv gunits, fparts;    // by group_units and parts
     int spans;                 // dense: spans per sequence
 };
 
@@ -56,43 +60,44 @@ struct Place {
     int seq, row0, len;  // row0: the sequence's first row (packed), len: its steps
     int c;               // first channel
     unsigned chain;      // seq * width + c
-    int part, leader;    // GROUPED: part of the group, lane of the group's first channel in this warp
+    int part;            // GROUPED: part of the group
+    // lanes without channels of their own (!active) walk along with another's and store nothing
     __device__ __forceinline__ Place(const RecArgs &a, unsigned tile) {
         const int lane = threadIdx.x & 31;
         unsigned u;
         part = 0;
-        leader = 0;
         if (!GROUPED) {
             u = tile * 32 + lane;
-            active = tile < a.tiles && u < a.units;
+            active = u < a.units;
         } else if (a.parts == 1) {
-            const unsigned g = lane / a.group_units;
-            leader = g * a.group_units;
-            u = (tile * a.groups_per_tile + g) * a.group_units + lane - leader;
-            active = tile < a.tiles && (int)g < a.groups_per_tile && u < a.units;
+            const unsigned g = a.gunits.div(lane);
+            u = (tile * a.groups_per_tile + g) * a.group_units + lane - g * a.group_units;
+            active = (int)g < a.groups_per_tile && u < a.units;
+            if ((int)g >= a.groups_per_tile) u = (tile * a.groups_per_tile + g) * a.group_units - 1;
         } else {
-            part = tile % a.parts;
+            const unsigned t = a.fparts.div(tile);
+            part = tile - t * a.parts;
             const int pos = part * 32 + lane;
-            u = tile / a.parts * a.group_units + pos;
-            active = tile < a.tiles && pos < a.group_units;
+            u = t * a.group_units + min(pos, a.group_units - 1);
+            active = pos < a.group_units;
         }
-        if (!active) u = 0;
+        const bool some = tile < a.tiles;
+        active = active && some;
+        u = some ? min(u, a.units - 1) : 0u;
         seq = (int)a.upr.div(u);
         c = (int)(u - seq * a.upr.d) * VE;
         chain = u * VE;
         row0 = 0;
-        len = a.steps;
-        if (!active) {
-            len = 0;
-        } else if (a.packed) {
+        len = some ? a.steps : 0;
+        if (a.packed && some) {
             row0 = offset_at(a, seq);
             len = max(offset_at(a, seq + 1) - row0, 0);
         }
     }
     // element offset of the first step's row in a tensor (the next step's is stride_t further on, or before if reversed)
-    __device__ __forceinline__ long long first(const RecArgs &a, long long stride_s, long long stride_t) const {
-        const long long base = a.packed ? row0 * stride_t : seq * stride_s;
-        return a.reverse ? base + (len - 1) * stride_t : base;
+    __device__ __forceinline__ long long first(const RecArgs &a, long long stride_s, int stride_t) const {
+        const long long base = a.packed ? (long long)row0 * stride_t : seq * stride_s;
+        return a.reverse ? base + (long long)(len - 1) * stride_t : base;
     }
     // row of `saved` that holds the state before span k >= 1
     __device__ __forceinline__ long long saved_row(const RecArgs &a, int k) const {
@@ -105,7 +110,7 @@ struct Place {
         if (a.splits > 1) {
             unsigned per = a.per;
             if (a.packed) {
-                const unsigned round = a.warps * SPAN, rounds = ((unsigned)len + round - 1) / round;
+                const unsigned round = SPAN << a.wlog, rounds = ((unsigned)len + round - 1) / round;
                 per = (rounds + a.splits - 1) / a.splits * round;
             }
             t0 = (int)min((long long)len, (long long)split * per);
@@ -118,20 +123,22 @@ struct Place {
 // has left the range of a float.
 __device__ __forceinline__ float through(float A, float H, float c) { return c == 0.0f ? H : fmaf(A, c, H); }
 
-// SPAN steps of N channels as they lie in memory, the ones past n filled with `rest`.
+// SPAN steps of N channels as they lie in memory, `step` elements apart.
 template <class T, int N>
 struct Span {
     Vec<T, N> d[SPAN];
-    // KEEP: others read it again soon
-    template <bool KEEP>
-    __device__ __forceinline__ void load(const T *p, long long step, int n, float rest) {
+    // FULL: all steps are there, else the ones past n are filled with `rest`.  KEEP: others read it again soon
+    template <bool FULL, bool KEEP>
+    __device__ __forceinline__ void load(const T *p, int step, int n, float rest) {
+        const int bytes = step * (int)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < SPAN; ++i, p += step) {
-            if (i < n && KEEP) d[i].load(p);
-            else if (i < n) d[i].load_stream(p);
-            else
+        for (int i = 0; i < SPAN; ++i) {
+            const T *at = reinterpret_cast<const T *>(reinterpret_cast<const char *>(p) + (long long)bytes * i);
+            if (!FULL && i >= n)
 #pragma unroll
                 for (int v = 0; v < N; ++v) d[i].set(v, rest);
+            else if (KEEP) d[i].load(at);
+            else d[i].load_stream(at);
         }
     }
     __device__ __forceinline__ float at(int i, int v) const { return d[i].get(N == 1 ? 0 : v); }
@@ -140,6 +147,8 @@ struct Span {
         if constexpr (N * sizeof(T) == 2) asm volatile("" : "+h"(d[i].raw[0]));
         else if constexpr (N * sizeof(T) == 4) asm volatile("" : "+r"(d[i].raw[0]));
         else if constexpr (N * sizeof(T) == 8) asm volatile("" : "+r"(d[i].raw[0].x), "+r"(d[i].raw[0].y));
+        else if constexpr (N * sizeof(T) == 16)
+            asm volatile("" : "+r"(d[i].raw[0].x), "+r"(d[i].raw[0].y), "+r"(d[i].raw[0].z), "+r"(d[i].raw[0].w));
     }
 };
 
@@ -164,23 +173,23 @@ __device__ __forceinline__ void stretch(const Span<GT, GN> &g, const Span<T, VE>
 }
 
 // barrier of the W warps that share a tile
-__device__ __forceinline__ void tile_sync(int W) {
-    const int id = 1 + (threadIdx.x >> 5) / W;
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 * W) : "memory");
+__device__ __forceinline__ void tile_sync(int wlog) {
+    const int id = 1 + (threadIdx.x >> (5 + wlog));
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 << wlog) : "memory");
 }
 
 // The state that enters warp w's stretch, from the state `carry` that enters all W of them; carry becomes what leaves them.
 // BACK: warps are passed from the last to the first.  buf: (2, W, 32 VE) floats, not the one of the call before.
 template <bool BACK, int VE>
-__device__ __forceinline__ void exchange(float *buf, int W, const float (&A)[VE], const float (&H)[VE], float (&carry)[VE], float (&in)[VE]) {
-    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1);
+__device__ __forceinline__ void exchange(float *buf, int wlog, const float (&A)[VE], const float (&H)[VE], float (&carry)[VE], float (&in)[VE]) {
+    const int W = 1 << wlog, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1);
     float *sa = buf, *sh = buf + W * 32 * VE;
 #pragma unroll
     for (int v = 0; v < VE; ++v) {
         sa[(w * VE + v) * 32 + lane] = A[v];
         sh[(w * VE + v) * 32 + lane] = H[v];
     }
-    tile_sync(W);
+    tile_sync(wlog);
 #pragma unroll
     for (int v = 0; v < VE; ++v) in[v] = carry[v];
 #pragma unroll 4
@@ -199,7 +208,7 @@ __device__ __forceinline__ void exchange(float *buf, int W, const float (&A)[VE]
 template <bool BACK, int VE>
 __device__ __forceinline__ void fold_splits(const RecArgs &a, unsigned chain, int split, float *buf, float (&c)[VE]) {
     const long long chains = a.seqs * a.width;
-    const int W = a.warps, w = (threadIdx.x >> 5) & (W - 1);
+    const int W = 1 << a.wlog, w = (threadIdx.x >> 5) & (W - 1);
     const int n = BACK ? a.splits - 1 - split : split;
     if (n == 0) return;
     // parts in the order of the walk: warp w (BACK: W - 1 - w) has the w-th
@@ -223,8 +232,8 @@ __device__ __forceinline__ void fold_splits(const RecArgs &a, unsigned chain, in
         }
     }
     if (W > 1) {
-        exchange<BACK>(buf, W, A, H, c, unused);
-        tile_sync(W);  // the rounds that follow use the buffer again
+        exchange<BACK>(buf, a.wlog, A, H, c, unused);
+        tile_sync(a.wlog);  // the rounds that follow use the buffer again
     } else {
 #pragma unroll
         for (int v = 0; v < VE; ++v) c[v] = through(A[v], H[v], c[v]);
@@ -260,12 +269,12 @@ __device__ __forceinline__ void clear_rest(const RecArgs &a, void *out, long lon
 }
 
 __device__ __forceinline__ unsigned my_tile(const RecArgs &a) {
-    return blockIdx.x * (WARPS / a.warps) + (threadIdx.x >> 5) / a.warps;
+    return blockIdx.x * (WARPS >> a.wlog) + (threadIdx.x >> (5 + a.wlog));
 }
 // a tile's part of the exchange buffers: two of (2, W, 32 VE) floats
 template <int VE>
 __device__ __forceinline__ float *my_buffers(const RecArgs &a, float *smem) {
-    return smem + (threadIdx.x >> 5) / a.warps * (4 * a.warps * 32 * VE);
+    return smem + ((threadIdx.x >> (5 + a.wlog)) << a.wlog) * (4 * 32 * VE);
 }
 __device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(0xffffffffu, v); }
 
@@ -273,15 +282,15 @@ __device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(0xffff
 template <bool BACK, class T, class GT, int VE, bool SHARED>
 __global__ void __launch_bounds__(32 * WARPS) recurrence_split_kernel(const RecArgs a) {
     extern __shared__ __align__(16) float smem[];
-    const int W = a.warps, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
+    const int W = 1 << a.wlog, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
     const Place<VE, false> me(a, my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
     float *bufs = my_buffers<VE>(a, smem);
-    const int round = W * SPAN, n = (warp_max(t1 - t0) + round - 1) / round;
+    const int round = SPAN << a.wlog, n = (warp_max(t1 - t0) + round - 1) >> (4 + a.wlog);
     const T *src = static_cast<const T *>(BACK ? a.dh : a.x);
-    const long long src_t = BACK ? a.dh_t : a.x_t;
-    const long long gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -src_t : src_t;
+    const int src_t = BACK ? a.dh_t : a.x_t;
+    const int gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -src_t : src_t;
     const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + a.share.div(me.c);
     const T *xp = src + me.first(a, BACK ? a.dh_s : a.x_s, src_t) + me.c;
     float A[VE], H[VE], tA[VE], tH[VE], unused[VE];
@@ -294,11 +303,16 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_split_kernel(const RecA
         const int t = t0 + (BACK ? n - 1 - k : k) * round + w * SPAN, left = t1 - t;
         Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x;
-        g.template load<true>(gp + t * gs, gs, left, 1.0f);
-        x.template load<true>(xp + t * xs, xs, src ? left : 0, 0.0f);
+        if (__all_sync(0xffffffffu, left >= SPAN) && src) {
+            g.template load<true, true>(gp + (long long)t * gs, gs, 0, 1.0f);
+            x.template load<true, true>(xp + (long long)t * xs, xs, 0, 0.0f);
+        } else {
+            g.template load<false, true>(gp + (long long)t * gs, gs, left, 1.0f);
+            x.template load<false, true>(xp + (long long)t * xs, xs, src ? left : 0, 0.0f);
+        }
         stretch<BACK>(g, x, A, H);
         float *buf = bufs + (k & 1) * 2 * W * 32 * VE;
-        exchange<BACK>(buf, W, A, H, tH, unused);
+        exchange<BACK>(buf, a.wlog, A, H, tH, unused);
         // the product of the round's gates, in the same buffer
         for (int o = 0; o < W; ++o)
 #pragma unroll
@@ -315,54 +329,64 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_split_kernel(const RecA
 template <class T, class GT, int VE, bool SHARED>
 __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const RecArgs a) {
     extern __shared__ __align__(16) float smem[];
-    const int W = a.warps, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
+    const int W = 1 << a.wlog, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
     const Place<VE, false> me(a, my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
     float *bufs = my_buffers<VE>(a, smem);
-    const int round = W * SPAN, n = (warp_max(t1 - t0) + round - 1) / round;
-    const long long gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t, hs = a.reverse ? -a.h_t : a.h_t;
+    const int round = SPAN << a.wlog, n = (warp_max(t1 - t0) + round - 1) >> (4 + a.wlog);
+    const int gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t, hs = a.reverse ? -a.h_t : a.h_t;
     const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + a.share.div(me.c);
     const T *xp = static_cast<const T *>(a.x) + me.first(a, a.x_s, a.x_t) + me.c;
     T *hp = static_cast<T *>(a.h) + me.first(a, a.h_s, a.h_t) + me.c;
     float carry[VE], h[VE], A[VE], H[VE];
     load_ends<VE>(a.state, me.chain, me.active, carry);
     if (a.splits > 1) fold_splits<false, VE>(a, me.chain, split, bufs, carry);
-    for (int k = 0; k < n; ++k) {
-        const int t = t0 + k * round + w * SPAN, left = t1 - t;
+    // a span of which every lane has all steps needs no tests
+    auto span = [&](auto full, int k, int t, int left) {
+        constexpr bool FULL = decltype(full)::value;
         Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x;
-        g.template load<SHARED>(gp + t * gs, gs, left, 1.0f);
-        x.template load<false>(xp + t * xs, xs, left, 0.0f);
+        g.template load<FULL, SHARED>(gp + (long long)t * gs, gs, left, 1.0f);
+        x.template load<FULL, false>(xp + (long long)t * xs, xs, left, 0.0f);
         if (W > 1) {
             stretch<false>(g, x, A, H);
-            exchange<false>(bufs + (k & 1) * 2 * W * 32 * VE, W, A, H, carry, h);
+            exchange<false>(bufs + (k & 1) * 2 * W * 32 * VE, a.wlog, A, H, carry, h);
         } else {
 #pragma unroll
             for (int v = 0; v < VE; ++v) h[v] = carry[v];
         }
-        if (a.saved && left > 0 && t > 0) store_ends<VE>(a.saved + me.saved_row(a, t / SPAN) * a.width + me.c, h);
+        if (a.saved && me.active && left > 0 && t > 0) store_ends<VE>(a.saved + me.saved_row(a, t / SPAN) * a.width + me.c, h);
         if (a.h) {
-            T *p = hp + t * hs;
+            const int bytes = hs * (int)sizeof(T);
+            char *p = reinterpret_cast<char *>(hp + (long long)t * hs);
 #pragma unroll
-            for (int i = 0; i < SPAN; ++i, p += hs) {
+            for (int i = 0; i < SPAN; ++i) {
                 Vec<T, VE> o;
+                x.hold(i);
 #pragma unroll
                 for (int v = 0; v < VE; ++v) {
                     h[v] = fmaf(g.at(i, v), h[v], x.at(i, v));
                     o.set(v, h[v]);
                 }
-                if (i < left) o.store_stream(p);
+                if (me.active && (FULL || i < left)) o.store_stream(reinterpret_cast<T *>(p + (long long)bytes * i));
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < SPAN; ++i)
+            for (int i = 0; i < SPAN; ++i) {
+                x.hold(i);
 #pragma unroll
                 for (int v = 0; v < VE; ++v) h[v] = fmaf(g.at(i, v), h[v], x.at(i, v));
+            }
         }
         if (W == 1)
 #pragma unroll
             for (int v = 0; v < VE; ++v) carry[v] = h[v];
+    };
+    for (int k = 0; k < n; ++k) {
+        const int t = t0 + k * round + w * SPAN, left = t1 - t;
+        if (__all_sync(0xffffffffu, left >= SPAN)) span(std::true_type{}, k, t, left);
+        else span(std::false_type{}, k, t, left);
     }
     if (w == 0 && split == a.splits - 1 && me.active) store_ends<VE>(a.last + me.chain, carry);
     if (a.packed && a.h) clear_rest<T>(a, a.h, a.h_t, a.width);
@@ -373,16 +397,16 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const Re
 template <class T, class GT, int VE, bool SHARED, bool DH>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(const RecArgs a) {
     extern __shared__ __align__(16) float smem[];
-    const int W = a.warps, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
+    const int W = 1 << a.wlog, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
     const Place<VE, SHARED> me(a, my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
     float *bufs = my_buffers<VE>(a, smem);
     float *sums = smem + (W > 1 ? 4 * WARPS * 32 * VE : 0) + (threadIdx.x >> 5) * (SPAN * SUM_STRIDE);
-    const int round = W * SPAN, n = (warp_max(t1 - t0) + round - 1) / round;
+    const int round = SPAN << a.wlog, n = (warp_max(t1 - t0) + round - 1) >> (4 + a.wlog);
     const int gc = (int)a.share.div(me.c);
-    const long long gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t;
-    const long long dhs = a.reverse ? -a.dh_t : a.dh_t, dxs = a.reverse ? -a.dx_t : a.dx_t, dgs = a.reverse ? -a.dgate_t : a.dgate_t;
+    const int gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t;
+    const int dhs = a.reverse ? -a.dh_t : a.dh_t, dxs = a.reverse ? -a.dx_t : a.dx_t, dgs = a.reverse ? -a.dgate_t : a.dgate_t;
     const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + gc;
     const T *xp = static_cast<const T *>(a.x) + me.first(a, a.x_s, a.x_t) + me.c;
     const T *dhp = DH ? static_cast<const T *>(a.dh) + me.first(a, a.dh_s, a.dh_t) + me.c : nullptr;
@@ -391,20 +415,20 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
     float carry[VE], mu[VE], A[VE], H[VE];
     load_ends<VE>(a.dlast, me.chain, me.active, carry);
     if (a.splits > 1) fold_splits<true, VE>(a, me.chain, split, bufs, carry);
-    for (int k = 0; k < n; ++k) {
-        const int t = t0 + (n - 1 - k) * round + w * SPAN, left = t1 - t;
+    auto span = [&](auto full, int k, int t, int left) {
+        constexpr bool FULL = decltype(full)::value;
         Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x, dh;
-        g.template load<SHARED>(gp + t * gs, gs, left, 1.0f);
-        if (DH) dh.template load<false>(dhp + t * dhs, dhs, left, 0.0f);
-        x.template load<false>(xp + t * xs, xs, left, 0.0f);
+        g.template load<FULL, SHARED>(gp + (long long)t * gs, gs, left, 1.0f);
+        if (DH) dh.template load<FULL, false>(dhp + (long long)t * dhs, dhs, left, 0.0f);
+        x.template load<FULL, false>(xp + (long long)t * xs, xs, left, 0.0f);
         float before[SPAN][VE];  // the state before each step
         if (t > 0) load_ends<VE>(a.saved + me.saved_row(a, t / SPAN) * a.width, me.c, left > 0, before[0]);
         else load_ends<VE>(a.state, me.chain, left > 0, before[0]);
         if (W > 1) {
-            if (!DH) dh.template load<false>(nullptr, 0, 0, 0.0f);
+            if (!DH) dh.template load<false, false>(nullptr, 0, 0, 0.0f);
             stretch<true>(g, dh, A, H);
-            exchange<true>(bufs + (k & 1) * 2 * W * 32 * VE, W, A, H, carry, mu);
+            exchange<true>(bufs + (k & 1) * 2 * W * 32 * VE, a.wlog, A, H, carry, mu);
         } else {
 #pragma unroll
             for (int v = 0; v < VE; ++v) mu[v] = carry[v];
@@ -415,10 +439,10 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
 #pragma unroll
             for (int v = 0; v < VE; ++v) before[i + 1][v] = fmaf(g.at(i, v), before[i][v], x.at(i, v));
         }
-        T *px = dxp + (t + SPAN - 1) * dxs;
-        GT *pg = dgp + (t + SPAN - 1) * dgs;
+        const int dxb = dxs * (int)sizeof(T), dgb = dgs * (int)sizeof(GT);
+        char *px = reinterpret_cast<char *>(dxp + (long long)t * dxs), *pg = reinterpret_cast<char *>(dgp + (long long)t * dgs);
 #pragma unroll
-        for (int i = SPAN - 1; i >= 0; --i, px -= dxs, pg -= dgs) {
+        for (int i = SPAN - 1; i >= 0; --i) {
             Vec<T, VE> o;
             Vec<GT, SHARED ? 1 : VE> og;
             float sum = 0.0f;
@@ -431,9 +455,10 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
                 else og.set(v, lambda * before[i][v]);
                 mu[v] = g.at(i, v) * lambda;
             }
-            if (i < left) o.store_stream(px);
+            const bool mine = me.active && (FULL || i < left);
+            if (mine) o.store_stream(reinterpret_cast<T *>(px + (long long)dxb * i));
             if (SHARED) sums[i * SUM_STRIDE + lane] = sum;
-            else if (i < left) og.store_stream(pg);
+            else if (mine) og.store_stream(reinterpret_cast<GT *>(pg + (long long)dgb * i));
         }
         if (SHARED) {
             // (step, group) sums over the group's lanes in this warp, in the lanes' order
@@ -443,15 +468,16 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
                 const int i = o % SPAN, from = o / SPAN * a.group_units;
                 const int src = min(from, 31);
                 // the group's place, from its first lane
-                const int oleft = __shfl_sync(0xffffffffu, left, src), oseq = __shfl_sync(0xffffffffu, me.seq, src);
+                const int oleft = __shfl_sync(0xffffffffu, me.active ? left : 0, src), oseq = __shfl_sync(0xffffffffu, me.seq, src);
                 const int orow = __shfl_sync(0xffffffffu, me.row0, src), olen = __shfl_sync(0xffffffffu, me.len, src);
                 const int ogc = __shfl_sync(0xffffffffu, gc, src), ot = __shfl_sync(0xffffffffu, t, src) + i;
                 if (o >= outs || i >= oleft) continue;
                 float sum = 0.0f;
                 for (int l = 0; l < units; ++l) sum += sums[i * SUM_STRIDE + from + l];
-                const long long at = a.reverse ? olen - 1 - ot : ot;
+                const int at = a.reverse ? olen - 1 - ot : ot;
                 if (a.parts == 1) {
-                    static_cast<GT *>(a.dgate)[(a.packed ? orow * a.dgate_t : oseq * a.dgate_s) + at * a.dgate_t + ogc] = from_f32<GT>(sum);
+                    static_cast<GT *>(a.dgate)[(a.packed ? (long long)orow * a.dgate_t : oseq * a.dgate_s) + (long long)at * a.dgate_t + ogc] =
+                        from_f32<GT>(sum);
                 } else {
                     const long long row = (a.packed ? orow : (long long)oseq * a.steps) + at;
                     a.partial[(me.part * a.rows + row) * a.groups + ogc] = sum;
@@ -462,6 +488,11 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
         if (W == 1)
 #pragma unroll
             for (int v = 0; v < VE; ++v) carry[v] = mu[v];
+    };
+    for (int k = 0; k < n; ++k) {
+        const int t = t0 + (n - 1 - k) * round + w * SPAN, left = t1 - t;
+        if (__all_sync(0xffffffffu, left >= SPAN)) span(std::true_type{}, k, t, left);
+        else span(std::false_type{}, k, t, left);
     }
     if (a.dstate && w == 0 && split == 0 && me.active) store_ends<VE>(a.dstate + me.chain, carry);
     if (a.packed) {
@@ -509,6 +540,9 @@ bool vec_fits(const flare_recurrence_args *a, int ve, bool backward) {
            (share > 1 || ok(a->dgate, a->dgate_s, a->dgate_t, gs));
 }
 
+// channels per lane: the gradient holds x, dh, 32-bit states and gates of a span in 128 registers a thread
+constexpr int widest_backward(bool f32, bool shared) { return (f32 ? 1 : 2) * (shared ? 2 : 1); }
+
 RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
     RecPlan p{};
     const int share = a->width / a->groups;
@@ -516,8 +550,9 @@ RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
     p.rows = a->offsets ? a->steps : a->seqs * a->steps;
     const long long chains = a->seqs * a->width;
     // the widest vectors that leave the machine enough warps
-    // the gradient holds x, dh, 32-bit states and gates of a span in 128 registers a thread
-    const int widest = !backward ? 4 : (a->x_type == FLARE_F32 ? 1 : 2) * (p.shared ? 2 : 1);
+    // forward 16 bytes a lane where gates take no more than a register a step (160k x 16 x 96 f16: 90 us, with 8 bytes 125 us)
+    const bool f32 = a->x_type == FLARE_F32;
+    const int widest = backward ? widest_backward(f32, p.shared) : p.shared && !f32 ? 8 : 4;
     p.ve = widest;
     while (p.ve > 1 && (!vec_fits(a, p.ve, backward) || chains / p.ve < 32ll * 8 * SMS)) p.ve >>= 1;
     while (p.ve < 2 && a->x_type != FLARE_F32 && vec_fits(a, 2 * p.ve, backward)) p.ve *= 2;  // 4 bytes a lane at least
@@ -562,16 +597,19 @@ RecArgs rec_args(const flare_recurrence_args *in, const RecPlan &p) {
     a.agg = static_cast<float *>(in->workspace);
     a.partial = reinterpret_cast<float *>(static_cast<char *>(in->workspace) + p.agg_bytes);
     a.seqs = in->seqs, a.steps = (int)in->steps, a.rows = p.rows;
-    a.gate_s = in->gate_s, a.gate_t = in->gate_t, a.x_s = in->x_s, a.x_t = in->x_t, a.h_s = in->h_s, a.h_t = in->h_t;
-    a.dh_s = in->dh_s, a.dh_t = in->dh_t, a.dgate_s = in->dgate_s, a.dgate_t = in->dgate_t, a.dx_s = in->dx_s, a.dx_t = in->dx_t;
+    a.gate_s = in->gate_s, a.x_s = in->x_s, a.h_s = in->h_s, a.dh_s = in->dh_s, a.dgate_s = in->dgate_s, a.dx_s = in->dx_s;
+    a.gate_t = (int)in->gate_t, a.x_t = (int)in->x_t, a.h_t = (int)in->h_t;
+    a.dh_t = (int)in->dh_t, a.dgate_t = (int)in->dgate_t, a.dx_t = (int)in->dx_t;
     a.width = in->width, a.groups = in->groups, a.share = FastDiv((unsigned)(in->width / in->groups));
     a.off64 = in->offsets_type == FLARE_I64, a.reverse = in->reverse != 0, a.packed = in->offsets != nullptr;
-    a.warps = p.warps, a.splits = p.splits, a.tiles = (unsigned)p.tiles;
+    while ((1 << a.wlog) < p.warps) ++a.wlog;
+    a.splits = p.splits, a.tiles = (unsigned)p.tiles;
     const long long round = (long long)p.warps * SPAN, rounds = (in->steps + round - 1) / round;
     a.per = (int)std::min<long long>((rounds + p.splits - 1) / p.splits * round, 0x7fffffff);
     a.units = (unsigned)(in->seqs * in->width / p.ve);
     a.upr = FastDiv((unsigned)(in->width / p.ve));
     a.group_units = p.group_units, a.groups_per_tile = p.groups_per_tile, a.parts = p.parts;
+    a.gunits = FastDiv((unsigned)p.group_units), a.fparts = FastDiv((unsigned)p.parts);
     a.spans = (int)((in->steps + SPAN - 1) / SPAN);
     return a;
 }
@@ -585,6 +623,8 @@ int rec_dispatch(const flare_recurrence_args *in, const RecPlan &p, F f) {
                 if (p.shared) f(t, gt, ve, std::true_type{});
                 else f(t, gt, ve, std::false_type{});
             };
+            if constexpr (!std::is_same_v<T, float>)
+                if (p.ve == 8) return f(t, gt, std::integral_constant<int, 8>{}, std::true_type{});  // shared gates, forward
             if (p.ve == 4) vec(std::integral_constant<int, 4>{});
             else if (p.ve == 2) vec(std::integral_constant<int, 2>{});
             else vec(std::integral_constant<int, 1>{});
@@ -607,24 +647,24 @@ int run_recurrence(const flare_recurrence_args *in, bool backward, cudaStream_t 
         using GT = typename decltype(gt)::type;
         constexpr int VE = decltype(ve)::value;
         constexpr bool SH = decltype(shared)::value;
-        if (p.splits > 1) {
-            // the split kernel's tiles are plain ones, whatever the main kernel's
-            RecArgs plain = a;
-            plain.tiles = (a.units + 31) / 32;
-            const dim3 sgrid((plain.tiles + at_once - 1) / at_once, (unsigned)p.splits);
-            if (backward) recurrence_split_kernel<true, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
-            else recurrence_split_kernel<false, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
-        }
+        // the split kernel's tiles are plain ones, whatever the main kernel's
+        RecArgs plain = a;
+        plain.tiles = (a.units + 31) / 32;
+        const dim3 sgrid((plain.tiles + at_once - 1) / at_once, (unsigned)p.splits);
         if (!backward) {
+            if (p.splits > 1) recurrence_split_kernel<false, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
             recurrence_forward_kernel<T, GT, VE, SH><<<grid, 32 * WARPS, buffers, st>>>(a);
             return;
         }
-        const size_t sums = SH ? sizeof(float) * WARPS * SPAN * SUM_STRIDE : 0;
-        if (a.dh) recurrence_backward_kernel<T, GT, VE, SH, true><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
-        else recurrence_backward_kernel<T, GT, VE, SH, false><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
-        if (p.parts > 1) {
-            const long long n = p.rows * in->groups;
-            recurrence_join_kernel<GT><<<(unsigned)std::min<long long>((n + 255) / 256, 16 * SMS), 256, 0, st>>>(a);
+        if constexpr (VE <= widest_backward(sizeof(T) == 4, SH)) {
+            if (p.splits > 1) recurrence_split_kernel<true, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
+            const size_t sums = SH ? sizeof(float) * WARPS * SPAN * SUM_STRIDE : 0;
+            if (a.dh) recurrence_backward_kernel<T, GT, VE, SH, true><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
+            else recurrence_backward_kernel<T, GT, VE, SH, false><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
+            if (p.parts > 1) {
+                const long long n = p.rows * in->groups;
+                recurrence_join_kernel<GT><<<(unsigned)std::min<long long>((n + 255) / 256, 16 * SMS), 256, 0, st>>>(a);
+            }
         }
     });
     OPS_LAUNCHED(backward ? "flare_recurrence_backward" : "flare_recurrence_forward");
@@ -640,6 +680,10 @@ int rec_check(const flare_recurrence_args *a, bool backward, const char *what) {
               "%s: %lld sequences of %lld steps, %d channels in %d groups", what, a->seqs, a->steps, a->width, a->groups);
     OPS_CHECK(a->seqs < 0x40000000ll && a->seqs * a->width < 0x40000000ll && a->steps < 0x40000000ll,
               "%s: %lld sequences of %lld steps, %d channels", what, a->seqs, a->steps, a->width);
+    // a tensor's steps are addressed by 32-bit distances
+    const long long gate = std::max(std::abs(a->gate_t), std::abs(a->dgate_t)) * type_size(a->gate_type);
+    const long long rest = std::max({std::abs(a->x_t), std::abs(a->h_t), std::abs(a->dh_t), std::abs(a->dx_t)}) * type_size(a->x_type);
+    OPS_CHECK(gate < 0x7fffffffll && rest < 0x7fffffffll, "%s: steps %lld bytes apart, less than 2^31 needed", what, std::max(gate, rest));
     OPS_CHECK(a->offsets_type == FLARE_I32 || a->offsets_type == FLARE_I64, "%s: unknown offsets type %d", what, a->offsets_type);
     const bool some = a->seqs > 0, data = (some || a->offsets) && a->steps > 0;
     OPS_CHECK(!data || (a->gate && a->x), "%s: NULL gate or x", what);
