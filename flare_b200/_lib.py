@@ -100,17 +100,18 @@ class RecurrenceArgs(ctypes.Structure):
 
 
 RECURRENCE_SPAN = 16
+PRODUCT_ROWS = 16
 # The operators' calls are short, so their argument structs are packed in one go: the same members as above.
 PACK_LOOKUP = struct.Struct("@5P4q4if")
 PACK_LOOKUP_GRAD = struct.Struct("@7P5q4if")
 PACK_RECURRENCE = struct.Struct("@13P15q6i")
-PACK_PRODUCT = struct.Struct("@7P4q2i")
+PACK_PRODUCT = struct.Struct("@8P5q3i")
 
 
 class ProductArgs(ctypes.Structure):
-    _fields_ = [("a_codes", vp), ("a_scales", vp), ("b_codes", vp), ("b_scales", vp), ("out", vp), ("workspace", vp),
-                ("status", vp), ("m", ll), ("n", ll), ("out_stride", ll), ("workspace_bytes", ll), ("k", ctypes.c_int),
-                ("out_type", ctypes.c_int)]
+    _fields_ = [("a_codes", vp), ("a_scales", vp), ("b_codes", vp), ("b_scales", vp), ("x", vp), ("out", vp),
+                ("workspace", vp), ("status", vp), ("m", ll), ("n", ll), ("out_stride", ll), ("x_stride", ll),
+                ("workspace_bytes", ll), ("k", ctypes.c_int), ("out_type", ctypes.c_int), ("x_type", ctypes.c_int)]
 
 
 class Stats(ctypes.Structure):

@@ -12,6 +12,8 @@
 // Warps 0-3 read a finished D from TMEM, a row per thread, round it once and store it through shared memory by TMA, while
 // the next tile goes into the other half of TMEM.  Few tiles and a long K: up to 8 blocks of a cluster take a part of K
 // each and add their tiles through distributed shared memory, in order.
+// A few rows that are not quantised yet (at most 16) are Q as they come: warps 4-7 quantise a stage of them on the way into
+// shared memory, a block of 32 elements per thread, which saves such a call a launch and a matrix.
 // Every wait is bounded; where one ran out the block's tiles are NaN and a bit of the status word is set.
 #include <cuda.h>
 
@@ -41,7 +43,51 @@ struct ProductArgs {
     int accs;                     // accumulators in TMEM
     unsigned ptiles, tiles;
     int wide;                     // scales may be read 16 bytes at a time
+    const void *x;                // Q before quantisation, else NULL
+    long long x_stride;
+    int x_vec;                    // its rows may be read 16 bytes at a time
 };
+
+constexpr int X_ROWS = FLARE_PRODUCT_ROWS;
+static_assert(X_ROWS * (KSTAGE / 32) == 128, "a block of 32 elements per thread of four warps");
+
+// 32 elements of a row, in flight
+template <class X>
+struct Raw32 {
+    Vec<X, 16 / (int)sizeof(X)> v[2 * (int)sizeof(X)];
+    // left: elements from p to the row's end
+    __device__ __forceinline__ void load(const X *p, int left, bool vec) {
+        constexpr int N = 16 / (int)sizeof(X);
+#pragma unroll
+        for (int i = 0; i < 32 / N; ++i) {
+            if (vec && left >= (i + 1) * N) {
+                v[i].load(p + i * N);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[i].el[e] = i * N + e < left ? p[i * N + e] : from_f32<X>(0.0f);
+            }
+        }
+    }
+    // its 16 bytes of codes and scale byte
+    __device__ __forceinline__ uint4 quantize(unsigned *byte) const {
+        constexpr int N = 16 / (int)sizeof(X);
+        unsigned most = 0, w[4] = {};
+#pragma unroll
+        for (int k = 0; k < 32; ++k) most = max(most, __float_as_uint(v[k / N].get(k % N)) & 0x7fffffffu);
+        *byte = 255;
+        if (most < 0x7f800000u) {
+            const int e = max((int)(most >> 23) - 127 - 2, -127);
+            *byte = (unsigned)(e + 127);
+            const float inv = __uint_as_float((unsigned)(127 - e) << 23);
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                w[k / 4] |= micro_code_pair(v[2 * k / N].get(2 * k % N) * inv, v[2 * k / N].get((2 * k + 1) % N) * inv) << (8 * (k % 4));
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <>
+struct Raw32<void> {};
 
 // D (+)= A B^T, 64 elements of K; the scales' columns in TMEM, which half of their words in idesc
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
@@ -160,7 +206,8 @@ __device__ __forceinline__ void stage_output(unsigned char *to, uint32_t tmem) {
 // stages of K per block of a cluster: an even number, as scales are read two stages at a time
 __host__ __device__ constexpr int part_of_k(int all, int S) { return S == 1 ? all : ((all + S - 1) / S + 1) / 2 * 2; }
 
-template <int BN, class O>
+// X: the type of a Q that is quantised here, or void
+template <int BN, class O, class X>
 __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap qmap,
                                                              const __grid_constant__ CUtensorMap omap, const ProductArgs a) {
     using Tile = ProductTile<BN>;
@@ -210,9 +257,9 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
                     if (round) ok = mbar_wait(&empty[st], (round - 1) & 1);
                     if (!ok) break;
                     unsigned char *t = smem + st * Tile::STAGE;
-                    arrive_expect(&full[st], Tile::CODES);
+                    arrive_expect(&full[st], std::is_void_v<X> ? Tile::CODES : PT * KBYTES);
                     tma_rows(t, &pmap, (s0 + i) * KBYTES, y, &full[st]);
-                    tma_rows(t + PT * KBYTES, &qmap, (s0 + i) * KBYTES, z, &full[st]);
+                    if constexpr (std::is_void_v<X>) tma_rows(t + PT * KBYTES, &qmap, (s0 + i) * KBYTES, z, &full[st]);
                     ++issued;
                     if (++st == a.stages) st = 0, ++round;
                 }
@@ -254,6 +301,52 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
                 }
                 mma_commit(&ready[buf]);
             }
+        }
+    } else if (warp >= 4 && !std::is_void_v<X>) {
+        if constexpr (!std::is_void_v<X>) {
+            // thread r has row r of P's scales, two words a stage, and block r mod 8 of row r / 8 of Q; one stage ahead
+            const int r = threadIdx.x - 128, qr = r >> 3, qb = r & 7;
+            unsigned w[2] = {}, w_next[2] = {};
+            Raw32<X> x, x_next;
+            auto fetch = [&](unsigned n, int i) {
+                if (n >= mine) return;
+                const long long row = tile_p(n) + r;
+                const int word = (s0 + i) * 2, e0 = (s0 + i) * KSTAGE + qb * 32;
+                w_next[0] = w_next[1] = 0;
+                if (row < a.p) {
+                    const unsigned *src = reinterpret_cast<const unsigned *>(a.ps + row * a.pitch);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int left = a.blocks - 4 * (word + h);
+                        if (left > 0) w_next[h] = __ldg(src + word + h) & (left < 4 ? (1u << (8 * left)) - 1u : 0xffffffffu);
+                    }
+                }
+                x_next.load(static_cast<const X *>(a.x) + qr * a.x_stride + e0, qr < a.q ? a.k - e0 : 0, a.x_vec);
+            };
+            if (steps) fetch(0, 0);
+            int st = 0, round = 0;
+            bool ok = true;
+            for (unsigned n = 0; n < mine && ok; ++n)
+                for (int i = 0; i < steps; ++i) {
+                    w[0] = w_next[0], w[1] = w_next[1];
+                    x = x_next;
+                    fetch(i + 1 < steps ? n : n + 1, i + 1 < steps ? i + 1 : 0);
+                    if (round) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1));
+                    if (!ok) break;
+                    unsigned char *t = smem + st * Tile::STAGE, *sc = t + Tile::CODES;
+                    const int at = (r & 31) * 16 + (r >> 5) * 4;
+                    *reinterpret_cast<unsigned *>(sc + at) = w[0];
+                    *reinterpret_cast<unsigned *>(sc + ROWS * 512 + at) = w[1];
+                    unsigned byte;
+                    const uint4 codes = x.quantize(&byte);
+                    *reinterpret_cast<uint4 *>(t + PT * KBYTES + qr * 128 + ((qb ^ (qr & 7)) << 4)) = codes;
+                    sc[((qb >> 2) * ROWS + 1) * 512 + qr * 16 + (qb & 3)] = (unsigned char)byte;
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) arrive(&full[st]);
+                    if (++st == a.stages) st = 0, ++round;
+                }
+            if (!ok && lane == 0) atomicExch(&gave_up, 1);
         }
     } else if (warp >= 4) {
         // thread r has row r of P and rows r, r + 128 of Q, 4 words (2 stages) at a time: groups (tile, pair of stages), two ahead
@@ -640,7 +733,7 @@ int matrix_map(CUtensorMap *map, CUtensorMapDataType type, int size, const void 
     return FLARE_OK;
 }
 
-template <int BN, class O>
+template <int BN, class O, class X>
 int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorMap &om, ProductArgs a, int split, cudaStream_t st) {
     using Tile = ProductTile<BN>;
     const int per = part_of_k((a.k + KSTAGE - 1) / KSTAGE, split);
@@ -657,7 +750,7 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorM
     a.stages = (int)std::min<long long>(Tile::MAX_STAGES, per * ((tiles + grid - 1) / grid));
     int smem = a.stages * Tile::STAGE + 4 * OUT_BYTES + 1024;
     if (split > 1) smem = std::max(smem, PT * BN * 4 + 1024);
-    auto fn = product_kernel<BN, O>;
+    auto fn = product_kernel<BN, O, X>;
     const int e0 = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_micro_product");
     if (e0) return e0;
     cudaLaunchConfig_t cfg{};
@@ -692,7 +785,7 @@ int launch_narrow(const CUtensorMap &om, const unsigned char *pc, const unsigned
 
 int run_product(const flare_product_args *in, cudaStream_t st) {
     ProductArgs a{};
-    a.swap = in->m < in->n;  // the larger matrix gives the tiles' 128 rows
+    a.swap = in->m < in->n || in->x;  // the larger matrix gives the tiles' 128 rows
     const unsigned char *pc = a.swap ? in->b_codes : in->a_codes, *qc = a.swap ? in->a_codes : in->b_codes;
     a.ps = a.swap ? in->b_scales : in->a_scales;
     a.qs = a.swap ? in->a_scales : in->b_scales;
@@ -701,6 +794,9 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     a.out = in->out;
     a.status = in->status;
     a.out_stride = in->out_stride;
+    a.x = in->x;
+    a.x_stride = in->x_stride;
+    a.x_vec = in->x && fits_vec(in->x, in->x_stride, type_size(in->x_type), 16 / type_size(in->x_type));
     a.k = in->k;
     a.blocks = (in->k + 31) / 32;
     a.pitch = 4 * ((a.blocks + 3) / 4);
@@ -711,7 +807,7 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     CUtensorMap pm, qm, om{};
     int e = FLARE_OK;
     // one stage of K and one tile of Q, over at least two tiles a multiprocessor
-    if (in->k <= KSTAGE && a.q <= 128 && a.p >= 2ll * SMS * PT) {
+    if (!in->x && in->k <= KSTAGE && a.q <= 128 && a.p >= 2ll * SMS * PT) {
         int bn = 16;
         while (bn < a.q) bn *= 2;
         a.bulk = !a.swap && a.vec && bn * size >= 128;
@@ -742,18 +838,20 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     // whole 128-byte pieces of output rows go by TMA
     a.bulk = !a.swap && split == 1 && a.vec && bn * size >= 128;
     e = matrix_map(&pm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pc, a.p, 16ll * a.blocks, 16ll * a.blocks, PT);
-    if (!e) e = matrix_map(&qm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, a.q, 16ll * a.blocks, 16ll * a.blocks, bn);
+    if (!e && !in->x) e = matrix_map(&qm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, a.q, 16ll * a.blocks, 16ll * a.blocks, bn);
     if (!e && a.bulk)
         e = matrix_map(&om, out_map, size, in->out, in->m, in->n, in->out_stride, 32);
     if (e) return e;
     return with_type(in->out_type, [&](auto t) {
         using O = typename decltype(t)::type;
+        if (in->x)
+            return with_type(in->x_type, [&](auto x) { return launch_product<16, O, typename decltype(x)::type>(pm, qm, om, a, split, st); });
         switch (bn) {
-            case 16: return launch_product<16, O>(pm, qm, om, a, split, st);
-            case 32: return launch_product<32, O>(pm, qm, om, a, split, st);
-            case 64: return launch_product<64, O>(pm, qm, om, a, split, st);
-            case 128: return launch_product<128, O>(pm, qm, om, a, split, st);
-            default: return launch_product<192, O>(pm, qm, om, a, split, st);
+            case 16: return launch_product<16, O, void>(pm, qm, om, a, split, st);
+            case 32: return launch_product<32, O, void>(pm, qm, om, a, split, st);
+            case 64: return launch_product<64, O, void>(pm, qm, om, a, split, st);
+            case 128: return launch_product<128, O, void>(pm, qm, om, a, split, st);
+            default: return launch_product<192, O, void>(pm, qm, om, a, split, st);
         }
     });
 }
@@ -775,7 +873,9 @@ int flare_micro_product(const flare_product_args *a, void *stream) {
     OPS_CHECK(a->m >= 0 && a->n >= 0 && a->k >= 1 && a->k <= (1 << 30), "flare_micro_product: %lld x %lld x %d", a->m, a->n, a->k);
     OPS_CHECK(a->m < 0x40000000ll && a->n < 0x40000000ll, "flare_micro_product: %lld x %lld outputs", a->m, a->n);
     if (a->m == 0 || a->n == 0) return FLARE_OK;
-    OPS_CHECK(a->a_codes && a->a_scales && a->b_codes && a->b_scales && a->out, "flare_micro_product: NULL buffer");
+    OPS_CHECK(((a->a_codes && a->a_scales) || a->x) && a->b_codes && a->b_scales && a->out, "flare_micro_product: NULL buffer");
+    OPS_CHECK(!a->x || (is_float_type(a->x_type) && a->m <= FLARE_PRODUCT_ROWS && a->x_stride >= a->k),
+              "flare_micro_product: x of type %d, %lld rows (at most %d) of stride %lld", a->x_type, a->m, FLARE_PRODUCT_ROWS, a->x_stride);
     OPS_CHECK(a->out_stride >= a->n, "flare_micro_product: output rows of stride %lld overlap", a->out_stride);
     for (const void *p : {(const void *)a->a_codes, (const void *)a->b_codes})
         OPS_CHECK(reinterpret_cast<uintptr_t>(p) % 16 == 0, "flare_micro_product: codes must be 16-byte aligned");

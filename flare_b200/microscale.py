@@ -13,6 +13,7 @@ from . import _lib, _ops
 
 BLOCK = 32  # elements that share a scale
 _FLOATS = tuple(_ops.TYPE_CODE)
+_BYTES = (torch.uint8,)
 
 
 class Micro4:
@@ -30,15 +31,17 @@ class Micro4:
         """Checks and keeps the two tensors."""
         width = int(width)
         blocks = -(-width // BLOCK)
-        _ops.need(codes, "codes", (torch.uint8,))
-        _ops.need(scales, "scales", (torch.uint8,), codes.device)
+        _ops.need(codes, "codes", _BYTES)
+        _ops.need(scales, "scales", _BYTES, codes.device)
         if width < 1 or codes.dim() != 2:
             raise ValueError(f"codes: shape {tuple(codes.shape)} for a width of {width}")
-        _ops.need_shape(codes, "codes", (codes.shape[0], 16 * blocks))
-        _ops.need_shape(scales, "scales", (codes.shape[0], -(-blocks // 4) * 4))
-        for t, name, align in ((codes, "codes", 16), (scales, "scales", 4)):
-            if not t.is_contiguous() or t.data_ptr() % align:
-                raise ValueError(f"{name}: tensor must be contiguous and aligned to {align} bytes")
+        rows = codes.shape[0]
+        _ops.need_shape(codes, "codes", (rows, 16 * blocks))
+        _ops.need_shape(scales, "scales", (rows, (blocks + 3) // 4 * 4))
+        if not codes.is_contiguous() or codes.data_ptr() % 16:
+            raise ValueError("codes: tensor must be contiguous and aligned to 16 bytes")
+        if not scales.is_contiguous() or scales.data_ptr() % 4:
+            raise ValueError("scales: tensor must be contiguous and aligned to 4 bytes")
         self.codes, self.scales, self.width = codes, scales, width
 
     @property
@@ -88,30 +91,38 @@ def quantize(x) -> Micro4:
 def product(x, w: Micro4, dtype=torch.bfloat16, check=False):
     """x (m, k) times the transpose of w (n, k): a new (m, n) tensor of f32, f16 or bf16, accumulated in 32 bits.
 
-    x: a `Micro4`, or a tensor that is quantized first.  check: wait for the product and raise FlareError if a wait
+    x: a `Micro4`, or an f32, f16 or bf16 tensor that is quantized first (up to 16 rows inside the product).  check: wait for the product and raise FlareError if a wait
     inside the kernel ran out (without it such a tile is NaN).
     """
     lib = _lib.load()
     if not isinstance(w, Micro4):
         raise ValueError(f"w: expected a Micro4, got {type(w).__name__}")
+    dev = w.codes.device
+    plain = None
     if not isinstance(x, Micro4):
-        _ops.need(x, "x", _FLOATS, w.device)
-        x = quantize(x)
+        _ops.need(x, "x", _FLOATS, dev)
+        if x.dim() != 2:
+            raise ValueError(f"x: shape {tuple(x.shape)}, expected (m, {w.width})")
+        if x.shape[0] <= _lib.PRODUCT_ROWS:
+            plain = _ops.rows(x)  # quantized on the way
+        else:
+            x = quantize(x)
     if dtype not in _ops.TYPE_CODE:
         raise ValueError(f"dtype: {dtype}, expected one of {', '.join(str(d) for d in _FLOATS)}")
-    if x.width != w.width:
-        raise ValueError(f"x has {x.width} columns, w has {w.width}")
-    if x.device != w.device:
-        raise ValueError(f"w: tensor on {w.device}, expected {x.device}")
-    (m, k), n = x.shape, w.shape[0]
-    with _ops.on(x.device):
-        out = torch.empty((m, n), dtype=dtype, device=x.device)
-        ws = _ops.workspace(lib.flare_micro_product_workspace(m, n, k), x.device)
-        status = torch.zeros(1, dtype=torch.int32, device=x.device) if check else None
-        a = _lib.PACK_PRODUCT.pack(x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
-                                   _ops.ptr(ws), _ops.ptr(status), m, n, n, 0 if ws is None else ws.numel(), k,
-                                   _ops.TYPE_CODE[dtype])
-        _lib.check(lib.flare_micro_product(a, _ops.stream(x.device)), "product")
+    (m, k), n = x.shape, w.codes.shape[0]
+    if k != w.width:
+        raise ValueError(f"x has {k} columns, w has {w.width}")
+    if x.device != dev:
+        raise ValueError(f"w: tensor on {dev}, expected {x.device}")
+    with _ops.on(dev):
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+        ws = _ops.workspace(lib.flare_micro_product_workspace(m, n, k), dev)
+        status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+        a, scales, p, stride, code = (x.codes.data_ptr(), x.scales.data_ptr(), 0, 0, 0) if plain is None else (
+            0, 0, plain.data_ptr(), plain.stride(0), _ops.TYPE_CODE[plain.dtype])
+        a = _lib.PACK_PRODUCT.pack(a, scales, w.codes.data_ptr(), w.scales.data_ptr(), p, out.data_ptr(), _ops.ptr(ws), _ops.ptr(status),
+                                   m, n, n, stride, 0 if ws is None else ws.numel(), k, _ops.TYPE_CODE[dtype], code)
+        _lib.check(lib.flare_micro_product(a, _ops.stream(dev)), "product")
     if check and int(status):
         raise _lib.FlareError(f"product: device reported error bits 0x{int(status):x} (tensor-core wait timeout)")
     return out

@@ -452,17 +452,21 @@ int flare_micro_dequantize(const unsigned char *codes, const unsigned char *scal
                            int type, long long stride, void *stream);
 
 /*
- * out (m, n) = A (m, k) B (n, k)^T of two 4-bit matrices, accumulated in 32 bits on the tensor cores.
+ * out (m, n) = A (m, k) B (n, k)^T of two 4-bit matrices, accumulated in 32 bits on the tensor cores.  A of at
+ * most FLARE_PRODUCT_ROWS rows may be given as x, of x_type and rows x_stride elements apart, instead of codes and
+ * scales: it is quantised on the way, as flare_micro_quantize does it.
  * workspace: flare_micro_product_workspace bytes, 16-byte aligned, contents irrelevant.  status (optional, a
  * device int) gets a FLARE error bit OR-ed in if a wait inside the kernel ran out; the tile concerned is NaN.
  */
+#define FLARE_PRODUCT_ROWS 16
 typedef struct flare_product_args {
     const unsigned char *a_codes, *a_scales, *b_codes, *b_scales;
+    const void *x;                /* or NULL */
     void *out;
     void *workspace;
     int *status;
-    long long m, n, out_stride, workspace_bytes;
-    int k, out_type;
+    long long m, n, out_stride, x_stride, workspace_bytes;
+    int k, out_type, x_type;
 } flare_product_args;
 long long flare_micro_product_workspace(long long m, long long n, int k);
 int flare_micro_product(const flare_product_args *a, void *stream);

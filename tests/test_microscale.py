@@ -136,6 +136,26 @@ def test_product_of_a_tensor_quantizes_it():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("x", [F32, F16, BF16])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 700, 1030), (4, 5, 33), (16, 300, 256), (16, 3, 4096), (7, 129, 250), (3, 20_011, 300), (9, 40, 31)])
+def test_product_of_a_few_rows_quantizes_them_on_the_way(m, n, k, x):
+    g = torch.Generator().manual_seed(m)
+    t = (torch.randn(m, k + 8, generator=g) * torch.exp(3 * torch.randn(m, 1, generator=g))).to(x).to(DEV)
+    w = microscale.quantize(torch.randn(n, k, generator=g).to(DEV))
+    for v in (t[:, :k], t[:, 3:k + 3], t[:, :k].contiguous()):
+        got = microscale.product(v, w, dtype=F32, check=True)
+        want = microscale.product(microscale.quantize(v), w, dtype=F32)
+        # the same codes and scales; sums over K may run in another order
+        va, vb = (ref.values(q.codes.cpu().numpy(), q.scales.cpu().numpy(), k) for q in (microscale.quantize(v), w))
+        err = (k + 2) * 2 * ref.U * (np.abs(va) @ np.abs(vb).T)
+        ref.close(got, va @ vb.T, err)
+        ref.close(got, ref.f64(want), 2 * err)
+    bad = t[:, :k].clone()
+    bad[0, k // 2] = float("inf")
+    assert torch.isnan(microscale.product(bad, w)[0]).all() and torch.isfinite(microscale.product(bad, w)[1:]).all()
+
+
+@pytest.mark.gpu
 def test_product_passes_nan_and_range():
     a, b = torch.randn(140, 96), torch.randn(33, 96)
     a[3, 40], b[7, 70] = float("nan"), float("inf")
@@ -195,7 +215,8 @@ def test_refusals_on_the_device():
     for bad in (lambda: microscale.quantize(torch.ones(4, device=DEV)), lambda: microscale.quantize(torch.ones(4, 0, device=DEV)),
                 lambda: q.dequantize(torch.float64), lambda: microscale.product(q, other), lambda: microscale.product(q, q, dtype=torch.int8),
                 lambda: microscale.Micro4(q.codes, q.scales, 65), lambda: microscale.Micro4(q.codes[:2], q.scales, 40),
-                lambda: microscale.Micro4(q.codes[:, :16], q.scales, 32), lambda: microscale.product(torch.ones(2, 39, device=DEV), q)):
+                lambda: microscale.Micro4(q.codes[:, :16], q.scales, 32), lambda: microscale.product(torch.ones(2, 39, device=DEV), q),
+                lambda: microscale.product(torch.ones(40, device=DEV), q), lambda: microscale.product(torch.ones(99, 39, device=DEV), q)):
         with pytest.raises(ValueError):
             bad()
 
@@ -211,5 +232,7 @@ def test_c_entry_refuses_bad_arguments():
     assert lib.flare_micro_product(ctypes.byref(a), None) == 1
     a = _lib.ProductArgs(m=1, n=1, k=32, out_stride=1)
     assert lib.flare_micro_product(ctypes.byref(a), None) == 1 and b"NULL" in lib.flare_last_error()
+    a = _lib.ProductArgs(m=17, n=1, k=32, out_stride=1, x=16, x_stride=32, b_codes=16, b_scales=16, out=16)
+    assert lib.flare_micro_product(ctypes.byref(a), None) == 1 and b"17 rows" in lib.flare_last_error()
     a = _lib.ProductArgs(m=1, n=1, k=32, out_stride=1, a_codes=8, b_codes=16, a_scales=16, b_scales=16, out=16)
     assert lib.flare_micro_product(ctypes.byref(a), None) == 1 and b"aligned" in lib.flare_last_error()

@@ -12,7 +12,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PAIRS = {"LookupArgs": "flare_lookup_args", "LookupGradArgs": "flare_lookup_grad_args", "RecurrenceArgs": "flare_recurrence_args",
          "ProductArgs": "flare_product_args"}
 VALUES = {"FLARE_F32": 0, "FLARE_F16": 1, "FLARE_BF16": 2, "FLARE_MICRO": _ops.MICRO, "FLARE_I32": 0, "FLARE_I64": 1,
-          "FLARE_RECURRENCE_SPAN": _lib.RECURRENCE_SPAN}
+          "FLARE_RECURRENCE_SPAN": _lib.RECURRENCE_SPAN, "FLARE_PRODUCT_ROWS": _lib.PRODUCT_ROWS}
 
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="needs a C compiler")
