@@ -125,8 +125,45 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const LookupArgs a) 
     }
 }
 
+// Rows whose elements go one or two at a time: a warp per row and 32 UNROLL VE columns of it, so that the index, the weight and
+// the addresses are worked out once and not per element (16383 rows of 1023 bf16: 48 us).
+constexpr int LK_UNROLL = 8;
+template <class T, class O, class I, int VE>
+__global__ void __launch_bounds__(LK_THREADS) lookup_wide_kernel(const LookupArgs a, const unsigned items, const FastDiv parts) {
+    const int lane = threadIdx.x & 31;
+    for (unsigned it = (blockIdx.x * LK_THREADS + threadIdx.x) >> 5; it < items; it += gridDim.x * (LK_THREADS / 32)) {
+        const unsigned r = parts.div(it), c0 = (it - r * parts.d) * (32 * LK_UNROLL) + lane;  // vectors
+        const long long i = a.first + r, p = row_of<I>(a.index, i, a.rows);
+        const float s = a.weight ? a.scale * __ldg(a.weight + i) : a.scale;
+        const T *from = static_cast<const T *>(a.table) + (p < 0 ? 0 : p) * a.table_stride;
+        O *to = static_cast<O *>(a.out) + i * a.out_stride;
+        Vec<T, VE> t[LK_UNROLL];
+        if (p >= 0)
+#pragma unroll
+            for (int k = 0; k < LK_UNROLL; ++k)
+                if (c0 + 32 * k < a.vpr.d) t[k].load(from + (c0 + 32 * k) * VE);
+#pragma unroll
+        for (int k = 0; k < LK_UNROLL; ++k)
+            if (c0 + 32 * k < a.vpr.d) {
+                Vec<O, VE> o;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) o.set(e, p < 0 ? 0.0f : t[k].get(e) * s);
+                o.store_stream(to + (c0 + 32 * k) * VE);
+            }
+    }
+}
+
 template <class T, class O, class I>
 void launch_lookup(const LookupArgs &a, int ve, cudaStream_t st) {
+    if constexpr (!std::is_void_v<T>)
+        if (ve <= 2 && a.vpr.d >= 64) {
+            const FastDiv parts((a.vpr.d + 32 * LK_UNROLL - 1) / (32 * LK_UNROLL));
+            const unsigned items = a.items / a.vpr.d * parts.d, per_block = LK_THREADS / 32;
+            const unsigned blocks = std::min((items + per_block - 1) / per_block, (unsigned)(LK_BLOCKS * SMS));
+            if (ve == 2) lookup_wide_kernel<T, O, I, 2><<<blocks, LK_THREADS, 0, st>>>(a, items, parts);
+            else lookup_wide_kernel<T, O, I, 1><<<blocks, LK_THREADS, 0, st>>>(a, items, parts);
+            return;
+        }
     const unsigned blocks = std::min((a.items + LK_THREADS - 1) / LK_THREADS, (unsigned)(LK_BLOCKS * SMS));
     switch (ve) {
         case 8: lookup_kernel<T, O, I, 8><<<blocks, LK_THREADS, 0, st>>>(a); break;
@@ -184,8 +221,8 @@ int run_lookup(const flare_lookup_args *in, cudaStream_t st) {
 // Stable radix sort of the entries by row; entries that name no row get key `rows` and end behind all others.
 // Per digit of up to 10 bits: count per tile, scan over tiles, scatter.  A tile is 4096 consecutive entries of one block;
 // warp w ranks entries [256 w, 256 w + 256) of it 32 at a time, so ranks follow the entries' order.  Lanes with equal
-// digits find one another by a ballot per bit (match.any took three times the whole kernel's time).  Up to one tile of
-// entries is sorted by one block in shared memory.
+// digits find one another by a ballot per bit (match.any took three times the whole kernel's time).  Short lists are
+// sorted by one block in shared memory.
 // ------------------------------------------------------------------------------------------------
 constexpr int RS_THREADS = 512, RS_WARPS = RS_THREADS / 32, RS_ROUNDS = 8, RS_TILE = RS_THREADS * RS_ROUNDS;
 constexpr int RS_MAX_BITS = 10, RS_BINS = 1 << RS_MAX_BITS, RS_SMALL_BITS = 8;
@@ -230,6 +267,7 @@ __global__ void __launch_bounds__(RS_THREADS) sort_count_kernel(const SortArgs a
 }
 
 // exclusive sum over the block, `total` gets the sum of all
+template <int WARPS>
 __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned *warp_sums, unsigned *total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     unsigned inc = v;
@@ -243,7 +281,7 @@ __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned *warp_s
     __syncthreads();
     unsigned before = 0, all = 0;
 #pragma unroll
-    for (int k = 0; k < RS_WARPS; ++k) {
+    for (int k = 0; k < WARPS; ++k) {
         if (k < w) before += warp_sums[k];
         all += warp_sums[k];
     }
@@ -260,7 +298,7 @@ __global__ void __launch_bounds__(RS_THREADS) sort_scan_kernel(const SortArgs a)
         const unsigned t = t0 + threadIdx.x;
         const unsigned v = t < a.tiles ? h[t] : 0u;
         unsigned all;
-        const unsigned ex = block_exclusive(v, sums, &all);
+        const unsigned ex = block_exclusive<RS_WARPS>(v, sums, &all);
         if (t < a.tiles) h[t] = carry + ex;
         carry += all;
         __syncthreads();
@@ -330,7 +368,7 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sort_scatter_kernel(const SortA
         const unsigned d = b * RS_THREADS + threadIdx.x;
         if (b * RS_THREADS >= bins) break;
         unsigned all;
-        const unsigned digit = block_exclusive(total[b], sums, &all);
+        const unsigned digit = block_exclusive<RS_WARPS>(total[b], sums, &all);
         if (d < bins) {
             at[d] = carry + digit + hist[b];
             unsigned short before = 0;
@@ -358,53 +396,86 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sort_scatter_kernel(const SortA
     }
 }
 
-// at most one tile: all digits by one block, entries in registers between passes through shared memory
-__global__ void __launch_bounds__(RS_THREADS) sort_small_kernel(const SortArgs a) {
-    constexpr unsigned BINS = 1u << RS_SMALL_BITS;
-    __shared__ uint2 entry[RS_TILE];
-    __shared__ unsigned short cnt[RS_WARPS * BINS];
-    __shared__ unsigned at[BINS], sums[RS_WARPS];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const unsigned base = w * (32 * RS_ROUNDS) + lane;
-    uint2 e[RS_ROUNDS];
-    unsigned short rank[RS_ROUNDS];
+// At most RS_SMALL entries: all digits of 8 bits by one block, entries in registers between passes through shared memory (one
+// launch instead of six; with 16383 entries it takes longer than the six, 37 us against 30).  Warp w has entries [32 R w, 32 R (w + 1)), R rounds.
+constexpr int RS_SMALL_THREADS = 1024, RS_SMALL_WARPS = 32, RS_SMALL_ROUNDS = 8, RS_SMALL = RS_SMALL_THREADS * RS_SMALL_ROUNDS;
+
+__global__ void __launch_bounds__(RS_SMALL_THREADS) sort_small_kernel(const SortArgs a) {
+    constexpr unsigned BINS = 1u << RS_SMALL_BITS, MASK = BINS - 1;
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ unsigned at[BINS], sums[RS_SMALL_WARPS];
+    const int rounds = (int)((a.n + RS_SMALL_THREADS - 1) / RS_SMALL_THREADS), lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    unsigned *keys = reinterpret_cast<unsigned *>(raw);
+    unsigned short *nums = reinterpret_cast<unsigned short *>(keys + rounds * RS_SMALL_THREADS);
+    unsigned short *cnt = nums + rounds * RS_SMALL_THREADS;  // (warps, bins)
+    const unsigned base = w * (32 * rounds) + lane;
+    unsigned key[RS_SMALL_ROUNDS];
+    unsigned short num[RS_SMALL_ROUNDS], rank[RS_SMALL_ROUNDS];
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) {
+    for (int r = 0; r < RS_SMALL_ROUNDS; ++r) {
         const unsigned i = base + r * 32;
-        e[r] = i < a.n ? make_uint2(index_key(a, i), i) : make_uint2(0, 0);
-        if (i < a.n && a.dweight && e[r].x == (unsigned)a.rows) a.dweight[i] = 0.0f;
+        key[r] = 0;
+        num[r] = (unsigned short)i;
+        if (r < rounds && i < a.n) {
+            key[r] = index_key(a, i);
+            if (a.dweight && key[r] == (unsigned)a.rows) a.dweight[i] = 0.0f;
+        }
     }
     for (int shift = 0; shift < a.key_bits; shift += RS_SMALL_BITS) {
-        for (unsigned b = threadIdx.x; b < BINS * RS_WARPS / 2; b += RS_THREADS) reinterpret_cast<unsigned *>(cnt)[b] = 0;
+        for (unsigned b = threadIdx.x; b < BINS * RS_SMALL_WARPS / 2; b += RS_SMALL_THREADS) reinterpret_cast<unsigned *>(cnt)[b] = 0;
         __syncthreads();
-        warp_ranks(cnt + w * BINS, e, shift, RS_SMALL_BITS, base, a.n, rank);
-        __syncthreads();
-        unsigned all = 0, before = 0;
-        if (threadIdx.x < BINS)
+        unsigned short *mine = cnt + w * BINS;
 #pragma unroll
-            for (int k = 0; k < RS_WARPS; ++k) {
-                const unsigned c = cnt[k * BINS + threadIdx.x];
-                cnt[k * BINS + threadIdx.x] = (unsigned short)before;
-                before += c;
+        for (int r = 0; r < RS_SMALL_ROUNDS; ++r) {
+            if (r >= rounds) break;
+            const bool in = base + r * 32 < a.n;
+            const unsigned d = (key[r] >> shift) & MASK, some = __ballot_sync(0xffffffffu, in);
+            unsigned same = in ? some : ~some;
+#pragma unroll
+            for (int b = 0; b < RS_SMALL_BITS; ++b) {
+                const bool one = (d >> b) & 1u;
+                const unsigned ones = __ballot_sync(0xffffffffu, one);
+                same &= one ? ones : ~ones;
             }
-        const unsigned digit = block_exclusive(before, sums, &all);
+            const unsigned below = __popc(same & ((1u << lane) - 1u)), before = in ? mine[d] : 0u;
+            __syncwarp();
+            if (in && below == 0) mine[d] = (unsigned short)(before + __popc(same));
+            __syncwarp();
+            rank[r] = (unsigned short)(before + below);
+        }
+        __syncthreads();
+        // first positions: digits before this one, then warps before this one
+        unsigned count = 0, all = 0;
+        if (threadIdx.x < BINS)
+#pragma unroll 8
+            for (int k = 0; k < RS_SMALL_WARPS; ++k) {
+                const unsigned c = cnt[k * BINS + threadIdx.x];
+                cnt[k * BINS + threadIdx.x] = (unsigned short)count;
+                count += c;
+            }
+        const unsigned digit = block_exclusive<RS_SMALL_WARPS>(count, sums, &all);
         if (threadIdx.x < BINS) at[threadIdx.x] = digit;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < RS_ROUNDS; ++r) {
-            const unsigned d = (e[r].x >> shift) & (BINS - 1);
-            if (base + r * 32 < a.n) entry[at[d] + cnt[w * BINS + d] + rank[r]] = e[r];
+        for (int r = 0; r < RS_SMALL_ROUNDS; ++r) {
+            if (r >= rounds || base + r * 32 >= a.n) break;
+            const unsigned d = (key[r] >> shift) & MASK, pos = at[d] + mine[d] + rank[r];
+            keys[pos] = key[r];
+            nums[pos] = num[r];
         }
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < RS_ROUNDS; ++r)
-            if (base + r * 32 < a.n) e[r] = entry[base + r * 32];
+        for (int r = 0; r < RS_SMALL_ROUNDS; ++r)
+            if (r < rounds && base + r * 32 < a.n) {
+                key[r] = keys[base + r * 32];
+                num[r] = nums[base + r * 32];
+            }
     }
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r)
-        if (base + r * 32 < a.n) {
-            a.key_out[base + r * 32] = e[r].x;
-            a.val_out[base + r * 32] = e[r].y;
+    for (int r = 0; r < RS_SMALL_ROUNDS; ++r)
+        if (r < rounds && base + r * 32 < a.n) {
+            a.key_out[base + r * 32] = key[r];
+            a.val_out[base + r * 32] = num[r];
         }
 }
 
@@ -897,7 +968,7 @@ GradPlan grad_plan(long long rows, long long n, int width) {
     };
     g.key = take(4 * n);
     g.val = take(4 * n);
-    if (g.tiles > 1) {
+    if (n > RS_SMALL) {
         for (int b = 0; b < 2; ++b) g.entries[b] = take(b < g.passes - 1 ? 8 * n : 0);
         g.hist = take((4ll << (g.bits + g.passes - 1) / g.passes) * g.tiles);
         g.total = take(4ll * RS_BINS);
@@ -920,8 +991,11 @@ int sort_entries(const flare_lookup_grad_args *in, const GradPlan &g, bool dot, 
     s.n = (unsigned)in->n;
     s.tiles = g.tiles;
     s.key_bits = g.bits;
-    if (g.tiles == 1) {
-        sort_small_kernel<<<1, RS_THREADS, 0, st>>>(s);
+    if (in->n <= RS_SMALL) {
+        const int e = allow_shared_memory(reinterpret_cast<const void *>(sort_small_kernel), "flare_lookup_backward");
+        if (e) return e;
+        const int entries = (int)((in->n + RS_SMALL_THREADS - 1) / RS_SMALL_THREADS) * RS_SMALL_THREADS;
+        sort_small_kernel<<<1, RS_SMALL_THREADS, entries * 6 + RS_SMALL_WARPS * 2 * (1 << RS_SMALL_BITS), st>>>(s);
     } else {
         s.hist = words(g.hist);
         s.total = words(g.total);

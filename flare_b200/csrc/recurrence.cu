@@ -3,7 +3,7 @@
 // A stretch of steps maps the state that enters it to A h + H (A the product of its gates, H what it yields from 0), and
 // two stretches join to (A2 A1, A2 H1 + H2), so a sequence can be cut in time:
 //   * a thread holds SPAN = 16 steps of VE neighbouring channels in registers, all loaded before the first is used;
-//   * the W warps of a block take W consecutive spans, exchange their (A, H) through shared memory and run their own
+//   * the W warps of a tile take W consecutive spans, pass the state through their (A, H) in shared memory and run their own
 //     span again from the state that enters it (from registers: every input is read once);
 //   * with few channels and many steps, S blocks share a sequence: a first kernel writes each block's (A, H), the
 //     second folds the ones before its own (the inputs are then read twice, the second time mostly from L2).
@@ -178,37 +178,67 @@ __device__ __forceinline__ void tile_sync(int wlog) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 << wlog) : "memory");
 }
 
-// The state that enters warp w's stretch, from the state `carry` that enters all W of them; carry becomes what leaves them.
-// BACK: warps are passed from the last to the first.  buf: (2, W, 32 VE) floats, not the one of the call before.
+// How the W warps of a tile pass the state along time.  Of a lane's VE channels thread (w, lane) looks after v = w, w + W, ...:
+// it holds their state at the round's border and passes it through all W stretches, so that the walk over the warps is
+// done once per channel and not once per warp (which took 2.5 of the 8 instructions an element took).
+// BACK: warps are passed from the last to the first.
 template <bool BACK, int VE>
-__device__ __forceinline__ void exchange(float *buf, int wlog, const float (&A)[VE], const float (&H)[VE], float (&carry)[VE], float (&in)[VE]) {
-    const int W = 1 << wlog, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1);
-    float *sa = buf, *sh = buf + W * 32 * VE;
-#pragma unroll
-    for (int v = 0; v < VE; ++v) {
-        sa[(w * VE + v) * 32 + lane] = A[v];
-        sh[(w * VE + v) * 32 + lane] = H[v];
+struct Pass {
+    static constexpr int MINE = (VE + 1) / 2;  // W > 1
+    float *sa, *sh;                            // (W, VE, 32) each
+    int wlog, w, lane;
+    float carry[MINE];
+    __device__ __forceinline__ Pass(float *smem, int wlog_) : wlog(wlog_), w((threadIdx.x >> 5) & ((1 << wlog_) - 1)), lane(threadIdx.x & 31) {
+        sa = smem + ((threadIdx.x >> (5 + wlog)) << wlog) * (2 * VE * 32);
+        sh = sa + (VE * 32 << wlog);
     }
-    tile_sync(wlog);
+    template <class F>
+    __device__ __forceinline__ void each(F f) {  // f(q, v) for the channels that this thread looks after
 #pragma unroll
-    for (int v = 0; v < VE; ++v) in[v] = carry[v];
-#pragma unroll 4
-    for (int k = 0; k < W; ++k) {
-        const int o = BACK ? W - 1 - k : k;
-#pragma unroll
-        for (int v = 0; v < VE; ++v) {
-            if (o == w) in[v] = carry[v];
-            carry[v] = through(sa[(o * VE + v) * 32 + lane], sh[(o * VE + v) * 32 + lane], carry[v]);
+        for (int q = 0; q < MINE; ++q) {
+            const int v = w + (q << wlog);
+            if (v < VE) f(q, v);
         }
     }
-}
+    __device__ __forceinline__ void begin(const float *ends, unsigned chain) {
+        each([&](int q, int v) { carry[q] = ends ? ends[chain + v] : 0.0f; });
+    }
+    __device__ __forceinline__ void finish(float *ends, unsigned chain) {
+        each([&](int q, int v) { ends[chain + v] = carry[q]; });
+    }
+    // (A, H): this warp's stretch; in: the state that enters it.  prod (optional): times the product of all stretches' A
+    __device__ __forceinline__ void run(const float (&A)[VE], const float (&H)[VE], float (&in)[VE], float *prod = nullptr) {
+        const int W = 1 << wlog;
+#pragma unroll
+        for (int v = 0; v < VE; ++v) {
+            sa[(w * VE + v) * 32 + lane] = A[v];
+            sh[(w * VE + v) * 32 + lane] = H[v];
+        }
+        tile_sync(wlog);
+        each([&](int q, int v) {
+            float c = carry[q];
+#pragma unroll 4
+            for (int k = 0; k < W; ++k) {
+                const int at = ((BACK ? W - 1 - k : k) * VE + v) * 32 + lane;
+                const float a = sa[at];
+                sa[at] = c;
+                c = through(a, sh[at], c);
+                if (prod) prod[q] *= a;
+            }
+            carry[q] = c;
+        });
+        tile_sync(wlog);
+#pragma unroll
+        for (int v = 0; v < VE; ++v) in[v] = sa[(w * VE + v) * 32 + lane];
+    }
+};
 
-// The state that enters block `split`: `c` through the blocks before it in the walk.  Each of the W warps joins a
+// The state that enters block `split`: pass.carry through the blocks before it in the walk.  Each of the W warps joins a
 // part of them, then the parts are passed in order.
 template <bool BACK, int VE>
-__device__ __forceinline__ void fold_splits(const RecArgs &a, unsigned chain, int split, float *buf, float (&c)[VE]) {
+__device__ __forceinline__ void fold_splits(const RecArgs &a, unsigned chain, int split, Pass<BACK, VE> &pass) {
     const long long chains = a.seqs * a.width;
-    const int W = 1 << a.wlog, w = (threadIdx.x >> 5) & (W - 1);
+    const int W = 1 << a.wlog, w = pass.w;
     const int n = BACK ? a.splits - 1 - split : split;
     if (n == 0) return;
     // parts in the order of the walk: warp w (BACK: W - 1 - w) has the w-th
@@ -231,13 +261,7 @@ __device__ __forceinline__ void fold_splits(const RecArgs &a, unsigned chain, in
             A[v] *= pa.get(v);
         }
     }
-    if (W > 1) {
-        exchange<BACK>(buf, a.wlog, A, H, c, unused);
-        tile_sync(a.wlog);  // the rounds that follow use the buffer again
-    } else {
-#pragma unroll
-        for (int v = 0; v < VE; ++v) c[v] = through(A[v], H[v], c[v]);
-    }
+    pass.run(A, H, unused);
 }
 
 template <int VE>
@@ -271,34 +295,27 @@ __device__ __forceinline__ void clear_rest(const RecArgs &a, void *out, long lon
 __device__ __forceinline__ unsigned my_tile(const RecArgs &a) {
     return blockIdx.x * (WARPS >> a.wlog) + (threadIdx.x >> (5 + a.wlog));
 }
-// a tile's part of the exchange buffers: two of (2, W, 32 VE) floats
-template <int VE>
-__device__ __forceinline__ float *my_buffers(const RecArgs &a, float *smem) {
-    return smem + ((threadIdx.x >> (5 + a.wlog)) << a.wlog) * (4 * 32 * VE);
-}
 __device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(0xffffffffu, v); }
 
 // BACK false: (A, H) of x; true: of dh, from the end.  grid (tiles, splits); W > 1
 template <bool BACK, class T, class GT, int VE, bool SHARED>
 __global__ void __launch_bounds__(32 * WARPS) recurrence_split_kernel(const RecArgs a) {
     extern __shared__ __align__(16) float smem[];
-    const int W = 1 << a.wlog, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
+    const int W = 1 << a.wlog, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
     const Place<VE, false> me(a, my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
-    float *bufs = my_buffers<VE>(a, smem);
-    const int round = SPAN << a.wlog, n = (warp_max(t1 - t0) + round - 1) >> (4 + a.wlog);
+    Pass<BACK, VE> pass(smem, a.wlog);
+    const int round = W * SPAN, n = (warp_max(t1 - t0) + round - 1) >> (4 + a.wlog);
     const T *src = static_cast<const T *>(BACK ? a.dh : a.x);
     const int src_t = BACK ? a.dh_t : a.x_t;
     const int gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -src_t : src_t;
     const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + a.share.div(me.c);
     const T *xp = src + me.first(a, BACK ? a.dh_s : a.x_s, src_t) + me.c;
-    float A[VE], H[VE], tA[VE], tH[VE], unused[VE];
+    float A[VE], H[VE], unused[VE], prod[Pass<BACK, VE>::MINE];
+    pass.begin(nullptr, 0);
 #pragma unroll
-    for (int v = 0; v < VE; ++v) {
-        tA[v] = 1.0f;
-        tH[v] = 0.0f;
-    }
+    for (int q = 0; q < Pass<BACK, VE>::MINE; ++q) prod[q] = 1.0f;
     for (int k = 0; k < n; ++k) {
         const int t = t0 + (BACK ? n - 1 - k : k) * round + w * SPAN, left = t1 - t;
         Span<GT, SHARED ? 1 : VE> g;
@@ -311,18 +328,13 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_split_kernel(const RecA
             x.template load<false, true>(xp + (long long)t * xs, xs, src ? left : 0, 0.0f);
         }
         stretch<BACK>(g, x, A, H);
-        float *buf = bufs + (k & 1) * 2 * W * 32 * VE;
-        exchange<BACK>(buf, a.wlog, A, H, tH, unused);
-        // the product of the round's gates, in the same buffer
-        for (int o = 0; o < W; ++o)
-#pragma unroll
-            for (int v = 0; v < VE; ++v) tA[v] *= buf[(o * VE + v) * 32 + lane];
+        pass.run(A, H, unused, prod);
     }
-    if (w == 0 && me.active) {
+    if (me.active) {
         const long long chains = a.seqs * a.width;
-        float *p = a.agg + (long long)split * 2 * chains + me.chain;
-        store_ends<VE>(p, tA);
-        store_ends<VE>(p + chains, tH);
+        float *p = a.agg + (long long)split * 2 * chains;
+        pass.each([&](int q, int v) { p[me.chain + v] = prod[q]; });
+        pass.finish(p + chains, me.chain);
     }
 }
 
@@ -333,17 +345,18 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const Re
     const Place<VE, false> me(a, my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
-    float *bufs = my_buffers<VE>(a, smem);
+    Pass<false, VE> pass(smem, a.wlog);
     const int round = SPAN << a.wlog, n = (warp_max(t1 - t0) + round - 1) >> (4 + a.wlog);
     const int gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t, hs = a.reverse ? -a.h_t : a.h_t;
     const GT *gp = static_cast<const GT *>(a.gate) + me.first(a, a.gate_s, a.gate_t) + a.share.div(me.c);
     const T *xp = static_cast<const T *>(a.x) + me.first(a, a.x_s, a.x_t) + me.c;
     T *hp = static_cast<T *>(a.h) + me.first(a, a.h_s, a.h_t) + me.c;
     float carry[VE], h[VE], A[VE], H[VE];
-    load_ends<VE>(a.state, me.chain, me.active, carry);
-    if (a.splits > 1) fold_splits<false, VE>(a, me.chain, split, bufs, carry);
+    if (W > 1) pass.begin(a.state, me.chain);
+    else load_ends<VE>(a.state, me.chain, true, carry);
+    if (a.splits > 1) fold_splits<false, VE>(a, me.chain, split, pass);
     // a span of which every lane has all steps needs no tests
-    auto span = [&](auto full, int k, int t, int left) {
+    auto span = [&](auto full, int t, int left) {
         constexpr bool FULL = decltype(full)::value;
         Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x;
@@ -351,7 +364,7 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const Re
         x.template load<FULL, false>(xp + (long long)t * xs, xs, left, 0.0f);
         if (W > 1) {
             stretch<false>(g, x, A, H);
-            exchange<false>(bufs + (k & 1) * 2 * W * 32 * VE, a.wlog, A, H, carry, h);
+            pass.run(A, H, h);
         } else {
 #pragma unroll
             for (int v = 0; v < VE; ++v) h[v] = carry[v];
@@ -385,14 +398,17 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const Re
     };
     for (int k = 0; k < n; ++k) {
         const int t = t0 + k * round + w * SPAN, left = t1 - t;
-        if (__all_sync(0xffffffffu, left >= SPAN)) span(std::true_type{}, k, t, left);
-        else span(std::false_type{}, k, t, left);
+        if (__all_sync(0xffffffffu, left >= SPAN)) span(std::true_type{}, t, left);
+        else span(std::false_type{}, t, left);
     }
-    if (w == 0 && split == a.splits - 1 && me.active) store_ends<VE>(a.last + me.chain, carry);
+    if (split == a.splits - 1 && me.active) {
+        if (W > 1) pass.finish(a.last, me.chain);
+        else store_ends<VE>(a.last + me.chain, carry);
+    }
     if (a.packed && a.h) clear_rest<T>(a, a.h, a.h_t, a.width);
 }
 
-// smem: the exchange buffers, then SHARED: 16 x 32 products per warp
+// smem: what the warps pass, then SHARED: 16 x 32 products per warp
 // DH: whether there is a gradient of every state, not of the last ones alone
 template <class T, class GT, int VE, bool SHARED, bool DH>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(const RecArgs a) {
@@ -401,8 +417,8 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
     const Place<VE, SHARED> me(a, my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
-    float *bufs = my_buffers<VE>(a, smem);
-    float *sums = smem + (W > 1 ? 4 * WARPS * 32 * VE : 0) + (threadIdx.x >> 5) * (SPAN * SUM_STRIDE);
+    Pass<true, VE> pass(smem, a.wlog);
+    float *sums = smem + (W > 1 ? 2 * WARPS * 32 * VE : 0) + (threadIdx.x >> 5) * (SPAN * SUM_STRIDE);
     const int round = SPAN << a.wlog, n = (warp_max(t1 - t0) + round - 1) >> (4 + a.wlog);
     const int gc = (int)a.share.div(me.c);
     const int gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t;
@@ -413,9 +429,10 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
     T *dxp = static_cast<T *>(a.dx) + me.first(a, a.dx_s, a.dx_t) + me.c;
     GT *dgp = static_cast<GT *>(a.dgate) + me.first(a, a.dgate_s, a.dgate_t) + gc;
     float carry[VE], mu[VE], A[VE], H[VE];
-    load_ends<VE>(a.dlast, me.chain, me.active, carry);
-    if (a.splits > 1) fold_splits<true, VE>(a, me.chain, split, bufs, carry);
-    auto span = [&](auto full, int k, int t, int left) {
+    if (W > 1) pass.begin(a.dlast, me.chain);
+    else load_ends<VE>(a.dlast, me.chain, true, carry);
+    if (a.splits > 1) fold_splits<true, VE>(a, me.chain, split, pass);
+    auto span = [&](auto full, int t, int left) {
         constexpr bool FULL = decltype(full)::value;
         Span<GT, SHARED ? 1 : VE> g;
         Span<T, VE> x, dh;
@@ -428,7 +445,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
         if (W > 1) {
             if (!DH) dh.template load<false, false>(nullptr, 0, 0, 0.0f);
             stretch<true>(g, dh, A, H);
-            exchange<true>(bufs + (k & 1) * 2 * W * 32 * VE, a.wlog, A, H, carry, mu);
+            pass.run(A, H, mu);
         } else {
 #pragma unroll
             for (int v = 0; v < VE; ++v) mu[v] = carry[v];
@@ -491,10 +508,13 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
     };
     for (int k = 0; k < n; ++k) {
         const int t = t0 + (n - 1 - k) * round + w * SPAN, left = t1 - t;
-        if (__all_sync(0xffffffffu, left >= SPAN)) span(std::true_type{}, k, t, left);
-        else span(std::false_type{}, k, t, left);
+        if (__all_sync(0xffffffffu, left >= SPAN)) span(std::true_type{}, t, left);
+        else span(std::false_type{}, t, left);
     }
-    if (a.dstate && w == 0 && split == 0 && me.active) store_ends<VE>(a.dstate + me.chain, carry);
+    if (a.dstate && split == 0 && me.active) {
+        if (W > 1) pass.finish(a.dstate, me.chain);
+        else store_ends<VE>(a.dstate + me.chain, carry);
+    }
     if (a.packed) {
         clear_rest<T>(a, a.dx, a.dx_t, a.width);
         if (a.parts == 1) clear_rest<GT>(a, a.dgate, a.dgate_t, a.groups);
@@ -591,7 +611,7 @@ RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
 RecArgs rec_args(const flare_recurrence_args *in, const RecPlan &p) {
     RecArgs a{};
     a.gate = in->gate, a.x = in->x, a.dh = in->dh, a.offsets = in->offsets;
-    a.state = in->state, a.dlast = in->dlast;
+    if (in->seqs) a.state = in->state, a.dlast = in->dlast;
     a.h = in->h, a.dgate = in->dgate, a.dx = in->dx;
     a.last = in->last, a.saved = in->saved, a.dstate = in->dstate;
     a.agg = static_cast<float *>(in->workspace);
@@ -641,7 +661,7 @@ int run_recurrence(const flare_recurrence_args *in, bool backward, cudaStream_t 
     const int at_once = WARPS / p.warps;  // tiles per block
     // a block is launched for rows of no sequence even where there is no sequence
     const dim3 grid((unsigned)std::max(1ll, (p.tiles + at_once - 1) / at_once), (unsigned)p.splits);
-    const size_t buffers = p.warps > 1 ? sizeof(float) * 4 * WARPS * 32 * p.ve : 0;
+    const size_t buffers = p.warps > 1 ? sizeof(float) * 2 * WARPS * 32 * p.ve : 0;
     rec_dispatch(in, p, [&](auto t, auto gt, auto ve, auto shared) {
         using T = typename decltype(t)::type;
         using GT = typename decltype(gt)::type;

@@ -36,7 +36,8 @@ FORWARD = [
     dict(rows=50, width=96, n=33, table=BF16, index=torch.int64, weight=False), dict(rows=300, width=32, n=257, table=F32),
     dict(rows=20, width=1023, n=40, table=BF16), dict(rows=20, width=2050, n=13), dict(rows=9, width=12, n=100),
     dict(rows=9, width=96, n=100, pad=8), dict(rows=9, width=96, n=100, pad=3), dict(rows=9, width=6, n=100, pad=1, table=F32),
-    dict(rows=40, width=96, n=48, shape=(16, 3)), dict(rows=3, width=8, n=20, empty=1.0),
+    dict(rows=40, width=96, n=48, shape=(16, 3)), dict(rows=3, width=8, n=20, empty=1.0), dict(rows=9, width=150, n=70, pad=1),
+    dict(rows=30, width=771, n=50, table=F32, weight=False), dict(rows=30, width=64, n=50, pad=1),
 ]
 
 
@@ -88,7 +89,9 @@ BACKWARD = [
     dict(rows=2, width=64, n=255, empty=0.0), dict(rows=1, width=64, n=256, empty=0.0), dict(rows=1, width=64, n=257, empty=0.0),
     dict(rows=3, width=260, n=5000, table=F32, weight=False), dict(rows=9, width=1023, n=700, table=BF16),
     dict(rows=50, width=4, n=4097, table=F32), dict(rows=12, width=16, n=64, empty=1.0), dict(rows=9, width=24, n=100, pad=8),
-    dict(rows=40, width=96, n=48, shape=(16, 3)),
+    dict(rows=40, width=96, n=48, shape=(16, 3)), dict(rows=100_000, width=5, n=17_000), dict(rows=300, width=96, n=16_383, hot=0.5),
+    dict(rows=2000, width=20, n=40_000, table=F32, hot=0.3), dict(rows=70, width=200, n=3000), dict(rows=50, width=192, n=2000, table=BF16),
+    dict(rows=50, width=256, n=900, pad=8), dict(rows=50, width=128, n=900, table=F32), dict(rows=50, width=132, n=900, table=F32),
 ]
 
 
@@ -114,7 +117,7 @@ def test_lookup_backward(c):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n", [4095, 4096, 4097, 100_000])
+@pytest.mark.parametrize("n", [1023, 1025, 4097, 8192, 8193, 100_000])
 def test_lookup_backward_many_equal_entries(n):
     """Rows of 0, 1 and thousands of entries, runs that end inside a chunk: whole numbers sum exactly, so equality."""
     g = torch.Generator().manual_seed(n)
