@@ -992,7 +992,7 @@ int sort_entries(const flare_lookup_grad_args *in, const GradPlan &g, bool dot, 
     s.tiles = g.tiles;
     s.key_bits = g.bits;
     if (in->n <= RS_SMALL) {
-        const int e = allow_shared_memory(reinterpret_cast<const void *>(sort_small_kernel), "flare_lookup_backward");
+        const int e = allow_shared_memory<sort_small_kernel>("flare_lookup_backward");
         if (e) return e;
         const int entries = (int)((in->n + RS_SMALL_THREADS - 1) / RS_SMALL_THREADS) * RS_SMALL_THREADS;
         sort_small_kernel<<<1, RS_SMALL_THREADS, entries * 6 + RS_SMALL_WARPS * 2 * (1 << RS_SMALL_BITS), st>>>(s);
@@ -1042,10 +1042,9 @@ int launch_ring(GradArgs a, cudaStream_t st) {
     a.work_blocks = (unsigned)(((long long)a.ranges * a.tiles + GROUPS - 1) / GROUPS);
     a.empty_rows = empty_rows(a.rows);
     const unsigned empty_blocks = (unsigned)((a.rows + a.empty_rows * RING_WARPS - 1) / (a.empty_rows * RING_WARPS));
-    auto fn = grad_ring_kernel<D, T, G, DOT>;
-    const int e = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_lookup_backward");
+    const int e = allow_shared_memory<grad_ring_kernel<D, T, G, DOT>>("flare_lookup_backward");
     if (e) return e;
-    fn<<<a.work_blocks + empty_blocks, 32 * RING_WARPS, GROUPS * RING_STAGES * Piece::bytes(a.pieces), st>>>(a);
+    grad_ring_kernel<D, T, G, DOT><<<a.work_blocks + empty_blocks, 32 * RING_WARPS, GROUPS * RING_STAGES * Piece::bytes(a.pieces), st>>>(a);
     launch_join<Piece::VE>(a, st);
     return FLARE_OK;
 }

@@ -5,33 +5,10 @@
 // exchange.  With 8 elements a lane the instructions per element bound it (3M x 96 f16: 207 us to codes and 150 us back).
 // Other rows go by 8 elements a lane, four lanes to a block.
 #include <algorithm>
-#include <mutex>
-#include <set>
-#include <utility>
 
 #include "ops.cuh"
 
 namespace flare {
-
-int allow_shared_memory(const void *kernel, const char *what) {
-    static std::mutex lock;
-    static std::set<std::pair<const void *, int>> allowed;
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess) {
-        std::lock_guard<std::mutex> hold(lock);
-        if (allowed.count({kernel, device})) return FLARE_OK;
-        cudaFuncAttributes at{};
-        e = cudaFuncGetAttributes(&at, kernel);
-        // 227 KB a block, less what the kernel has already
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)at.sharedSizeBytes);
-        if (e == cudaSuccess) allowed.insert({kernel, device});
-    }
-    if (e == cudaSuccess) return FLARE_OK;
-    set_error("%s: %s", what, cudaGetErrorString(e));
-    return FLARE_E_CUDA;
-}
 
 constexpr int MQ_THREADS = 256;
 

@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/flare_b200.h"
@@ -132,8 +133,25 @@ struct FastDiv {
     __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
 };
 
-// Lets a kernel have all of a multiprocessor's shared memory, once per device.
-int allow_shared_memory(const void *kernel, const char *what);
+// Lets kernel K have all of a multiprocessor's shared memory, once per device.
+template <auto K>
+int allow_shared_memory(const char *what) {
+    static std::atomic<unsigned long long> done{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (e == cudaSuccess && (done.load() & bit)) return FLARE_OK;
+    cudaFuncAttributes at{};
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, K);
+    // 227 KB a block, less what the kernel has already
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)at.sharedSizeBytes);
+    if (e != cudaSuccess) {
+        set_error("%s: %s", what, cudaGetErrorString(e));
+        return FLARE_E_CUDA;
+    }
+    done.fetch_or(bit);
+    return FLARE_OK;
+}
 
 template <class T>
 struct TypeTag { using type = T; };

@@ -750,8 +750,7 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorM
     a.stages = (int)std::min<long long>(Tile::MAX_STAGES, per * ((tiles + grid - 1) / grid));
     int smem = a.stages * Tile::STAGE + 4 * OUT_BYTES + 1024;
     if (split > 1) smem = std::max(smem, PT * BN * 4 + 1024);
-    auto fn = product_kernel<BN, O, X>;
-    const int e0 = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_micro_product");
+    const int e0 = allow_shared_memory<product_kernel<BN, O, X>>("flare_micro_product");
     if (e0) return e0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid, 1, (unsigned)split);
@@ -764,7 +763,7 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorM
     attr.val.clusterDim.z = (unsigned)split;
     cfg.attrs = &attr;
     cfg.numAttrs = split > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, pm, qm, om, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, product_kernel<BN, O, X>, pm, qm, om, a);
     if (e != cudaSuccess) {
         set_error("flare_micro_product: %s", cudaGetErrorString(e));
         return FLARE_E_CUDA;
@@ -775,10 +774,9 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorM
 template <int BN, class O>
 int launch_narrow(const CUtensorMap &om, const unsigned char *pc, const unsigned char *qc, ProductArgs a, cudaStream_t st) {
     a.tiles = (unsigned)((a.p + PT - 1) / PT);
-    auto fn = product_narrow_kernel<BN, O>;
-    const int e = allow_shared_memory(reinterpret_cast<const void *>(fn), "flare_micro_product");
+    const int e = allow_shared_memory<product_narrow_kernel<BN, O>>("flare_micro_product");
     if (e) return e;
-    fn<<<std::min(a.tiles, (unsigned)(NARROW_BLOCKS * SMS)), PR_THREADS, NarrowTile<BN>::SMEM, st>>>(om, pc, qc, a);
+    product_narrow_kernel<BN, O><<<std::min(a.tiles, (unsigned)(NARROW_BLOCKS * SMS)), PR_THREADS, NarrowTile<BN>::SMEM, st>>>(om, pc, qc, a);
     OPS_LAUNCHED("flare_micro_product");
     return FLARE_OK;
 }

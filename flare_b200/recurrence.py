@@ -33,8 +33,10 @@ def _like(t, width, dtype):
 
 
 def _strides(t):
-    """(per sequence, per step) in elements."""
-    return (0, 0) if t is None else t.stride()[:2] if t.dim() == 3 else (0, t.stride(0))
+    """(per sequence, per step) in elements; a single step's stride means nothing."""
+    if t is None:
+        return 0, 0
+    return (t.stride(0) if t.dim() == 3 else 0), (t.stride(-2) if t.shape[-2] > 1 else 0)
 
 
 def _inputs(gate, x, state, offsets):
@@ -94,7 +96,8 @@ def scan(gate, x, state=None, offsets=None, reverse=False, states=True, training
     sequence s is rows offsets[s] to offsets[s + 1]; it may be empty.  Rows of no sequence get zeros.
     h: every state, of x's shape and type (None if not states); last: the final states (sequences, width) f32; saved:
     what scan_backward needs (None if not training).  The recurrence runs in 32 bits, h is rounded once; a product of
-    gates over any stretch of steps has to stay within the range of a float.
+    gates over any stretch of steps has to stay within the range of a float.  A tensor's steps are less than 2 GB apart
+    (FlareError).
     """
     lib = _lib.load()
     gate, x, offsets, seqs = _inputs(gate, x, state, offsets)

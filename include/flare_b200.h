@@ -409,7 +409,8 @@ int flare_lookup_backward(const flare_lookup_grad_args *a, void *stream);
  * backward needs: the state before every FLARE_RECURRENCE_SPAN-th step, flare_recurrence_saved floats).
  * Backward reads gate, x, state, saved, dh (NULL: 0) and dlast (NULL: 0) and writes dgate, dx and, if not
  * NULL, dstate.  workspace: flare_recurrence_workspace bytes, 16-byte aligned, contents irrelevant.
- * A product of gates over a stretch of steps has to stay within the range of a float.
+ * A product of gates over a stretch of steps has to stay within the range of a float.  seqs * width and steps are
+ * below 2^30, the steps of a tensor less than 2^31 bytes apart.
  */
 #define FLARE_RECURRENCE_SPAN 16
 typedef struct flare_recurrence_args {
