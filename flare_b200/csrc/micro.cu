@@ -48,17 +48,12 @@ __global__ void __launch_bounds__(MQ_THREADS) micro_quantize_kernel(const MicroA
     for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(f[e]) & 0x7fffffffu);
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    unsigned byte, bits = 0;
-    if (most >= 0x7f800000u) {
-        byte = 255;
-    } else {
-        // floor(log2) of the largest is its exponent field - 127; below 2^-125 (subnormal ones too) the clamp decides
-        const int e = most == 0 ? -127 : max((int)(most >> 23) - 127 - 2, -127);
-        byte = (unsigned)(e + 127);
-        const float inv = __uint_as_float((unsigned)(127 - e) << 23);  // 2^-e, e in [-127, 125]
+    float inv;
+    const unsigned byte = micro_byte(most, &inv);
+    unsigned bits = 0;
+    if (byte != 255)
 #pragma unroll
         for (int p = 0; p < 4; ++p) bits |= micro_code_pair(f[2 * p] * inv, f[2 * p + 1] * inv) << (8 * p);
-    }
     if (!in) return;
     *reinterpret_cast<unsigned *>(a.codes + row * (16ll * a.blocks) + 4 * piece) = bits;
     if ((piece & 3) == 0) {
@@ -98,7 +93,7 @@ __global__ void __launch_bounds__(MQ_THREADS) micro_dequantize_kernel(const Micr
 }
 
 // 32 bytes, aligned to as many
-__device__ __forceinline__ void load32(const void *p, unsigned (&w)[8]) {
+__device__ __forceinline__ void load32(const void *p, unsigned *w) {
     asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                  : "l"(p));
@@ -108,48 +103,18 @@ __device__ __forceinline__ void store32(void *p, const unsigned (&w)[8]) {
                  "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
 }
-__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) {
-    unsigned d;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-
-// 16 elements of T in 32-byte words, and the largest magnitude's bits as a float's
+// 16 elements of T
 template <class T>
 struct Sixteen {
     static constexpr int N = (int)sizeof(T) / 2;  // 32-byte pieces
-    unsigned w[N][8];
+    unsigned w[8 * N];
     __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) load32(reinterpret_cast<const char *>(p) + 32 * i, w[i]);
+        for (int i = 0; i < N; ++i) load32(reinterpret_cast<const char *>(p) + 32 * i, w + 8 * i);
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[i][k] = 0;
-    }
-    __device__ __forceinline__ float2 pair(int k) const {  // elements 2k, 2k + 1
-        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[k / 4][2 * k % 8]), __uint_as_float(w[k / 4][2 * k % 8 + 1]));
-        else if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2 *>(&w[0][k]));
-        else return make_float2(__uint_as_float(w[0][k] << 16), __uint_as_float(w[0][k] & 0xffff0000u));
-    }
-    // magnitudes compare as their bits do; infinities and NaN are the largest
-    __device__ __forceinline__ unsigned most() const {
-        unsigned m = 0;
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) m = max(m, w[i][k] & 0x7fffffffu);
-            return m;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) m = max_u16x2(m, w[0][k] & 0x7fff7fffu);
-            m = max(m & 0xffffu, m >> 16);
-            if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
-            else return m << 16;
-        }
+        for (int k = 0; k < 8 * N; ++k) w[k] = 0;
     }
 };
 
@@ -163,21 +128,14 @@ __global__ void __launch_bounds__(MQ_THREADS) micro_quantize16_kernel(const Micr
     Sixteen<T> x;
     if (in && (int)piece * 16 < a.width) x.load(static_cast<const T *>(a.x) + row * a.stride + piece * 16);
     else x.zero();
-    unsigned most = x.most();
+    unsigned most = words_most<T, 8 * Sixteen<T>::N>(x.w);
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    unsigned byte = 255, lo = 0, hi = 0;
-    if (most < 0x7f800000u) {
-        // floor(log2) of the largest is its exponent field - 127; below 2^-125 (subnormal ones too) the clamp decides
-        const int e = max((int)(most >> 23) - 127 - 2, -127);
-        byte = (unsigned)(e + 127);
-        const float inv = __uint_as_float((unsigned)(127 - e) << 23);  // 2^-e, e in [-127, 125]
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float2 v = x.pair(k);
-            const unsigned c = micro_code_pair(v.x * inv, v.y * inv);
-            if (k < 4) lo |= c << (8 * k);
-            else hi |= c << (8 * (k - 4));
-        }
+    float inv;
+    const unsigned byte = micro_byte(most, &inv);
+    unsigned lo = 0, hi = 0;
+    if (byte != 255) {
+        lo = micro_codes8<T>(x.w, 0, inv);
+        hi = micro_codes8<T>(x.w, 4, inv);
     }
     if (!in) return;
     __stcs(reinterpret_cast<uint2 *>(a.codes + row * (16ll * a.blocks)) + piece, make_uint2(lo, hi));

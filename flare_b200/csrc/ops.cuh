@@ -121,6 +121,50 @@ __device__ __forceinline__ unsigned micro_code_pair(float lo, float hi) {
     return c;
 }
 
+__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) {
+    unsigned d;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// Elements 2k and 2k + 1 of T as they lie in 32-bit words.
+template <class T>
+__device__ __forceinline__ float2 words_pair(const unsigned *w, int k) {
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+    else if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+    else return make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+}
+// The largest magnitude in N words, as a float's bits.  Magnitudes compare as their bits do; infinities and NaN are the largest.
+template <class T, int N>
+__device__ __forceinline__ unsigned words_most(const unsigned *w) {
+    unsigned m[4] = {};
+#pragma unroll
+    for (int k = 0; k < N; ++k) m[k & 3] = sizeof(T) == 4 ? max(m[k & 3], w[k] & 0x7fffffffu) : max_u16x2(m[k & 3], w[k] & 0x7fff7fffu);
+    if constexpr (sizeof(T) == 4) return max(max(m[0], m[1]), max(m[2], m[3]));
+    const unsigned p = max_u16x2(max_u16x2(m[0], m[1]), max_u16x2(m[2], m[3])), h = max(p & 0xffffu, p >> 16);
+    if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+    else return h << 16;
+}
+// The scale byte of a block whose largest magnitude is `most`, and 2^-e for its elements (0 where the block stands for NaN).
+__device__ __forceinline__ unsigned micro_byte(unsigned most, float *inv) {
+    *inv = 0.0f;
+    if (most >= 0x7f800000u) return 255;
+    // floor(log2) of the largest is its exponent field - 127; below 2^-125 (subnormal ones too) the clamp decides
+    const int e = max((int)(most >> 23) - 127 - 2, -127);
+    *inv = __uint_as_float((unsigned)(127 - e) << 23);  // e in [-127, 125]
+    return (unsigned)(e + 127);
+}
+// Codes of eight elements, from the 4 pairs k, k + 1, ...
+template <class T>
+__device__ __forceinline__ unsigned micro_codes8(const unsigned *w, int k, float inv) {
+    unsigned c = 0;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const float2 v = words_pair<T>(w, k + p);
+        c |= micro_code_pair(v.x * inv, v.y * inv) << (8 * p);
+    }
+    return c;
+}
+
 // Exact quotient of 31-bit values by a fixed divisor d >= 1 (multiply and shift, Granlund and Montgomery 1994).
 struct FastDiv {
     unsigned d, mul, shift;

@@ -54,36 +54,28 @@ static_assert(X_ROWS * (KSTAGE / 32) == 128, "a block of 32 elements per thread 
 // 32 elements of a row, in flight
 template <class X>
 struct Raw32 {
-    Vec<X, 16 / (int)sizeof(X)> v[2 * (int)sizeof(X)];
+    static constexpr int N = 16 / (int)sizeof(X);  // elements of a 16-byte piece
+    unsigned w[8 * (int)sizeof(X)];
     // left: elements from p to the row's end
     __device__ __forceinline__ void load(const X *p, int left, bool vec) {
-        constexpr int N = 16 / (int)sizeof(X);
 #pragma unroll
         for (int i = 0; i < 32 / N; ++i) {
+            Vec<X, N> v;
             if (vec && left >= (i + 1) * N) {
-                v[i].load(p + i * N);
+                v.load(p + i * N);
             } else {
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[i].el[e] = i * N + e < left ? p[i * N + e] : from_f32<X>(0.0f);
+                for (int e = 0; e < N; ++e) v.el[e] = i * N + e < left ? p[i * N + e] : from_f32<X>(0.0f);
             }
+            w[4 * i] = v.raw[0].x, w[4 * i + 1] = v.raw[0].y, w[4 * i + 2] = v.raw[0].z, w[4 * i + 3] = v.raw[0].w;
         }
     }
     // its 16 bytes of codes and scale byte
     __device__ __forceinline__ uint4 quantize(unsigned *byte) const {
-        constexpr int N = 16 / (int)sizeof(X);
-        unsigned most = 0, w[4] = {};
-#pragma unroll
-        for (int k = 0; k < 32; ++k) most = max(most, __float_as_uint(v[k / N].get(k % N)) & 0x7fffffffu);
-        *byte = 255;
-        if (most < 0x7f800000u) {
-            const int e = max((int)(most >> 23) - 127 - 2, -127);
-            *byte = (unsigned)(e + 127);
-            const float inv = __uint_as_float((unsigned)(127 - e) << 23);
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-                w[k / 4] |= micro_code_pair(v[2 * k / N].get(2 * k % N) * inv, v[2 * k / N].get((2 * k + 1) % N) * inv) << (8 * (k % 4));
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        float inv;
+        *byte = micro_byte(words_most<X, 8 * (int)sizeof(X)>(w), &inv);
+        if (*byte == 255) return make_uint4(0, 0, 0, 0);
+        return make_uint4(micro_codes8<X>(w, 0, inv), micro_codes8<X>(w, 4, inv), micro_codes8<X>(w, 8, inv), micro_codes8<X>(w, 12, inv));
     }
 };
 template <>
@@ -230,6 +222,10 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
     while (cols < (uint32_t)(a.accs * BN + a.stages * Tile::SCOLS)) cols *= 2;
 
     if (warp == 9) tmem_alloc(&tmem_slot, cols);
+    if (threadIdx.x == 256) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&pmap) : "memory");
+        if constexpr (std::is_void_v<X>) asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
+    }
     if (threadIdx.x == 0) {
         gave_up = copies = 0;
         for (int s = 0; s < a.stages; ++s) {
@@ -304,47 +300,54 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
         }
     } else if (warp >= 4 && !std::is_void_v<X>) {
         if constexpr (!std::is_void_v<X>) {
-            // thread r has row r of P's scales, two words a stage, and block r mod 8 of row r / 8 of Q; one stage ahead
-            const int r = threadIdx.x - 128, qr = r >> 3, qb = r & 7;
-            unsigned w[2] = {}, w_next[2] = {};
-            Raw32<X> x, x_next;
-            auto fetch = [&](unsigned n, int i) {
-                if (n >= mine) return;
-                const long long row = tile_p(n) + r;
-                const int word = (s0 + i) * 2, e0 = (s0 + i) * KSTAGE + qb * 32;
-                w_next[0] = w_next[1] = 0;
+            // thread r has row r of P's scales, two words a stage, and block r mod 8 of row r / 8 of Q; AHEAD stages ahead, as a
+            // stage takes less time than a load
+            constexpr int AHEAD = 4;
+            const int r = threadIdx.x - 128, qr = r >> 3, qb = r & 7, total = (int)mine * steps;
+            unsigned w[AHEAD][2];
+            Raw32<X> x[AHEAD];
+            unsigned fn = 0;
+            int fi = 0;
+            auto fetch = [&](unsigned (&word)[2], Raw32<X> &raw) {
+                if (fn >= mine) return;
+                const long long row = tile_p(fn) + r;
+                const int first = (s0 + fi) * 2, e0 = (s0 + fi) * KSTAGE + qb * 32;
+                word[0] = word[1] = 0;
                 if (row < a.p) {
                     const unsigned *src = reinterpret_cast<const unsigned *>(a.ps + row * a.pitch);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int left = a.blocks - 4 * (word + h);
-                        if (left > 0) w_next[h] = __ldg(src + word + h) & (left < 4 ? (1u << (8 * left)) - 1u : 0xffffffffu);
+                        const int left = a.blocks - 4 * (first + h);
+                        if (left > 0) word[h] = __ldg(src + first + h) & (left < 4 ? (1u << (8 * left)) - 1u : 0xffffffffu);
                     }
                 }
-                x_next.load(static_cast<const X *>(a.x) + qr * a.x_stride + e0, qr < a.q ? a.k - e0 : 0, a.x_vec);
+                raw.load(static_cast<const X *>(a.x) + qr * a.x_stride + e0, qr < a.q ? a.k - e0 : 0, a.x_vec);
+                if (++fi == steps) fi = 0, ++fn;
             };
-            if (steps) fetch(0, 0);
+            if (total)
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) fetch(w[u], x[u]);
             int st = 0, round = 0;
             bool ok = true;
-            for (unsigned n = 0; n < mine && ok; ++n)
-                for (int i = 0; i < steps; ++i) {
-                    w[0] = w_next[0], w[1] = w_next[1];
-                    x = x_next;
-                    fetch(i + 1 < steps ? n : n + 1, i + 1 < steps ? i + 1 : 0);
+            for (int i0 = 0; i0 < total && ok; i0 += AHEAD)
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    if (i0 + u >= total || !ok) break;
                     if (round) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1));
                     if (!ok) break;
                     unsigned char *t = smem + st * Tile::STAGE, *sc = t + Tile::CODES;
                     const int at = (r & 31) * 16 + (r >> 5) * 4;
-                    *reinterpret_cast<unsigned *>(sc + at) = w[0];
-                    *reinterpret_cast<unsigned *>(sc + ROWS * 512 + at) = w[1];
+                    *reinterpret_cast<unsigned *>(sc + at) = w[u][0];
+                    *reinterpret_cast<unsigned *>(sc + ROWS * 512 + at) = w[u][1];
                     unsigned byte;
-                    const uint4 codes = x.quantize(&byte);
+                    const uint4 codes = x[u].quantize(&byte);
                     *reinterpret_cast<uint4 *>(t + PT * KBYTES + qr * 128 + ((qb ^ (qr & 7)) << 4)) = codes;
                     sc[((qb >> 2) * ROWS + 1) * 512 + qr * 16 + (qb & 3)] = (unsigned char)byte;
                     fence_async_smem();
                     __syncwarp();
                     if (lane == 0) arrive(&full[st]);
                     if (++st == a.stages) st = 0, ++round;
+                    fetch(w[u], x[u]);
                 }
             if (!ok && lane == 0) atomicExch(&gave_up, 1);
         }
@@ -829,10 +832,10 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     auto tiles = [&](int b) { return ptiles * ((a.q + b - 1) / b); };
     if (bn < a.q && tiles(192) >= SMS) bn = 192;
     while (bn > 64 && tiles(bn) < SMS) bn /= 2;
-    // and then parts of K, at least two stages each
+    // and then parts of K (two stages each at least), as long as all blocks of the clusters run at once
     const int steps = (in->k + KSTAGE - 1) / KSTAGE;
     int split = 1;
-    while (split < 8 && tiles(bn) * split * 2 <= SMS && steps >= split * 4) split *= 2;
+    while (split < 8 && tiles(bn) * split * 2 <= SMS && steps >= split * 2) split *= 2;
     // whole 128-byte pieces of output rows go by TMA
     a.bulk = !a.swap && split == 1 && a.vec && bn * size >= 128;
     e = matrix_map(&pm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pc, a.p, 16ll * a.blocks, 16ll * a.blocks, PT);
