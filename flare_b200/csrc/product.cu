@@ -12,8 +12,8 @@
 // Warps 0-3 read a finished D from TMEM, a row per thread, round it once and store it through shared memory by TMA, while
 // the next tile goes into the other half of TMEM.  Few tiles and a long K: up to 8 blocks of a cluster take a part of K
 // each and add their tiles through distributed shared memory, in order.
-// A few rows that are not quantised yet (at most 16) are Q as they come: warps 4-7 quantise a stage of them on the way into
-// shared memory, a block of 32 elements per thread, which saves such a call a launch and a matrix.
+// A few rows that are not quantised yet (at most 16) are Q as they come: four times warps 4-7 quantise a stage of them on the way
+// into shared memory, a block of 32 elements per thread, which saves such a call a launch and a matrix.
 // Every wait is bounded; where one ran out the block's tiles are NaN and a bit of the status word is set.
 #include <cuda.h>
 
@@ -48,6 +48,9 @@ struct ProductArgs {
     int x_vec;                    // its rows may be read 16 bytes at a time
 };
 
+// threads of a product whose Q is quantised on the way: a stage takes a warp longer (0.8 us) than its codes need to arrive, so
+// four teams of four warps take the stages in turn
+constexpr int X_TEAMS = 4, X_THREADS = PR_THREADS + 128 * (X_TEAMS - 1);
 constexpr int X_ROWS = FLARE_PRODUCT_ROWS;
 static_assert(X_ROWS * (KSTAGE / 32) == 128, "a block of 32 elements per thread of four warps");
 
@@ -81,19 +84,34 @@ struct Raw32 {
 template <>
 struct Raw32<void> {};
 
+// A matrix descriptor's words: the low one is the address / 16 and a leading offset of 16 bytes, so that tiles, stages and steps of
+// K add to it; the high one is fixed.  One thread issues all products, so its own instructions count (4096 x 4096 x 4096: 57 us
+// with whole descriptors built for each of them, 53.5 us so).
+constexpr uint32_t DESC_ROWS = 64u | (1u << 14) | (2u << 29);  // 8 rows are 1024 bytes, version 1, 128-byte swizzle
+constexpr uint32_t DESC_SCALES = 8u | (1u << 14);              // 8 rows are 128 bytes, version 1, no swizzle
+__device__ __forceinline__ uint32_t desc_low(const void *p) { return (smem_u32(p) >> 4) | (1u << 16); }
+
 // D (+)= A B^T, 64 elements of K; the scales' columns in TMEM, which half of their words in idesc
-__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+        "mov.b64 da, {%1, %7};\n\t"
+        "mov.b64 db, {%2, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %3, [%4], [%5], p;\n\t}\n"
         :
-        : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        : "r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(sa), "r"(sb), "r"(acc), "r"(DESC_ROWS)
         : "memory");
 }
 // 32 rows x 16 bytes of shared memory to 4 columns of TMEM, the same in all four quarters of the lanes
-__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t low) {
+    asm volatile(
+        "{\n\t.reg .b64 d;\n\t"
+        "mov.b64 d, {%1, %2};\n\t"
+        "tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}\n"
+        :
+        : "r"(taddr), "r"(low), "r"(DESC_SCALES)
+        : "memory");
 }
 // instruction descriptor of kind::mxf4: [4,6) scale id of B, [7,10) A and [10,12) B element type (1: e2m1), [17,23) N >> 3,
 // [23] scales are powers of two, [27,29) M >> 7, [29,31) scale id of A
@@ -101,9 +119,6 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(int N, int half) {
     return ((uint32_t)(2 * half) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | (1u << 27) |
            ((uint32_t)(2 * half) << 29);
 }
-// matrix descriptor of a K-major tile of 128-byte rows, 128-byte swizzle: 8 rows are 1024 bytes
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) { return sdesc(saddr, 16, 1024) | (2ull << 61); }
-
 __device__ __forceinline__ void tma_rows(void *dst, const CUtensorMap *map, int x, int y, void *bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
                      smem_u32(dst)),
@@ -200,7 +215,7 @@ __host__ __device__ constexpr int part_of_k(int all, int S) { return S == 1 ? al
 
 // X: the type of a Q that is quantised here, or void
 template <int BN, class O, class X>
-__global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap qmap,
+__global__ void __launch_bounds__(std::is_void_v<X> ? PR_THREADS : X_THREADS) product_kernel(const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap qmap,
                                                              const __grid_constant__ CUtensorMap omap, const ProductArgs a) {
     using Tile = ProductTile<BN>;
     constexpr int ROWS = Tile::ROWS;
@@ -267,6 +282,7 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
         if (lane == 0) {
             int st = 0, round = 0;
             bool ok = true;
+            const uint32_t low0 = desc_low(smem);
             for (unsigned n = 0; n < mine && ok; ++n) {
                 const int buf = a.accs == 2 ? n & 1 : 0;
                 const unsigned use = a.accs == 2 ? n >> 1 : n;  // how often the accumulator was used before
@@ -276,17 +292,16 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
                     ok = mbar_wait(&full[st], round & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t t = smem_u32(smem + st * Tile::STAGE), sc = t + Tile::CODES, scol = scales + st * Tile::SCOLS;
+                    const uint32_t t = low0 + st * (Tile::STAGE / 16), scol = scales + st * Tile::SCOLS;
                     // half h of the stage: the word of P's rows, then those of Q's
 #pragma unroll
-                    for (int b = 0; b < 2 * ROWS; ++b) scales_to_tmem(scol + 4 * b, sdesc(sc + 512 * b, 16, 128));
+                    for (int b = 0; b < 2 * ROWS; ++b) scales_to_tmem(scol + 4 * b, t + Tile::CODES / 16 + 32 * b);
                     const int left = a.k - (s0 + i) * KSTAGE;
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
                         if (m * 64 >= left) break;
                         const uint32_t sa = scol + (m / 2) * 4 * ROWS;
-                        mma_mxf4(d, desc_sw128(t + m * 32), desc_sw128(t + PT * KBYTES + m * 32), idesc_mxf4(BN, m & 1), sa, sa + 4,
-                                 (i | m) != 0);
+                        mma_mxf4(d, t + 2 * m, t + PT * KBYTES / 16 + 2 * m, idesc_mxf4(BN, m & 1), sa, sa + 4, (i | m) != 0);
                     }
                     mma_commit(&empty[st]);
                     if (++st == a.stages) st = 0, ++round;
@@ -300,15 +315,16 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
         }
     } else if (warp >= 4 && !std::is_void_v<X>) {
         if constexpr (!std::is_void_v<X>) {
-            // thread r has row r of P's scales, two words a stage, and block r mod 8 of row r / 8 of Q; AHEAD stages ahead, as a
-            // stage takes less time than a load
-            constexpr int AHEAD = 4;
-            const int r = threadIdx.x - 128, qr = r >> 3, qb = r & 7, total = (int)mine * steps;
+            // thread r of a team has row r of P's scales, two words a stage, and block r mod 8 of row r / 8 of Q
+            constexpr int AHEAD = 2;
+            const int team = warp < 8 ? 0 : 1 + (warp - 10) / 4, r = (warp < 8 ? warp - 4 : (warp - 10) & 3) * 32 + lane;
+            const int qr = r >> 3, qb = r & 7, total = (int)mine * steps;
             unsigned w[AHEAD][2];
             Raw32<X> x[AHEAD];
             unsigned fn = 0;
-            int fi = 0;
+            int fi = team;
             auto fetch = [&](unsigned (&word)[2], Raw32<X> &raw) {
+                while (fi >= steps && fn < mine) fi -= steps, ++fn;
                 if (fn >= mine) return;
                 const long long row = tile_p(fn) + r;
                 const int first = (s0 + fi) * 2, e0 = (s0 + fi) * KSTAGE + qb * 32;
@@ -322,17 +338,18 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
                     }
                 }
                 raw.load(static_cast<const X *>(a.x) + qr * a.x_stride + e0, qr < a.q ? a.k - e0 : 0, a.x_vec);
-                if (++fi == steps) fi = 0, ++fn;
+                fi += X_TEAMS;
             };
             if (total)
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) fetch(w[u], x[u]);
-            int st = 0, round = 0;
+            int st = team, round = 0;
             bool ok = true;
-            for (int i0 = 0; i0 < total && ok; i0 += AHEAD)
+            for (int i0 = team; i0 < total && ok; i0 += AHEAD * X_TEAMS)
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {
-                    if (i0 + u >= total || !ok) break;
+                    if (i0 + u * X_TEAMS >= total || !ok) break;
+                    while (st >= a.stages) st -= a.stages, ++round;
                     if (round) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1));
                     if (!ok) break;
                     unsigned char *t = smem + st * Tile::STAGE, *sc = t + Tile::CODES;
@@ -346,7 +363,7 @@ __global__ void __launch_bounds__(PR_THREADS) product_kernel(const __grid_consta
                     fence_async_smem();
                     __syncwarp();
                     if (lane == 0) arrive(&full[st]);
-                    if (++st == a.stages) st = 0, ++round;
+                    st += X_TEAMS;
                     fetch(w[u], x[u]);
                 }
             if (!ok && lane == 0) atomicExch(&gave_up, 1);
@@ -586,7 +603,8 @@ __global__ void __launch_bounds__(PR_THREADS, NARROW_BLOCKS) product_narrow_kern
     if (warp == 9) {
         if (lane == 0) {
             bool ok = true;
-            for (int h = 0; h < 2; ++h) scales_to_tmem(qscol + 4 * h, sdesc(smem_u32(qscale) + 512 * h, 16, 128));
+            const uint32_t qlow = desc_low(qtile), plow = desc_low(ptile), slow = desc_low(pscale);
+            for (int h = 0; h < 2; ++h) scales_to_tmem(qscol + 4 * h, desc_low(qscale) + 32 * h);
             for (unsigned n = 0; n < mine && ok; ++n) {
                 const int st = n % ST, buf = n % Tile::ACCS;
                 const unsigned use = n / Tile::ACCS;
@@ -594,11 +612,13 @@ __global__ void __launch_bounds__(PR_THREADS, NARROW_BLOCKS) product_narrow_kern
                 if (ok) ok = mbar_wait(&full[st], (n / ST) & 1);
                 if (ok) {
                     tc_fence_after();
-                    const uint32_t t = smem_u32(ptile + st * Tile::P), sc = smem_u32(pscale + st * Tile::PS), scol = pscol + 8 * st;
-                    for (int h = 0; h < 2; ++h) scales_to_tmem(scol + 4 * h, sdesc(sc + 512 * h, 16, 128));
-                    for (int m = 0; m * 64 < a.k; ++m)
-                        mma_mxf4(tmem + buf * BN, desc_sw128(t + m * 32), desc_sw128(smem_u32(qtile) + m * 32), idesc_mxf4(BN, m & 1),
-                                 scol + (m / 2) * 4, qscol + (m / 2) * 4, m != 0);
+                    const uint32_t t = plow + st * (Tile::P / 16), scol = pscol + 8 * st;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) scales_to_tmem(scol + 4 * h, slow + st * (Tile::PS / 16) + 32 * h);
+#pragma unroll
+                    for (int m = 0; m < 4; ++m)
+                        if (m * 64 < a.k)
+                            mma_mxf4(tmem + buf * BN, t + 2 * m, qlow + 2 * m, idesc_mxf4(BN, m & 1), scol + (m / 2) * 4, qscol + (m / 2) * 4, m != 0);
                     mma_commit(&empty[st]);
                 } else {
                     atomicExch(&gave_up, 1);
@@ -757,7 +777,7 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorM
     if (e0) return e0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid, 1, (unsigned)split);
-    cfg.blockDim = dim3(PR_THREADS);
+    cfg.blockDim = dim3(std::is_void_v<X> ? PR_THREADS : X_THREADS);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute attr{};
