@@ -408,7 +408,8 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const Re
     if (a.packed && a.h) clear_rest<T>(a, a.h, a.h_t, a.width);
 }
 
-// smem: what the warps pass, then SHARED: 16 x 32 products per warp
+// smem: what the warps pass, then SHARED: 16 x 32 products per warp.  The states before a span's steps stay in registers: in shared
+// memory, for a third block per multiprocessor, 160k x 16 x 96 f16 takes 316 us instead of 275.
 // DH: whether there is a gradient of every state, not of the last ones alone
 template <class T, class GT, int VE, bool SHARED, bool DH>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(const RecArgs a) {

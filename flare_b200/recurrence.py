@@ -165,7 +165,7 @@ def step(gate, x, state, out=None):
             raise ValueError(f"{name}: tensor must be contiguous")
     gate, x = _dense(gate), _dense(x)
     with _ops.on(dev):
-        h = torch.empty((seqs, width), dtype=x.dtype, device=dev)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
         # one step of `seqs` sequences: the rows are the sequences
         a = _lib.PACK_RECURRENCE.pack(gate.data_ptr(), x.data_ptr(), state.data_ptr(), 0, h.data_ptr(), out.data_ptr(), 0, 0, 0, 0, 0, 0,
                                       0, 0, seqs, 1, gate.stride(0), 0, x.stride(0), 0, width, 0, 0, 0, 0, 0, 0, 0, width,
