@@ -24,7 +24,6 @@ constexpr int SPAN = FLARE_RECURRENCE_SPAN;
 static_assert(SPAN == 16, "shifts by 4");
 constexpr int WARPS = 8;         // warps per block: W along time times WARPS / W tiles of channels
 constexpr int MAX_SPLITS = 128;  // blocks along time
-constexpr int SUM_STRIDE = 33;   // row stride of a warp's 16 x 32 products, off the banks' 32
 
 struct RecArgs {
     const void *gate, *x, *dh, *offsets;
@@ -52,32 +51,36 @@ __device__ __forceinline__ int offset_at(const RecArgs &a, long long s) {
     return (int)min(max(o, 0ll), (long long)a.steps);
 }
 
-// Where a lane's channels lie.  GROUPED: tiles consist of whole groups of channels that share a gate, or of a part of
-// one such group (32 lanes at a time), so that sums over a group need no other warp.
-template <int VE, bool GROUPED>
+// Where a lane's channels lie.  LANES > 0: tiles of LANES lanes consist of whole groups of channels that share a gate, or of
+// a part of one such group, so that sums over a group need no other tile.
+template <int VE, int LANES>
 struct Place {
     bool active;
     int seq, row0, len;  // row0: the sequence's first row (packed), len: its steps
     int c;               // first channel
     unsigned chain;      // seq * width + c
-    int part;            // GROUPED: part of the group
+    int part;            // LANES: part of the group
+    int group, member;   // LANES: group of the tile, place in it
     // lanes without channels of their own (!active) walk along with another's and store nothing
     __device__ __forceinline__ Place(const RecArgs &a, unsigned tile) {
-        const int lane = threadIdx.x & 31;
+        const int lane = threadIdx.x & ((LANES ? LANES : 32) - 1);
         unsigned u;
-        part = 0;
-        if (!GROUPED) {
+        part = group = 0;
+        member = lane;
+        if (!LANES) {
             u = tile * 32 + lane;
             active = u < a.units;
         } else if (a.parts == 1) {
             const unsigned g = a.gunits.div(lane);
-            u = (tile * a.groups_per_tile + g) * a.group_units + lane - g * a.group_units;
+            group = (int)g;
+            member = lane - group * a.group_units;
+            u = (tile * a.groups_per_tile + g) * a.group_units + member;
             active = (int)g < a.groups_per_tile && u < a.units;
             if ((int)g >= a.groups_per_tile) u = (tile * a.groups_per_tile + g) * a.group_units - 1;
         } else {
             const unsigned t = a.fparts.div(tile);
             part = tile - t * a.parts;
-            const int pos = part * 32 + lane;
+            const int pos = part * LANES + lane;
             u = t * a.group_units + min(pos, a.group_units - 1);
             active = pos < a.group_units;
         }
@@ -302,7 +305,7 @@ template <bool BACK, class T, class GT, int VE, bool SHARED>
 __global__ void __launch_bounds__(32 * WARPS) recurrence_split_kernel(const RecArgs a) {
     extern __shared__ __align__(16) float smem[];
     const int W = 1 << a.wlog, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
-    const Place<VE, false> me(a, my_tile(a));
+    const Place<VE, 0> me(a, my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
     Pass<BACK, VE> pass(smem, a.wlog);
@@ -342,7 +345,7 @@ template <class T, class GT, int VE, bool SHARED>
 __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const RecArgs a) {
     extern __shared__ __align__(16) float smem[];
     const int W = 1 << a.wlog, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
-    const Place<VE, false> me(a, my_tile(a));
+    const Place<VE, 0> me(a, my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
     Pass<false, VE> pass(smem, a.wlog);
@@ -408,19 +411,34 @@ __global__ void __launch_bounds__(32 * WARPS) recurrence_forward_kernel(const Re
     if (a.packed && a.h) clear_rest<T>(a, a.h, a.h_t, a.width);
 }
 
-// smem: what the warps pass, then SHARED: 16 x 32 products per warp.  The states before a span's steps stay in registers: in shared
-// memory, for a third block per multiprocessor, 160k x 16 x 96 f16 takes 316 us instead of 275.
+// smem: what the warps pass, then SHARED: 16 x 32 sums of products per warp, a lane's channels each.  The states before a span's
+// steps stay in registers: in shared memory, for a third block per multiprocessor, 160k x 16 x 96 f16 took 15 % longer.
 // DH: whether there is a gradient of every state, not of the last ones alone
-template <class T, class GT, int VE, bool SHARED, bool DH>
+// LANES: lanes of a tile of groups (0: a gate per channel)
+template <class T, class GT, int VE, int LANES, bool DH>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(const RecArgs a) {
     extern __shared__ __align__(16) float smem[];
-    const int W = 1 << a.wlog, lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
-    const Place<VE, SHARED> me(a, my_tile(a));
+    const int W = 1 << a.wlog, w = (threadIdx.x >> 5) & (W - 1), split = blockIdx.y;
+    constexpr bool SHARED = LANES > 0, BLOCK = LANES > 32;
+    const Place<VE, LANES> me(a, BLOCK ? blockIdx.x : my_tile(a));
     int t0, t1;
     me.range(a, split, t0, t1);
     Pass<true, VE> pass(smem, a.wlog);
-    float *sums = smem + (W > 1 ? 2 * WARPS * 32 * VE : 0) + (threadIdx.x >> 5) * (SPAN * SUM_STRIDE);
-    const int round = SPAN << a.wlog, n = (warp_max(t1 - t0) + round - 1) >> (4 + a.wlog);
+    // SHARED, several groups in a tile: where a group's sums of this span go and how many they are
+    __shared__ char *group_at[SHARED ? 32 * WARPS : 1];
+    __shared__ int group_steps[SHARED ? 32 * WARPS : 1], longest;
+    constexpr int STRIDE = LANES + 1;  // of the sums' 16 rows, off the banks' 32
+    const int lane = threadIdx.x & ((BLOCK ? LANES : 32) - 1), first_group = threadIdx.x - lane;
+    float *sums = smem + (W > 1 ? 2 * WARPS * 32 * VE : 0) + (BLOCK ? 0 : (threadIdx.x >> 5) * (SPAN * STRIDE));
+    int most = warp_max(t1 - t0);
+    if (BLOCK && a.packed) {  // the block walks together
+        if (threadIdx.x == 0) longest = 0;
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) atomicMax(&longest, most);
+        __syncthreads();
+        most = longest;
+    }
+    const int round = SPAN << a.wlog, n = (most + round - 1) >> (4 + a.wlog);
     const int gc = (int)a.share.div(me.c);
     const int gs = a.reverse ? -a.gate_t : a.gate_t, xs = a.reverse ? -a.x_t : a.x_t;
     const int dhs = a.reverse ? -a.dh_t : a.dh_t, dxs = a.reverse ? -a.dx_t : a.dx_t, dgs = a.reverse ? -a.dgate_t : a.dgate_t;
@@ -429,6 +447,14 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
     const T *dhp = DH ? static_cast<const T *>(a.dh) + me.first(a, a.dh_s, a.dh_t) + me.c : nullptr;
     T *dxp = static_cast<T *>(a.dx) + me.first(a, a.dx_s, a.dx_t) + me.c;
     GT *dgp = static_cast<GT *>(a.dgate) + me.first(a, a.dgate_s, a.dgate_t) + gc;
+    // SHARED: where the group's sums of step 0 go, and the next step's from there
+    char *sum_at = reinterpret_cast<char *>(dgp);
+    int sum_t = dgs * (int)sizeof(GT);
+    if (SHARED && a.parts > 1) {
+        const long long row = (a.packed ? me.row0 : (long long)me.seq * a.steps) + (a.reverse ? me.len - 1 : 0);
+        sum_at = reinterpret_cast<char *>(a.partial + (me.part * a.rows + row) * a.groups + gc);
+        sum_t = (a.reverse ? -4 : 4) * a.groups;
+    }
     float carry[VE], mu[VE], A[VE], H[VE];
     if (W > 1) pass.begin(a.dlast, me.chain);
     else load_ends<VE>(a.dlast, me.chain, true, carry);
@@ -475,33 +501,8 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
             }
             const bool mine = me.active && (FULL || i < left);
             if (mine) o.store_stream(reinterpret_cast<T *>(px + (long long)dxb * i));
-            if (SHARED) sums[i * SUM_STRIDE + lane] = sum;
+            if (SHARED) sums[i * STRIDE + lane] = sum;
             else if (mine) og.store_stream(reinterpret_cast<GT *>(pg + (long long)dgb * i));
-        }
-        if (SHARED) {
-            // (step, group) sums over the group's lanes in this warp, in the lanes' order
-            __syncwarp();
-            const int units = min(a.group_units - me.part * 32, 32), outs = SPAN * a.groups_per_tile;
-            for (int o = lane; o < (outs + 31) / 32 * 32; o += 32) {
-                const int i = o % SPAN, from = o / SPAN * a.group_units;
-                const int src = min(from, 31);
-                // the group's place, from its first lane
-                const int oleft = __shfl_sync(0xffffffffu, me.active ? left : 0, src), oseq = __shfl_sync(0xffffffffu, me.seq, src);
-                const int orow = __shfl_sync(0xffffffffu, me.row0, src), olen = __shfl_sync(0xffffffffu, me.len, src);
-                const int ogc = __shfl_sync(0xffffffffu, gc, src), ot = __shfl_sync(0xffffffffu, t, src) + i;
-                if (o >= outs || i >= oleft) continue;
-                float sum = 0.0f;
-                for (int l = 0; l < units; ++l) sum += sums[i * SUM_STRIDE + from + l];
-                const int at = a.reverse ? olen - 1 - ot : ot;
-                if (a.parts == 1) {
-                    static_cast<GT *>(a.dgate)[(a.packed ? (long long)orow * a.dgate_t : oseq * a.dgate_s) + (long long)at * a.dgate_t + ogc] =
-                        from_f32<GT>(sum);
-                } else {
-                    const long long row = (a.packed ? orow : (long long)oseq * a.steps) + at;
-                    a.partial[(me.part * a.rows + row) * a.groups + ogc] = sum;
-                }
-            }
-            __syncwarp();
         }
         if (W == 1)
 #pragma unroll
@@ -511,6 +512,31 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_backward_kernel(cons
         const int t = t0 + (n - 1 - k) * round + w * SPAN, left = t1 - t;
         if (__all_sync(0xffffffffu, left >= SPAN)) span(std::true_type{}, t, left);
         else span(std::false_type{}, t, left);
+        if (SHARED) {
+            // (step, group) sums over the group's lanes of this tile, in the lanes' order
+            const bool one = a.groups_per_tile == 1;
+            char *mine = sum_at + (long long)sum_t * t;
+            if (!one && me.member == 0 && me.group < a.groups_per_tile) {
+                group_at[first_group + me.group] = mine;
+                group_steps[first_group + me.group] = me.active ? left : 0;
+            }
+            if (BLOCK) __syncthreads();
+            else __syncwarp();
+            const int units = min(a.group_units - me.part * LANES, LANES), outs = SPAN * a.groups_per_tile;
+            for (int o = lane; o < outs; o += LANES) {
+                const int i = o % SPAN, g = o / SPAN;
+                if (i >= (one ? left : group_steps[first_group + g])) continue;
+                const float *p = sums + i * STRIDE + g * a.group_units;
+                float sum = 0.0f;
+#pragma unroll 4
+                for (int l = 0; l < units; ++l) sum += p[l];
+                char *to = (one ? mine : group_at[first_group + g]) + (long long)sum_t * i;
+                if (a.parts == 1) *reinterpret_cast<GT *>(to) = from_f32<GT>(sum);
+                else *reinterpret_cast<float *>(to) = sum;
+            }
+            if (BLOCK) __syncthreads();
+            else __syncwarp();
+        }
     }
     if (a.dstate && split == 0 && me.active) {
         if (W > 1) pass.finish(a.dstate, me.chain);
@@ -541,7 +567,7 @@ __global__ void recurrence_join_kernel(const RecArgs a) {
 
 struct RecPlan {
     int ve, warps, splits, parts, group_units, groups_per_tile;
-    bool shared;
+    bool shared, block;  // block: a tile is the block's 256 lanes, not a warp's
     long long tiles, rows, agg_bytes, bytes;
 };
 
@@ -581,15 +607,15 @@ RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
     if (backward && p.shared)
         while (p.ve < widest && share / p.ve > 32 && vec_fits(a, 2 * p.ve, backward)) p.ve *= 2;
     p.group_units = p.parts = p.groups_per_tile = 1;
-    if (backward && p.shared) {
+    p.tiles = (chains / p.ve + 31) / 32;
+    auto group_tiles = [&](int lanes) {
         p.group_units = share / p.ve;
-        p.parts = (p.group_units + 31) / 32;
-        p.groups_per_tile = p.parts > 1 ? 1 : 32 / p.group_units;
+        p.parts = (p.group_units + lanes - 1) / lanes;
+        p.groups_per_tile = p.parts > 1 ? 1 : lanes / p.group_units;
         const long long groups = a->seqs * a->groups;
         p.tiles = p.parts > 1 ? groups * p.parts : (groups + p.groups_per_tile - 1) / p.groups_per_tile;
-    } else {
-        p.tiles = (chains / p.ve + 31) / 32;
-    }
+    };
+    if (backward && p.shared) group_tiles(32);
     // time is cut only as far as it takes to fill the machine: W spans at a time, then S blocks
     const long long mean = std::max<long long>(1, a->offsets ? a->steps / std::max<long long>(1, a->seqs) : a->steps);
     const long long spans = (mean + SPAN - 1) / SPAN;
@@ -598,6 +624,10 @@ RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
     // packed sequences are uneven: the longest ones finish last, so each gets several warps if the mean one can use them
     if (a->offsets)
         while (p.warps < WARPS && 2 * p.warps <= spans) p.warps *= 2;
+    // where no warps share a tile, the block is one tile if groups leave lanes of a warp idle: 96 channels are 24 lanes, of which
+    // 10 fit a block and 1 a warp (160k x 16 x 96 f16: 233 us, by warps 280; 30k x 64 x 4 groups of 8 lanes: 201, by warps 181)
+    p.block = backward && p.shared && p.warps == 1 && 32 % p.group_units != 0;
+    if (p.block) group_tiles(32 * WARPS);
     p.splits = 1;
     const long long have = p.tiles * p.warps, want = 24ll * SMS;
     if (p.warps == WARPS && have > 0 && have * 2 <= want) {
@@ -659,9 +689,9 @@ int rec_dispatch(const flare_recurrence_args *in, const RecPlan &p, F f) {
 int run_recurrence(const flare_recurrence_args *in, bool backward, cudaStream_t st) {
     const RecPlan p = rec_plan(in, backward);
     const RecArgs a = rec_args(in, p);
-    const int at_once = WARPS / p.warps;  // tiles per block
+    const int at_once = WARPS / p.warps;  // tiles of warps per block
     // a block is launched for rows of no sequence even where there is no sequence
-    const dim3 grid((unsigned)std::max(1ll, (p.tiles + at_once - 1) / at_once), (unsigned)p.splits);
+    const dim3 grid((unsigned)std::max(1ll, p.block ? p.tiles : (p.tiles + at_once - 1) / at_once), (unsigned)p.splits);
     const size_t buffers = p.warps > 1 ? sizeof(float) * 2 * WARPS * 32 * p.ve : 0;
     rec_dispatch(in, p, [&](auto t, auto gt, auto ve, auto shared) {
         using T = typename decltype(t)::type;
@@ -679,9 +709,15 @@ int run_recurrence(const flare_recurrence_args *in, bool backward, cudaStream_t 
         }
         if constexpr (VE <= widest_backward(sizeof(T) == 4, SH)) {
             if (p.splits > 1) recurrence_split_kernel<true, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
-            const size_t sums = SH ? sizeof(float) * WARPS * SPAN * SUM_STRIDE : 0;
-            if (a.dh) recurrence_backward_kernel<T, GT, VE, SH, true><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
-            else recurrence_backward_kernel<T, GT, VE, SH, false><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
+            const size_t sums = SH ? sizeof(float) * WARPS * SPAN * 33 : 0;
+            auto launch = [&](auto lanes) {
+                constexpr int LANES = decltype(lanes)::value;
+                if (a.dh) recurrence_backward_kernel<T, GT, VE, LANES, true><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
+                else recurrence_backward_kernel<T, GT, VE, LANES, false><<<grid, 32 * WARPS, buffers + sums, st>>>(a);
+            };
+            if constexpr (!SH) launch(std::integral_constant<int, 0>{});
+            else if (p.block) launch(std::integral_constant<int, 32 * WARPS>{});
+            else launch(std::integral_constant<int, 32>{});
             if (p.parts > 1) {
                 const long long n = p.rows * in->groups;
                 recurrence_join_kernel<GT><<<(unsigned)std::min<long long>((n + 255) / 256, 16 * SMS), 256, 0, st>>>(a);

@@ -60,6 +60,7 @@ SHAPES = [
     ("time", 50, 16, 96, 1), ("time", 7, 42, 4, 1), ("time", 3, 100, 64, 64), ("batch", 1, 1000, 32, 32),
     ("batch", 1, 5000, 64, 64), ("batch", 2, 2500, 10, 1), ("batch", 1, 4099, 40, 2), ("time", 4, 300, 70, 1),
     ("batch", 2, 40, 160, 1), ("batch", 2, 40, 321, 1), ("batch", 1, 700, 260, 2), ("batch", 300, 20, 33, 11),
+    ("batch", 2, 20, 1300, 1), ("time", 300, 31, 96, 1), ("batch", 130, 18, 100, 5), ("packed", 300, 2000, 24, 1),
     ("packed", 9, 200, 8, 2), ("packed", 5, 3000, 16, 16), ("packed", 40, 100, 5, 1), ("packed", 3, 9000, 130, 1),
 ]
 
