@@ -222,7 +222,7 @@ int run_lookup(const flare_lookup_args *in, cudaStream_t st) {
 // Per digit of up to 10 bits: count per tile, scan over tiles, scatter.  A tile is 4096 consecutive entries of one block;
 // warp w ranks entries [256 w, 256 w + 256) of it 32 at a time, so ranks follow the entries' order.  Lanes with equal
 // digits find one another by a ballot per bit (match.any took three times the whole kernel's time).  Short lists are
-// sorted by one block in shared memory.
+// sorted by one cluster in shared memory.
 // ------------------------------------------------------------------------------------------------
 constexpr int RS_THREADS = 512, RS_WARPS = RS_THREADS / 32, RS_ROUNDS = 8, RS_TILE = RS_THREADS * RS_ROUNDS;
 constexpr int RS_MAX_BITS = 10, RS_BINS = 1 << RS_MAX_BITS, RS_SMALL_BITS = 8;
@@ -396,19 +396,35 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sort_scatter_kernel(const SortA
     }
 }
 
-// At most RS_SMALL entries: all digits of 8 bits by one block, entries in registers between passes through shared memory (one
-// launch instead of six; with 16383 entries it takes longer than the six, 37 us against 30).  Warp w has entries [32 R w, 32 R (w + 1)), R rounds.
-constexpr int RS_SMALL_THREADS = 1024, RS_SMALL_WARPS = 32, RS_SMALL_ROUNDS = 8, RS_SMALL = RS_SMALL_THREADS * RS_SMALL_ROUNDS;
+// At most RS_SMALL entries: one launch instead of three a digit (16383 entries of 50k rows: 15 us instead of 30; 32768: 23 instead
+// of 30; 65536 would take 40 instead of 31, and 8192 in a single block took 20 where 8 take 11).  The blocks of a cluster hold
+// equal parts of the entries, in registers between passes of 8 bits; counts of digits are read from the other blocks' shared memory, and entries go to their
+// new places by stores into it.  Warp w of block b has entries [32 R (32 b + w), 32 R (32 b + w + 1)), R = 2^a.bits rounds.
+constexpr int RS_SMALL_THREADS = 1024, RS_SMALL_WARPS = 32, RS_SMALL_ROUNDS = 4, RS_SMALL_BLOCKS = 8;
+constexpr int RS_SMALL = RS_SMALL_THREADS * RS_SMALL_ROUNDS * RS_SMALL_BLOCKS;
+static_assert(RS_SMALL <= 65536, "entry numbers of 16 bits");
 
+__device__ __forceinline__ unsigned cluster_address(const void *p, unsigned block) {
+    unsigned at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(block));
+    return at;
+}
+__device__ __forceinline__ void small_sync(bool cluster) {
+    if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
+}
+
+// grid: one cluster of a.tiles blocks
 __global__ void __launch_bounds__(RS_SMALL_THREADS) sort_small_kernel(const SortArgs a) {
     constexpr unsigned BINS = 1u << RS_SMALL_BITS, MASK = BINS - 1;
     extern __shared__ __align__(16) unsigned char raw[];
-    __shared__ unsigned at[BINS], sums[RS_SMALL_WARPS];
-    const int rounds = (int)((a.n + RS_SMALL_THREADS - 1) / RS_SMALL_THREADS), lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    __shared__ unsigned at[BINS], counts[BINS], sums[RS_SMALL_WARPS];
+    const int rounds = 1 << a.bits, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const unsigned block_log = 10 + a.bits, block = blockIdx.x;  // log2 of a block's entries
     unsigned *keys = reinterpret_cast<unsigned *>(raw);
-    unsigned short *nums = reinterpret_cast<unsigned short *>(keys + rounds * RS_SMALL_THREADS);
-    unsigned short *cnt = nums + rounds * RS_SMALL_THREADS;  // (warps, bins)
-    const unsigned base = w * (32 * rounds) + lane;
+    unsigned short *nums = reinterpret_cast<unsigned short *>(keys + (1u << block_log));
+    unsigned short *cnt = nums + (1u << block_log);  // (warps, bins)
+    const unsigned local = w * (32 * rounds) + lane, base = (block << block_log) + local;
     unsigned key[RS_SMALL_ROUNDS];
     unsigned short num[RS_SMALL_ROUNDS], rank[RS_SMALL_ROUNDS];
 #pragma unroll
@@ -453,22 +469,39 @@ __global__ void __launch_bounds__(RS_SMALL_THREADS) sort_small_kernel(const Sort
                 cnt[k * BINS + threadIdx.x] = (unsigned short)count;
                 count += c;
             }
+        unsigned before = 0;  // of this digit in the blocks before this one
+        if (a.tiles > 1) {
+            if (threadIdx.x < BINS) counts[threadIdx.x] = count;
+            small_sync(true);
+            if (threadIdx.x < BINS) {
+                count = 0;
+#pragma unroll
+                for (unsigned b = 0; b < RS_SMALL_BLOCKS; ++b) {
+                    unsigned c = 0;
+                    if (b < a.tiles)
+                        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(cluster_address(counts + threadIdx.x, b)) : "memory");
+                    before += b < block ? c : 0u;
+                    count += c;
+                }
+            }
+        }
         const unsigned digit = block_exclusive<RS_SMALL_WARPS>(count, sums, &all);
-        if (threadIdx.x < BINS) at[threadIdx.x] = digit;
+        if (threadIdx.x < BINS) at[threadIdx.x] = digit + before;
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < RS_SMALL_ROUNDS; ++r) {
             if (r >= rounds || base + r * 32 >= a.n) break;
             const unsigned d = (key[r] >> shift) & MASK, pos = at[d] + mine[d] + rank[r];
-            keys[pos] = key[r];
-            nums[pos] = num[r];
+            const unsigned to = pos >> block_log, slot = pos & ((1u << block_log) - 1);
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_address(keys + slot, to)), "r"(key[r]) : "memory");
+            asm volatile("st.shared::cluster.u16 [%0], %1;" ::"r"(cluster_address(nums + slot, to)), "h"(num[r]) : "memory");
         }
-        __syncthreads();
+        small_sync(a.tiles > 1);
 #pragma unroll
         for (int r = 0; r < RS_SMALL_ROUNDS; ++r)
             if (r < rounds && base + r * 32 < a.n) {
-                key[r] = keys[base + r * 32];
-                num[r] = nums[base + r * 32];
+                key[r] = keys[local + r * 32];
+                num[r] = nums[local + r * 32];
             }
     }
 #pragma unroll
@@ -994,8 +1027,21 @@ int sort_entries(const flare_lookup_grad_args *in, const GradPlan &g, bool dot, 
     if (in->n <= RS_SMALL) {
         const int e = allow_shared_memory<sort_small_kernel>("flare_lookup_backward");
         if (e) return e;
-        const int entries = (int)((in->n + RS_SMALL_THREADS - 1) / RS_SMALL_THREADS) * RS_SMALL_THREADS;
-        sort_small_kernel<<<1, RS_SMALL_THREADS, entries * 6 + RS_SMALL_WARPS * 2 * (1 << RS_SMALL_BITS), st>>>(s);
+        s.tiles = 1;
+        while (s.tiles < RS_SMALL_BLOCKS && (long long)s.tiles * RS_SMALL_THREADS < in->n) s.tiles *= 2;
+        while (((long long)s.tiles * RS_SMALL_THREADS << s.bits) < in->n) ++s.bits;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = s.tiles;
+        cfg.blockDim = RS_SMALL_THREADS;
+        cfg.dynamicSmemBytes = (size_t)((RS_SMALL_THREADS << s.bits) * 6 + RS_SMALL_WARPS * 2 * (1 << RS_SMALL_BITS));
+        cfg.stream = st;
+        cudaLaunchAttribute cluster{};
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = s.tiles;
+        cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+        cfg.attrs = &cluster;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, sort_small_kernel, s);
     } else {
         s.hist = words(g.hist);
         s.total = words(g.total);
