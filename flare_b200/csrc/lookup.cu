@@ -219,12 +219,12 @@ int run_lookup(const flare_lookup_args *in, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------------------
 // Stable radix sort of the entries by row; entries that name no row get key `rows` and end behind all others.
-// Per digit of up to 10 bits: count per tile, scan over tiles, scatter.  A tile is 4096 consecutive entries of one block;
-// warp w ranks entries [256 w, 256 w + 256) of it 32 at a time, so ranks follow the entries' order.  Lanes with equal
+// Per digit of up to 10 bits: count per tile, scan over tiles, scatter.  A tile is 512 R consecutive entries of one block;
+// warp w ranks entries [32 R w, 32 R (w + 1)) of it 32 at a time, so ranks follow the entries' order.  Lanes with equal
 // digits find one another by a ballot per bit (match.any took three times the whole kernel's time).  Short lists are
 // sorted by one cluster in shared memory.
 // ------------------------------------------------------------------------------------------------
-constexpr int RS_THREADS = 512, RS_WARPS = RS_THREADS / 32, RS_ROUNDS = 8, RS_TILE = RS_THREADS * RS_ROUNDS;
+constexpr int RS_THREADS = 512, RS_WARPS = RS_THREADS / 32, RS_MAX_ROUNDS = 9;
 constexpr int RS_MAX_BITS = 10, RS_BINS = 1 << RS_MAX_BITS, RS_SMALL_BITS = 8;
 
 struct SortArgs {
@@ -248,14 +248,15 @@ __device__ __forceinline__ uint2 sort_entry(const SortArgs &a, unsigned i) {
     return a.first ? make_uint2(index_key(a, i), i) : a.in[i];
 }
 
+template <int ROUNDS>
 __global__ void __launch_bounds__(RS_THREADS) sort_count_kernel(const SortArgs a) {
     __shared__ unsigned h[RS_BINS];
     const unsigned bins = 1u << a.bits, mask = bins - 1u;
     for (unsigned b = threadIdx.x; b < bins; b += RS_THREADS) h[b] = 0;
     __syncthreads();
-    const unsigned base = blockIdx.x * RS_TILE;
+    const unsigned base = blockIdx.x * (RS_THREADS * ROUNDS);
 #pragma unroll 8
-    for (int r = 0; r < RS_ROUNDS; ++r) {
+    for (int r = 0; r < ROUNDS; ++r) {
         const unsigned i = base + r * RS_THREADS + threadIdx.x;
         if (i >= a.n) continue;
         const unsigned key = a.first ? index_key(a, i) : __ldg(&a.in[i].x);
@@ -306,26 +307,27 @@ __global__ void __launch_bounds__(RS_THREADS) sort_scan_kernel(const SortArgs a)
     if (threadIdx.x == 0) a.total[blockIdx.x] = carry;
 }
 
-// Ranks of a warp's RS_ROUNDS x 32 entries among those of equal digit; cnt (zeroed) ends as the digits' counts.  All ballots
+// Ranks of a warp's ROUNDS x 32 entries among those of equal digit; cnt (zeroed) ends as the digits' counts.  All ballots
 // come first, as they do not depend on one another; the rounds' counts do.
-__device__ __forceinline__ void warp_ranks(unsigned short *cnt, const uint2 (&e)[RS_ROUNDS], int shift, int bits, unsigned first, unsigned n,
-                                           unsigned short (&rank)[RS_ROUNDS]) {
+template <int ROUNDS>
+__device__ __forceinline__ void warp_ranks(unsigned short *cnt, const uint2 (&e)[ROUNDS], int shift, int bits, unsigned first, unsigned n,
+                                           unsigned short (&rank)[ROUNDS]) {
     const int lane = threadIdx.x & 31;
     const unsigned mask = (1u << bits) - 1u;
-    unsigned same[RS_ROUNDS];
+    unsigned same[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) same[r] = __ballot_sync(0xffffffffu, first + r * 32 < n);
+    for (int r = 0; r < ROUNDS; ++r) same[r] = __ballot_sync(0xffffffffu, first + r * 32 < n);
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) same[r] = first + r * 32 < n ? same[r] : ~same[r];
+    for (int r = 0; r < ROUNDS; ++r) same[r] = first + r * 32 < n ? same[r] : ~same[r];
     for (int b = shift; b < shift + bits; ++b)
 #pragma unroll
-        for (int r = 0; r < RS_ROUNDS; ++r) {
+        for (int r = 0; r < ROUNDS; ++r) {
             const bool one = (e[r].x >> b) & 1u;
             const unsigned ones = __ballot_sync(0xffffffffu, one);
             same[r] &= one ? ones : ~ones;
         }
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) {
+    for (int r = 0; r < ROUNDS; ++r) {
         const bool in = first + r * 32 < n;
         const unsigned d = (e[r].x >> shift) & mask, below = __popc(same[r] & ((1u << lane) - 1u));
         const unsigned before = in ? cnt[d] : 0u;
@@ -336,6 +338,7 @@ __device__ __forceinline__ void warp_ranks(unsigned short *cnt, const uint2 (&e)
     }
 }
 
+template <int ROUNDS>
 __global__ void __launch_bounds__(RS_THREADS, 2) sort_scatter_kernel(const SortArgs a) {
     extern __shared__ __align__(16) unsigned char raw[];
     unsigned *smem = reinterpret_cast<unsigned *>(raw);
@@ -345,11 +348,11 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sort_scatter_kernel(const SortA
     unsigned short *cnt = reinterpret_cast<unsigned short *>(smem + bins); // (warps, bins)
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     for (unsigned b = threadIdx.x; b < bins * RS_WARPS / 2; b += RS_THREADS) smem[bins + b] = 0;
-    const unsigned base = blockIdx.x * RS_TILE + w * (32 * RS_ROUNDS) + lane;
-    uint2 e[RS_ROUNDS];
-    unsigned short rank[RS_ROUNDS];
+    const unsigned base = blockIdx.x * (RS_THREADS * ROUNDS) + w * (32 * ROUNDS) + lane;
+    uint2 e[ROUNDS];
+    unsigned short rank[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) e[r] = base + r * 32 < a.n ? sort_entry(a, base + r * 32) : make_uint2(0, 0);
+    for (int r = 0; r < ROUNDS; ++r) e[r] = base + r * 32 < a.n ? sort_entry(a, base + r * 32) : make_uint2(0, 0);
     constexpr int PER = RS_BINS / RS_THREADS;
     unsigned total[PER], hist[PER];  // asked for early, used after the ranks
 #pragma unroll
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sort_scatter_kernel(const SortA
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) {
+    for (int r = 0; r < ROUNDS; ++r) {
         if (base + r * 32 >= a.n) continue;
         const unsigned d = (e[r].x >> a.shift) & mask;
         const unsigned pos = at[d] + cnt[w * bins + d] + rank[r];
@@ -396,11 +399,12 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sort_scatter_kernel(const SortA
     }
 }
 
-// At most RS_SMALL entries: one launch instead of three a digit (16383 entries of 50k rows: 15 us instead of 30; 32768: 23 instead
-// of 30; 65536 would take 40 instead of 31, and 8192 in a single block took 20 where 8 take 11).  The blocks of a cluster hold
-// equal parts of the entries, in registers between passes of 8 bits; counts of digits are read from the other blocks' shared memory, and entries go to their
-// new places by stores into it.  Warp w of block b has entries [32 R (32 b + w), 32 R (32 b + w + 1)), R = 2^a.bits rounds.
-constexpr int RS_SMALL_THREADS = 1024, RS_SMALL_WARPS = 32, RS_SMALL_ROUNDS = 4, RS_SMALL_BLOCKS = 8;
+// At most RS_SMALL entries: one launch instead of three a digit (16384 entries of 50k rows: 15 us instead of 18, of 1M rows 20
+// instead of 25; 32768 would take 23 instead of 18, and 8192 in a single block took 20 where 8 take 11).  The blocks of a cluster
+// hold equal parts of the entries, in registers between passes of 8 bits; counts of digits are read from the other blocks'
+// shared memory, and entries go to their new places by stores into it.  Warp w of block b has entries [32 R (32 b + w),
+// 32 R (32 b + w + 1)), R = 2^a.bits rounds.
+constexpr int RS_SMALL_THREADS = 1024, RS_SMALL_WARPS = 32, RS_SMALL_ROUNDS = 2, RS_SMALL_BLOCKS = 8;
 constexpr int RS_SMALL = RS_SMALL_THREADS * RS_SMALL_ROUNDS * RS_SMALL_BLOCKS;
 static_assert(RS_SMALL <= 65536, "entry numbers of 16 bits");
 
@@ -979,12 +983,21 @@ __global__ void zero_kernel(float *p, long long n) {
 struct GradPlan {
     long long entries[2], key, val, hist, total, partial, bytes;
     unsigned tiles, range, ranges;
-    int bits, passes;
+    int bits, passes, rounds;
 };
 
 GradPlan grad_plan(long long rows, long long n, int width) {
     GradPlan g{};
-    g.tiles = (unsigned)((n + RS_TILE - 1) / RS_TILE);
+    // A wave of two blocks a multiprocessor takes as long as R + 4 rounds (about 0.9 us each): the tile for which the waves
+    // that n takes are over first (2.56M entries: 9 rounds 108 us, 8 rounds 115; 1.28M: 62 and 73; 40k: 2 rounds 26, 8 rounds 38)
+    long long least = 0;
+    for (int r = 2; r <= RS_MAX_ROUNDS; ++r) {
+        const long long tiles = (n + RS_THREADS * r - 1) / (RS_THREADS * r), time = (tiles + 2 * SMS - 1) / (2 * SMS) * (r + 4);
+        if (r > 2 && time > least) continue;
+        least = time;
+        g.rounds = r;
+        g.tiles = (unsigned)tiles;
+    }
     // ranges of 256 entries, shorter where that leaves multiprocessors without a warp
     g.range = 256;
     const long long col_tiles = (width + 255) / 256;
@@ -1009,6 +1022,13 @@ GradPlan grad_plan(long long rows, long long n, int width) {
     g.partial = take(g.ranges > 1 ? 8ll * g.ranges * width : 0);
     g.bytes = at;
     return g;
+}
+
+template <int R = RS_MAX_ROUNDS, class F>
+void with_rounds(int rounds, F f) {
+    if constexpr (R > 2)
+        if (rounds < R) return with_rounds<R - 1>(rounds, f);
+    f(std::integral_constant<int, R>{});
 }
 
 int sort_entries(const flare_lookup_grad_args *in, const GradPlan &g, bool dot, cudaStream_t st) {
@@ -1052,9 +1072,11 @@ int sort_entries(const flare_lookup_grad_args *in, const GradPlan &g, bool dot, 
             s.in = reinterpret_cast<uint2 *>(ws + g.entries[(p + 1) & 1]);
             s.out = reinterpret_cast<uint2 *>(ws + g.entries[p & 1]);
             const size_t smem = (4 + 2 * RS_WARPS) << s.bits;
-            sort_count_kernel<<<g.tiles, RS_THREADS, 0, st>>>(s);
-            sort_scan_kernel<<<1u << s.bits, RS_THREADS, 0, st>>>(s);
-            sort_scatter_kernel<<<g.tiles, RS_THREADS, smem, st>>>(s);
+            with_rounds(g.rounds, [&](auto rounds) {
+                sort_count_kernel<decltype(rounds)::value><<<g.tiles, RS_THREADS, 0, st>>>(s);
+                sort_scan_kernel<<<1u << s.bits, RS_THREADS, 0, st>>>(s);
+                sort_scatter_kernel<decltype(rounds)::value><<<g.tiles, RS_THREADS, smem, st>>>(s);
+            });
             s.shift += s.bits;
         }
     }
@@ -1235,7 +1257,7 @@ int flare_lookup_backward(const flare_lookup_grad_args *a, void *stream) {
     OPS_CHECK(!a->dweight || is_float_type(a->table_type), "flare_lookup_backward: table type %d has no gradient", a->table_type);
     OPS_CHECK(a->index_type == FLARE_I32 || a->index_type == FLARE_I64, "flare_lookup_backward: unknown index type %d", a->index_type);
     OPS_CHECK(a->n >= 0 && a->rows >= 0 && a->width >= 0, "flare_lookup_backward: negative size");
-    OPS_CHECK(a->rows < 0x7fffffffll && a->n < 0x7fffffffll - RS_TILE, "flare_lookup_backward: %lld rows, %lld entries",
+    OPS_CHECK(a->rows < 0x7fffffffll && a->n < 0x7fffffffll - 8192, "flare_lookup_backward: %lld rows, %lld entries",
               a->rows, a->n);
     OPS_CHECK(a->n == 0 || (a->index && (a->dout || a->width == 0)), "flare_lookup_backward: NULL buffer");
     OPS_CHECK(!a->dweight || a->n == 0 || a->table || a->rows == 0 || a->width == 0, "flare_lookup_backward: dweight needs the table");

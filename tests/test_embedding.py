@@ -117,7 +117,7 @@ def test_lookup_backward(c):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n", [1023, 1025, 4097, 8192, 8193, 16_383, 32_768, 32_769, 100_000])
+@pytest.mark.parametrize("n", [1023, 1025, 4097, 8192, 8193, 16_384, 16_385, 32_769, 100_000, 160_000, 400_000, 700_000])
 def test_lookup_backward_many_equal_entries(n):
     """Rows of 0, 1 and thousands of entries, runs that end inside a chunk: whole numbers sum exactly, so equality."""
     g = torch.Generator().manual_seed(n)
