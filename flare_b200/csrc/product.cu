@@ -5,15 +5,17 @@
 // other its BN columns (Q); where that is B, the tile is stored transposed.  One block per multiprocessor walks over tiles;
 // per 256 elements of K (a stage):
 //   * warp 8 brings the codes, 128 bytes a row, by TMA into 128-byte-swizzled tiles;
-//   * warps 4-7 bring the scales, a word (128 elements of K) per row and half stage, into the order that tcgen05.cp spreads
-//     over TMEM: 32 rows of 16 bytes, row r the words of tile rows r, r + 32, r + 64, r + 96; a thread loads 4 words of a row
-//     at a time and is two such loads ahead (word by word they took 23 of 89 us at 4096 x 4096 x 4096);
-//   * warp 9 copies the scales to TMEM and issues the products; its commit frees the stage.
+//   * warps 4-7 bring the scales: asynchronous copies of 16 bytes a row (two stages) into a ring, three such groups ahead, from
+//     which each warp stores the words of tile rows l, l + 32, l + 64, l + 96 to lane l of its quarter of TMEM.  (tcgen05.cp from
+//     shared memory takes 80 cycles of the tensor pipe for each of six pieces a stage, whose products take 384: 54 us at
+//     4096 x 4096 x 4096, where this takes 44; scales through registers were waited for, 52; scales never fetched would be 39.)
+//   * warp 9 issues the products; its commit frees the stage.
 // Warps 0-3 read a finished D from TMEM, a row per thread, round it once and store it through shared memory by TMA, while
 // the next tile goes into the other half of TMEM.  Few tiles and a long K: up to 8 blocks of a cluster take a part of K
 // each and add their tiles through distributed shared memory, in order.
 // A few rows that are not quantised yet (at most 16) are Q as they come: four times warps 4-7 quantise a stage of them on the way
-// into shared memory, a block of 32 elements per thread, which saves such a call a launch and a matrix.
+// into shared memory, a block of 32 elements per thread, which saves such a call a launch and a matrix.  Scales then lie there
+// too, 32 rows of 16 bytes, row r the words of tile rows r, r + 32, r + 64, r + 96, and warp 9 spreads them over TMEM.
 // Every wait is bounded; where one ran out the block's tiles are NaN and a bit of the status word is set.
 #include <cuda.h>
 
@@ -113,6 +115,23 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t low) {
         : "r"(taddr), "r"(low), "r"(DESC_SCALES)
         : "memory");
 }
+// N pieces of 4 words a lane to 4 N columns of this warp's quarter of the lanes
+template <int N>
+__device__ __forceinline__ void words_to_tmem(uint32_t taddr, const uint4 *v) {
+    if constexpr (N >= 4) {
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+                         taddr),
+                     "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w), "r"(v[2].x),
+                     "r"(v[2].y), "r"(v[2].z), "r"(v[2].w), "r"(v[3].x), "r"(v[3].y), "r"(v[3].z), "r"(v[3].w)
+                     : "memory");
+        if constexpr (N > 4) words_to_tmem<N - 4>(taddr + 16, v + 4);
+    } else {
+        static_assert(N == 2, "4 or 6 pieces");
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0].x), "r"(v[0].y),
+                     "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w)
+                     : "memory");
+    }
+}
 // instruction descriptor of kind::mxf4: [4,6) scale id of B, [7,10) A and [10,12) B element type (1: e2m1), [17,23) N >> 3,
 // [23] scales are powers of two, [27,29) M >> 7, [29,31) scale id of A
 __host__ __device__ constexpr uint32_t idesc_mxf4(int N, int half) {
@@ -149,15 +168,17 @@ __device__ __forceinline__ float remote_f32(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-template <int BN>
+// PLAIN: both matrices are quantised already
+template <int BN, bool PLAIN>
 struct ProductTile {
     static constexpr int QBLOCKS = (BN + 127) / 128;                      // 128-row pieces of Q's scales
     static constexpr int ROWS = 1 + QBLOCKS;                              // scale rows per thread
     static constexpr int CODES = (PT + BN) * KBYTES;                      // bytes of codes per stage
-    static constexpr int SCALES = 2 * 512 * ROWS;                         // bytes of scales per stage
+    static constexpr int SCALES = PLAIN ? 0 : 2 * 512 * ROWS;             // bytes of scales per stage
+    static constexpr int AHEAD = 4, GROUP = PLAIN ? 128 * 16 * ROWS : 0;  // PLAIN: 16 bytes of scales per row, for two stages
     static constexpr int STAGE = CODES + SCALES;                          // a multiple of 1024
     static constexpr int SCOLS = 2 * 4 * ROWS;                            // TMEM columns of a stage's scales
-    static constexpr int FIT = (SMEM_MAX - SMEM_FIXED - 4 * OUT_BYTES) / STAGE;
+    static constexpr int FIT = (SMEM_MAX - SMEM_FIXED - 4 * OUT_BYTES - AHEAD * GROUP) / STAGE;
     static constexpr int MAX_STAGES = FIT > 8 ? 8 : FIT;
     static_assert(STAGE % 1024 == 0, "tiles start on swizzle atoms");
     static_assert(2 * BN + MAX_STAGES * SCOLS <= TMEM_COLS, "two accumulators and the scales fit TMEM");
@@ -217,7 +238,7 @@ __host__ __device__ constexpr int part_of_k(int all, int S) { return S == 1 ? al
 template <int BN, class O, class X>
 __global__ void __launch_bounds__(std::is_void_v<X> ? PR_THREADS : X_THREADS) product_kernel(const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap qmap,
                                                              const __grid_constant__ CUtensorMap omap, const ProductArgs a) {
-    using Tile = ProductTile<BN>;
+    using Tile = ProductTile<BN, std::is_void_v<X>>;
     constexpr int ROWS = Tile::ROWS;
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ uint32_t tmem_slot;
@@ -294,8 +315,9 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? PR_THREADS : X_THREADS) pr
                     tc_fence_after();
                     const uint32_t t = low0 + st * (Tile::STAGE / 16), scol = scales + st * Tile::SCOLS;
                     // half h of the stage: the word of P's rows, then those of Q's
+                    if constexpr (!std::is_void_v<X>)
 #pragma unroll
-                    for (int b = 0; b < 2 * ROWS; ++b) scales_to_tmem(scol + 4 * b, t + Tile::CODES / 16 + 32 * b);
+                        for (int b = 0; b < 2 * ROWS; ++b) scales_to_tmem(scol + 4 * b, t + Tile::CODES / 16 + 32 * b);
                     const int left = a.k - (s0 + i) * KSTAGE;
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
@@ -369,68 +391,93 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? PR_THREADS : X_THREADS) pr
             if (!ok && lane == 0) atomicExch(&gave_up, 1);
         }
     } else if (warp >= 4) {
-        // thread r has row r of P and rows r, r + 128 of Q, 4 words (2 stages) at a time: groups (tile, pair of stages), two ahead
+        // thread r copies the scales of row r of P and rows r, r + 128 of Q, 4 words (2 stages) at a time: groups (tile, pair of
+        // stages), in a ring of AHEAD.  Lane l of each warp then has the words of rows l + 32 j, which are columns j of its quarter.
+        constexpr int AHEAD = Tile::AHEAD;
         const int r = threadIdx.x - 128, pairs = (steps + 1) / 2, words = a.pitch / 4;
         const unsigned groups = mine * (unsigned)pairs;
-        unsigned ftile = 0;
+        unsigned char *ring = outs + 4 * OUT_BYTES;
+        unsigned ftile = 0, fgroup = 0;
         int fpair = 0;
-        auto fetch = [&](uint4 (&v)[ROWS]) {
+        const unsigned *src[ROWS];  // of the tile being fetched
+        bool some[ROWS];
+        auto fetch = [&] {
+            if (fgroup < groups) {
+                if (fpair == 0) {
+                    const long long p0 = tile_p(ftile), q0 = tile_q(ftile);
 #pragma unroll
-            for (int b = 0; b < ROWS; ++b) v[b] = make_uint4(0, 0, 0, 0);
-            if (ftile >= mine) return;
-            const int w = (s0 + 2 * fpair) * 2;
-#pragma unroll
-            for (int b = 0; b < ROWS; ++b) {
-                const int o = b ? (b - 1) * 128 + r : r;
-                const long long row = b ? tile_q(ftile) + o : tile_p(ftile) + o;
-                if (row >= (b ? a.q : a.p) || (b && o >= BN)) continue;
-                const unsigned *src = reinterpret_cast<const unsigned *>((b ? a.qs : a.ps) + row * a.pitch) + w;
-                if (a.wide) {
-                    v[b] = __ldg(reinterpret_cast<const uint4 *>(src));
-                } else {
-                    v[b].x = __ldg(src);
-                    if (w + 1 < words) v[b].y = __ldg(src + 1);
-                    if (w + 2 < words) v[b].z = __ldg(src + 2);
-                    if (w + 3 < words) v[b].w = __ldg(src + 3);
+                    for (int b = 0; b < ROWS; ++b) {
+                        const int o = b ? (b - 1) * 128 + r : r;
+                        const long long row = (b ? q0 : p0) + o;
+                        some[b] = row < (b ? a.q : a.p) && (!b || o < BN);
+                        src[b] = reinterpret_cast<const unsigned *>((b ? a.qs : a.ps) + (some[b] ? row * a.pitch : 0)) + s0 * 2;
+                    }
                 }
+                const int left = words - (s0 * 2 + 4 * fpair);  // of the row, at least 1
+                const uint32_t to = smem_u32(ring) + (fgroup % AHEAD) * Tile::GROUP + r * 16;
+#pragma unroll
+                for (int b = 0; b < ROWS; ++b) {
+                    if (a.wide) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + b * 2048), "l"(src[b]), "r"(some[b] ? 16 : 0)
+                                     : "memory");
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const bool in = some[b] && w < left;
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + b * 2048 + w * 4), "l"(src[b] + (in ? w : 0)),
+                                         "r"(in ? 4 : 0)
+                                         : "memory");
+                        }
+                    }
+                    src[b] += 4;
+                }
+                if (++fpair == pairs) fpair = 0, ++ftile;
             }
-            if (++fpair == pairs) fpair = 0, ++ftile;
+            ++fgroup;
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        uint4 next[2][ROWS];
-        if (pairs) {
-            fetch(next[0]);
-            fetch(next[1]);
-        }
+#pragma unroll
+        for (int u = 0; u < AHEAD - 1; ++u) fetch();
         int st = 0, round = 0, pair = 0;
         bool ok = true;
-        const int at = (r & 31) * 4 + (r >> 5);
-        for (unsigned g = 0; g < groups && ok; ++g) {
-            uint4 cur[ROWS];
+        const uint32_t quarter = scales + ((uint32_t)((warp & 3) * 32) << 16);
+        // a warp whose wait ran out still meets the others at every barrier
+        for (unsigned g = 0; g < groups; ++g) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 2) : "memory");
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            fetch();  // into the place that all four warps have read
+            const uint4 *from = reinterpret_cast<const uint4 *>(ring + (g % AHEAD) * Tile::GROUP) + lane;
+            uint4 v[ROWS][4];
 #pragma unroll
-            for (int b = 0; b < ROWS; ++b) {
-                cur[b] = next[0][b];
-                next[0][b] = next[1][b];
-            }
-            fetch(next[1]);
+            for (int b = 0; b < ROWS; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[b][j] = from[b * 128 + j * 32];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int i = 2 * pair + h;
                 if (i >= steps) break;
-                if (round) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1));
-                if (!ok) break;
-                unsigned *sc = reinterpret_cast<unsigned *>(smem + st * Tile::STAGE + Tile::CODES);
-                // bytes past the last block are not scales
-                const int left = a.blocks - (s0 + i) * 8;
-                const unsigned lo = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
-                const unsigned hi = left >= 8 ? 0xffffffffu : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u;
+                if (round && ok) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1));
+                if (ok) {
+                    tc_fence_after();
+                    // bytes past the last block are not scales
+                    const int left = a.blocks - (s0 + i) * 8;
+                    const unsigned lo = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+                    const unsigned hi = left >= 8 ? 0xffffffffu : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u;
+                    uint4 piece[2 * ROWS];
 #pragma unroll
-                for (int b = 0; b < ROWS; ++b) {
-                    sc[b * 128 + at] = (h ? cur[b].z : cur[b].x) & lo;
-                    sc[(ROWS + b) * 128 + at] = (h ? cur[b].w : cur[b].y) & hi;
+                    for (int b = 0; b < ROWS; ++b) {
+                        const uint4 *x = v[b];
+                        piece[b] = h ? make_uint4(x[0].z & lo, x[1].z & lo, x[2].z & lo, x[3].z & lo)
+                                     : make_uint4(x[0].x & lo, x[1].x & lo, x[2].x & lo, x[3].x & lo);
+                        piece[ROWS + b] = h ? make_uint4(x[0].w & hi, x[1].w & hi, x[2].w & hi, x[3].w & hi)
+                                            : make_uint4(x[0].y & hi, x[1].y & hi, x[2].y & hi, x[3].y & hi);
+                    }
+                    words_to_tmem<2 * ROWS>(quarter + st * Tile::SCOLS, piece);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(&full[st]);
                 }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) arrive(&full[st]);
                 if (++st == a.stages) st = 0, ++round;
             }
             if (++pair == pairs) pair = 0;
@@ -758,7 +805,7 @@ int matrix_map(CUtensorMap *map, CUtensorMapDataType type, int size, const void 
 
 template <int BN, class O, class X>
 int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorMap &om, ProductArgs a, int split, cudaStream_t st) {
-    using Tile = ProductTile<BN>;
+    using Tile = ProductTile<BN, std::is_void_v<X>>;
     const int per = part_of_k((a.k + KSTAGE - 1) / KSTAGE, split);
     a.ptiles = (unsigned)((a.p + PT - 1) / PT);
     const long long tiles = (long long)a.ptiles * ((a.q + BN - 1) / BN);
@@ -771,7 +818,7 @@ int launch_product(const CUtensorMap &pm, const CUtensorMap &qm, const CUtensorM
     a.accs = grid < a.tiles ? 2 : 1;
     // no more stages than the block's tiles have
     a.stages = (int)std::min<long long>(Tile::MAX_STAGES, per * ((tiles + grid - 1) / grid));
-    int smem = a.stages * Tile::STAGE + 4 * OUT_BYTES + 1024;
+    int smem = a.stages * Tile::STAGE + 4 * OUT_BYTES + Tile::AHEAD * Tile::GROUP + 1024;
     if (split > 1) smem = std::max(smem, PT * BN * 4 + 1024);
     const int e0 = allow_shared_memory<product_kernel<BN, O, X>>("flare_micro_product");
     if (e0) return e0;
