@@ -91,8 +91,8 @@ def quantize(x) -> Micro4:
 def product(x, w: Micro4, dtype=torch.bfloat16, check=False):
     """x (m, k) times the transpose of w (n, k): a new (m, n) tensor of f32, f16 or bf16, accumulated in 32 bits.
 
-    x: a `Micro4`, or an f32, f16 or bf16 tensor that is quantized first (up to 16 rows inside the product).  check: wait for the product and raise FlareError if a wait
-    inside the kernel ran out (without it such a tile is NaN).
+    x: a `Micro4`, or an f32, f16 or bf16 tensor that is quantized first (up to 16 rows inside the product).  check: wait for
+    the product and raise FlareError if a wait inside the kernel ran out (without it such a tile is NaN).
     """
     lib = _lib.load()
     if not isinstance(w, Micro4):

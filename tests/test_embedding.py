@@ -131,6 +131,16 @@ def test_lookup_backward_many_equal_entries(n):
 
 
 @pytest.mark.gpu
+def test_rows_of_no_columns():
+    idx = torch.tensor([[0, 2], [-1, 1]], device=DEV)
+    table, w = torch.zeros(3, 0, device=DEV), torch.ones(2, 2, device=DEV)
+    out = embedding.lookup(table, idx, w)
+    assert out.shape == (2, 2, 0)
+    dt, dw = embedding.lookup_backward(out, table, idx, w)
+    assert dt.shape == (3, 0) and torch.equal(dw, torch.zeros_like(w))
+
+
+@pytest.mark.gpu
 def test_gradient_agrees_with_differences():
     t, idx, w = _case(rows=6, width=5, n=20, table=F32)
     g = torch.Generator().manual_seed(2)

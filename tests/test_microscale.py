@@ -127,6 +127,19 @@ def test_product_of_whole_numbers_is_exact():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(2500, 2401, 600), (2333, 2600, 1000), (300, 20_000, 4096), (3001, 2000, 2049)])
+def test_product_of_many_wide_tiles_is_exact(m, n, k):
+    """Tiles of 192 columns, several per block, scale rows of whole 16 bytes and not: small whole numbers, so equality."""
+    g = torch.Generator().manual_seed(m)
+    a, b = (torch.randint(-1, 2, (r, k), generator=g).float() for r in (m, n))
+    for t in (a, b):
+        t[:, ::32] = 4.0  # every block's scale is 1 ...
+        t *= 2.0 ** torch.randint(0, 3, (t.shape[0], (k + 31) // 32), generator=g).repeat_interleave(32, 1)[:, :k]  # ... or 2 or 4
+    got = microscale.product(microscale.quantize(a.to(DEV)), microscale.quantize(b.to(DEV)), dtype=F32, check=True)
+    assert torch.equal(got.cpu(), a @ b.T)  # sums below 2^24
+
+
+@pytest.mark.gpu
 def test_product_of_a_tensor_quantizes_it():
     g = torch.Generator().manual_seed(3)
     x, w = torch.randn(50, 70, generator=g).to(DEV).half(), microscale.quantize(torch.randn(30, 70, generator=g).to(DEV))
