@@ -75,6 +75,11 @@ struct Vec {
 #pragma unroll
         for (int i = 0; i < R::N; ++i) raw[i] = __ldg(reinterpret_cast<const typename R::type *>(p) + i);
     }
+    // for memory that this kernel writes too, after reading it
+    __device__ __forceinline__ void load_plain(const T *p) {
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) raw[i] = *(reinterpret_cast<const typename R::type *>(p) + i);
+    }
     // read once: no line is kept for it
     __device__ __forceinline__ void load_stream(const T *p) {
 #pragma unroll
@@ -100,6 +105,12 @@ struct Vec {
 inline bool fits_vec(const void *p, long long stride, int size, int n) {
     const int bytes = n * size < 16 ? n * size : 16;
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride % n == 0;
+}
+
+// Whether two stretches of memory share a byte.
+inline bool overlaps(const void *p, long long p_bytes, const void *q, long long q_bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return p && q && p_bytes > 0 && q_bytes > 0 && a < b + (uintptr_t)q_bytes && b < a + (uintptr_t)p_bytes;
 }
 
 // 2^(byte - 127); byte 255 stands for NaN

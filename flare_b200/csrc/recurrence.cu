@@ -267,10 +267,11 @@ __device__ __forceinline__ void fold_splits(const RecArgs &a, unsigned chain, in
     pass.run(A, H, unused);
 }
 
+// plain loads: `last` may be `state` and `dstate` may be `dlast`, each written by the lanes that have read it
 template <int VE>
 __device__ __forceinline__ void load_ends(const float *p, unsigned chain, bool some, float (&f)[VE]) {
     Vec<float, VE> v;
-    if (p && some) v.load(p + chain);
+    if (p && some) v.load_plain(p + chain);
     else v.zero();
 #pragma unroll
     for (int e = 0; e < VE; ++e) f[e] = v.get(e);
@@ -568,8 +569,14 @@ __global__ void recurrence_join_kernel(const RecArgs a) {
 struct RecPlan {
     int ve, warps, splits, parts, group_units, groups_per_tile;
     bool shared, block;  // block: a tile is the block's 256 lanes, not a warp's
-    long long tiles, rows, agg_bytes, bytes;
+    long long tiles, rows, agg_bytes, ends_bytes, bytes;
 };
+
+// The ends that a call reads (state, or dlast), if it writes the new ones in their place.
+const float *ends_in_place(const flare_recurrence_args *a, bool backward) {
+    const float *in = backward ? a->dlast : a->state, *out = backward ? a->dstate : a->last;
+    return a->seqs && in == out ? in : nullptr;
+}
 
 // Vectors of `ve` channels: whole within a group of channels that share a gate, aligned in every tensor.
 bool vec_fits(const flare_recurrence_args *a, int ve, bool backward) {
@@ -635,7 +642,10 @@ RecPlan rec_plan(const flare_recurrence_args *a, bool backward) {
         p.splits = (int)std::max(1ll, std::min({want / have, rounds, (long long)MAX_SPLITS}));
     }
     p.agg_bytes = p.splits > 1 ? (8ll * p.splits * chains + 15) / 16 * 16 : 0;
-    p.bytes = p.agg_bytes + (p.parts > 1 ? 4ll * p.parts * p.rows * a->groups : 0);
+    // blocks that share a sequence all start from its state, and one of them writes the new one at a time of its own: where that
+    // takes the old one's place they start from a copy
+    p.ends_bytes = p.splits > 1 && ends_in_place(a, backward) ? (4 * chains + 15) / 16 * 16 : 0;
+    p.bytes = p.agg_bytes + p.ends_bytes + (p.parts > 1 ? 4ll * p.parts * p.rows * a->groups : 0);
     return p;
 }
 
@@ -646,7 +656,7 @@ RecArgs rec_args(const flare_recurrence_args *in, const RecPlan &p) {
     a.h = in->h, a.dgate = in->dgate, a.dx = in->dx;
     a.last = in->last, a.saved = in->saved, a.dstate = in->dstate;
     a.agg = static_cast<float *>(in->workspace);
-    a.partial = reinterpret_cast<float *>(static_cast<char *>(in->workspace) + p.agg_bytes);
+    a.partial = reinterpret_cast<float *>(static_cast<char *>(in->workspace) + p.agg_bytes + p.ends_bytes);
     a.seqs = in->seqs, a.steps = (int)in->steps, a.rows = p.rows;
     a.gate_s = in->gate_s, a.x_s = in->x_s, a.h_s = in->h_s, a.dh_s = in->dh_s, a.dgate_s = in->dgate_s, a.dx_s = in->dx_s;
     a.gate_t = (int)in->gate_t, a.x_t = (int)in->x_t, a.h_t = (int)in->h_t;
@@ -688,7 +698,17 @@ int rec_dispatch(const flare_recurrence_args *in, const RecPlan &p, F f) {
 
 int run_recurrence(const flare_recurrence_args *in, bool backward, cudaStream_t st) {
     const RecPlan p = rec_plan(in, backward);
-    const RecArgs a = rec_args(in, p);
+    RecArgs a = rec_args(in, p);
+    if (p.ends_bytes) {
+        float *copy = reinterpret_cast<float *>(static_cast<char *>(in->workspace) + p.agg_bytes);
+        const cudaError_t e = cudaMemcpyAsync(copy, ends_in_place(in, backward), sizeof(float) * (size_t)(in->seqs * in->width),
+                                              cudaMemcpyDeviceToDevice, st);
+        if (e != cudaSuccess) {
+            set_error("%s: %s", backward ? "flare_recurrence_backward" : "flare_recurrence_forward", cudaGetErrorString(e));
+            return FLARE_E_CUDA;
+        }
+        (backward ? a.dlast : a.state) = copy;
+    }
     const int at_once = WARPS / p.warps;  // tiles of warps per block
     // a block is launched for rows of no sequence even where there is no sequence
     const dim3 grid((unsigned)std::max(1ll, p.block ? p.tiles : (p.tiles + at_once - 1) / at_once), (unsigned)p.splits);
@@ -744,9 +764,12 @@ int rec_check(const flare_recurrence_args *a, bool backward, const char *what) {
     OPS_CHECK(a->offsets_type == FLARE_I32 || a->offsets_type == FLARE_I64, "%s: unknown offsets type %d", what, a->offsets_type);
     const bool some = a->seqs > 0, data = (some || a->offsets) && a->steps > 0;
     OPS_CHECK(!data || (a->gate && a->x), "%s: NULL gate or x", what);
+    const long long ends = 4 * a->seqs * a->width;
     if (!backward) {
         OPS_CHECK(!some || a->last, "%s: NULL last", what);
+        OPS_CHECK(a->last == a->state || !overlaps(a->last, ends, a->state, ends), "%s: last overlaps state", what);
     } else {
+        OPS_CHECK(a->dstate == a->dlast || !overlaps(a->dstate, ends, a->dlast, ends), "%s: dstate overlaps dlast", what);
         const bool spans = some && a->steps > SPAN;
         OPS_CHECK(!data || (a->dgate && a->dx), "%s: NULL gradient", what);
         OPS_CHECK(!spans || a->saved, "%s: NULL saved", what);

@@ -274,3 +274,50 @@ def test_c_entry_refuses_bad_arguments():
             assert fn(ctypes.byref(a), None) == 1 and why in lib.flare_last_error(), why
         assert fn(ctypes.byref(A(width=4, groups=4, seqs=0, steps=5)), None) == 0
     assert lib.flare_recurrence_saved(3, 16, 4, 0) == 0 and lib.flare_recurrence_saved(3, 17, 4, 0) == 12
+
+
+def _dense_args(gate, x, **more):
+    B, T, D = x.shape
+    return _lib.RecurrenceArgs(gate=gate.data_ptr(), x=x.data_ptr(), seqs=B, steps=T, gate_s=gate.stride(0), gate_t=gate.stride(1),
+                               x_s=T * D, x_t=D, h_s=T * D, h_t=D, dh_s=T * D, dh_t=D, dgate_s=gate.stride(0), dgate_t=gate.stride(1),
+                               dx_s=T * D, dx_t=D, width=D, groups=gate.shape[2], **more)
+
+
+def test_c_entry_takes_a_copy_of_a_state_kept_in_place():
+    """Blocks that share a sequence all read its state, one writes the new one: in place they need room for a copy."""
+    lib = _lib.load()
+    x, gate, ends = torch.zeros(1, 5000, 64), torch.zeros(1, 5000, 64), torch.zeros(3, 64)
+    p = [t.data_ptr() for t in ends]
+    for backward, (old, new) in ((0, ("state", "last")), (1, ("dlast", "dstate"))):
+        apart = lib.flare_recurrence_workspace(ctypes.byref(_dense_args(gate, x, **{old: p[0], new: p[1]})), backward)
+        place = lib.flare_recurrence_workspace(ctypes.byref(_dense_args(gate, x, **{old: p[0], new: p[0]})), backward)
+        assert apart > 0 and place == apart + 4 * 64
+        fn = lib.flare_recurrence_backward if backward else lib.flare_recurrence_forward
+        for part in (p[0] + 64, p[0] - 4):
+            a = _dense_args(gate, x, **{old: p[0], new: part})
+            a.dgate = a.dx = a.saved = 16
+            assert fn(ctypes.byref(a), None) == 1 and f"{new} overlaps {old}".encode() in lib.flare_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 5000, 64, 64), (1, 5000, 64, 1), (3, 40, 33, 11), (2, 9, 96, 1)], ids=str)
+def test_c_entry_keeps_a_state_in_place(shape):
+    B, T, D, G = shape
+    lib = _lib.load()
+    c = _case("batch", *shape)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def call(fn, backward, **more):
+        a = _dense_args(c["gate"], c["x"], **{k: v.data_ptr() for k, v in more.items()})
+        ws = torch.empty(max(16, lib.flare_recurrence_workspace(ctypes.byref(a), backward)), dtype=torch.uint8, device=DEV)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(fn(ctypes.byref(a), stream), "recurrence")
+
+    h, last, saved = recurrence.scan(c["gate"], c["x"], c["state"], training=True)
+    want = recurrence.scan_backward(c["gate"], c["x"], saved, c["dh"], c["dlast"], c["state"])
+    h2, saved2, state = torch.empty_like(h), torch.empty_like(saved), c["state"].clone()
+    call(lib.flare_recurrence_forward, 0, state=state, last=state, h=h2, saved=saved2)
+    assert torch.equal(h2, h) and torch.equal(state, last) and torch.equal(saved2, saved)
+    dg, dx, ends = torch.empty_like(c["gate"]), torch.empty_like(c["x"]), c["dlast"].clone()
+    call(lib.flare_recurrence_backward, 1, state=c["state"], saved=saved, dh=c["dh"], dlast=ends, dstate=ends, dgate=dg, dx=dx)
+    assert torch.equal(dg, want[0]) and torch.equal(dx, want[1]) and torch.equal(ends, want[2])
