@@ -101,11 +101,12 @@ class RecurrenceArgs(ctypes.Structure):
 
 RECURRENCE_SPAN = 16
 PRODUCT_ROWS = 16
-# The operators' calls are short, so their argument structs are packed in one go: the same members as above.
-PACK_LOOKUP = struct.Struct("@5P4q4if")
-PACK_LOOKUP_GRAD = struct.Struct("@7P5q4if")
-PACK_RECURRENCE = struct.Struct("@13P15q6i")
-PACK_PRODUCT = struct.Struct("@8P5q3i")
+# The operators' calls are short, so their argument structs are packed in one go: the same members as above,
+# and 0q for the padding at the struct's end.
+PACK_LOOKUP = struct.Struct("@5P4q4if0q")
+PACK_LOOKUP_GRAD = struct.Struct("@7P5q4if0q")
+PACK_RECURRENCE = struct.Struct("@13P15q6i0q")
+PACK_PRODUCT = struct.Struct("@8P5q3i0q")
 
 
 class ProductArgs(ctypes.Structure):

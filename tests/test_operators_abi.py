@@ -43,3 +43,10 @@ def test_packed_arguments_have_the_structs_layout():
         a = cls.from_buffer_copy(raw.ljust(ctypes.sizeof(cls), b"\0"))
         got = [getattr(a, name) for name, _ in cls._fields_]
         assert got == list(range(1, n + 1)) and ctypes.sizeof(cls) - len(raw) < 8
+
+
+def test_packed_arguments_are_as_long_as_the_structs():
+    """The library may copy a whole struct, so its padding has to be there."""
+    for pack, cls in ((_lib.PACK_LOOKUP, _lib.LookupArgs), (_lib.PACK_LOOKUP_GRAD, _lib.LookupGradArgs),
+                      (_lib.PACK_RECURRENCE, _lib.RecurrenceArgs), (_lib.PACK_PRODUCT, _lib.ProductArgs)):
+        assert pack.size == ctypes.sizeof(cls), cls.__name__
