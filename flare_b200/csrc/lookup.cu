@@ -1257,7 +1257,7 @@ int flare_lookup_backward(const flare_lookup_grad_args *a, void *stream) {
     OPS_CHECK(!a->dweight || is_float_type(a->table_type), "flare_lookup_backward: table type %d has no gradient", a->table_type);
     OPS_CHECK(a->index_type == FLARE_I32 || a->index_type == FLARE_I64, "flare_lookup_backward: unknown index type %d", a->index_type);
     OPS_CHECK(a->n >= 0 && a->rows >= 0 && a->width >= 0, "flare_lookup_backward: negative size");
-    OPS_CHECK(a->rows < 0x7fffffffll && a->n < 0x7fffffffll - 8192, "flare_lookup_backward: %lld rows, %lld entries",
+    OPS_CHECK(a->rows < 0x7fffffffll && a->n < 0x80000000ll - 8192, "flare_lookup_backward: %lld rows, %lld entries",
               a->rows, a->n);
     OPS_CHECK(a->n == 0 || (a->index && (a->dout || a->width == 0)), "flare_lookup_backward: NULL buffer");
     OPS_CHECK(!a->dweight || a->n == 0 || a->table || a->rows == 0 || a->width == 0, "flare_lookup_backward: dweight needs the table");

@@ -20,6 +20,7 @@ from .microscale import Micro4
 
 _FLOATS = tuple(_ops.TYPE_CODE)
 _INDICES = tuple(_ops.INDEX_CODE)
+MAX_ROWS, MAX_ENTRIES = 2 ** 31 - 2, 2 ** 31 - 8193  # of lookup_backward
 
 
 def _entries(idx, weight, device):
@@ -81,8 +82,8 @@ def lookup_backward(dout, table, idx, weight=None, scale=1.0, need_table=True, n
     _ops.need(dout, "dout", _FLOATS, device)
     _ops.need_shape(dout, "dout", tuple(idx.shape) + (width,))
     n = idx.numel()
-    if n_rows >= 2 ** 31 - 1 or n >= 2 ** 31 - 8192:
-        raise ValueError(f"lookup_backward: {n_rows} rows and {n} entries, at most 2^31 - 8192")
+    if n_rows > MAX_ROWS or n > MAX_ENTRIES:
+        raise ValueError(f"lookup_backward: {n_rows} rows and {n} entries, at most {MAX_ROWS} and {MAX_ENTRIES}")
     dout = _ops.rows(dout)
     need_weight = weight is not None if need_weight is None else need_weight
     with _ops.on(device):

@@ -379,7 +379,7 @@ int flare_lookup(const flare_lookup_args *a, void *stream);
  * 32 bits and in a fixed order (the entries are sorted by index, stably), so that results repeat bit for
  * bit; rows that no entry names get zeros.  dweight[i] = scale * <dout[i], table[index[i]]>, 0 where the
  * index names no row.  dtable or dweight may be NULL; table is read for dweight only.  workspace:
- * flare_lookup_workspace bytes, 16-byte aligned, contents irrelevant.  rows < 2^31 - 1, n < 2^31 - 4096.
+ * flare_lookup_workspace bytes, 16-byte aligned, contents irrelevant.  rows < 2^31 - 1, n < 2^31 - 8192.
  */
 typedef struct flare_lookup_grad_args {
     const void *dout;             /* (n, width) */

@@ -1,5 +1,6 @@
 """Row lookup with scaling and its gradient against a 64-bit restatement (GPU), refusals (CPU)."""
 import ctypes
+import os
 
 import numpy as np
 import pytest
@@ -238,3 +239,16 @@ def test_c_entry_refuses_bad_arguments():
     b = _lib.LookupGradArgs(n=5, rows=3, width=4, dout=16, index=16, dtable=16, dout_stride=4)
     assert lib.flare_lookup_backward(ctypes.byref(b), None) == 1 and b"workspace" in lib.flare_last_error()
     assert lib.flare_lookup_workspace(3, 5, 4) > 0 and lib.flare_lookup_workspace(0, 5, 4) == 0
+
+
+def test_one_bound_on_the_number_of_entries():
+    lib = _lib.load()
+    for n, why in ((embedding.MAX_ENTRIES, b"NULL buffer"), (embedding.MAX_ENTRIES + 1, b"entries")):
+        a = _lib.LookupGradArgs(n=n, rows=1, width=4)
+        assert lib.flare_lookup_backward(ctypes.byref(a), None) == 1 and why in lib.flare_last_error()
+    for rows, why in ((embedding.MAX_ROWS, b"NULL buffer"), (embedding.MAX_ROWS + 1, b"rows")):
+        a = _lib.LookupGradArgs(n=1, rows=rows, width=4)
+        assert lib.flare_lookup_backward(ctypes.byref(a), None) == 1 and why in lib.flare_last_error()
+    header = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "flare_b200.h")
+    text = " ".join(open(header).read().replace("\n *", " ").split())
+    assert f"rows < 2^31 - {2 ** 31 - 1 - embedding.MAX_ROWS}, n < 2^31 - {2 ** 31 - 1 - embedding.MAX_ENTRIES}." in text
