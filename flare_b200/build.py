@@ -15,7 +15,7 @@ OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libflare_b200.so")
 SOURCES = ["api.cu", "bvh.cu", "bvh4.cu", "ploc.cu", "trace.cu", "shade.cu", "viewer.cu", "optim.cu", "noalloc.cu",
            "lookup.cu", "recurrence.cu", "micro.cu", "product.cu"]
-HEADERS = ["common.cuh", "renderer.cuh", "umma.cuh", "ops.cuh"]
+HEADERS = ["common.cuh", "renderer.cuh", "umma.cuh", "ops.cuh", "product_plan.h"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
          "--expt-relaxed-constexpr"]

@@ -12,7 +12,7 @@
 //   * warp 9 issues the products; its commit frees the stage.
 // Warps 0-3 read a finished D from TMEM, a row per thread, round it once and store it through shared memory by TMA, while
 // the next tile goes into the other half of TMEM.  Few tiles and a long K: up to 8 blocks of a cluster take a part of K
-// each and add their tiles through distributed shared memory, in order.
+// each (product_plan.h) and add their tiles through distributed shared memory, in order.
 // A few rows that are not quantised yet (at most 16) are Q as they come: four times warps 4-7 quantise a stage of them on the way
 // into shared memory, a block of 32 elements per thread, which saves such a call a launch and a matrix.  Scales then lie there
 // too, 32 rows of 16 bytes, row r the words of tile rows r, r + 32, r + 64, r + 96, and warp 9 spreads them over TMEM.
@@ -23,6 +23,7 @@
 
 #include "common.cuh"
 #include "ops.cuh"
+#include "product_plan.h"
 #include "umma.cuh"
 
 namespace flare {
@@ -230,9 +231,6 @@ __device__ __forceinline__ void stage_output(unsigned char *to, uint32_t tmem) {
         *reinterpret_cast<uint4 *>(to + lane * 128 + ((b ^ (lane & 7)) << 4)) = v.raw[0];
     }
 }
-
-// stages of K per block of a cluster: an even number, as scales are read two stages at a time
-__host__ __device__ constexpr int part_of_k(int all, int S) { return S == 1 ? all : ((all + S - 1) / S + 1) / 2 * 2; }
 
 // X: the type of a Q that is quantised here, or void
 template <int BN, class O, class X>
@@ -899,10 +897,8 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     auto tiles = [&](int b) { return ptiles * ((a.q + b - 1) / b); };
     if (bn < a.q && tiles(192) >= SMS) bn = 192;
     while (bn > 64 && tiles(bn) < SMS) bn /= 2;
-    // and then parts of K (two stages each at least), as long as all blocks of the clusters run at once
-    const int steps = (in->k + KSTAGE - 1) / KSTAGE;
-    int split = 1;
-    while (split < 8 && tiles(bn) * split * 2 <= SMS && steps >= split * 2) split *= 2;
+    // and then parts of K
+    const int split = parts_of_k((in->k + KSTAGE - 1) / KSTAGE, tiles(bn), (int)std::min<long long>(a.q, bn), in->x != nullptr);
     // whole 128-byte pieces of output rows go by TMA
     a.bulk = !a.swap && split == 1 && a.vec && bn * size >= 128;
     e = matrix_map(&pm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pc, a.p, 16ll * a.blocks, 16ll * a.blocks, PT);

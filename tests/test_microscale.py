@@ -1,5 +1,8 @@
 """Microscaled 4-bit matrices: quantisation, values, lookup and product against a 64-bit restatement (GPU), refusals (CPU)."""
 import ctypes
+import os
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -249,3 +252,49 @@ def test_c_entry_refuses_bad_arguments():
     assert lib.flare_micro_product(ctypes.byref(a), None) == 1 and b"17 rows" in lib.flare_last_error()
     a = _lib.ProductArgs(m=1, n=1, k=32, out_stride=1, a_codes=8, b_codes=16, a_scales=16, b_scales=16, out=16)
     assert lib.flare_micro_product(ctypes.byref(a), None) == 1 and b"aligned" in lib.flare_last_error()
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs a C++ compiler")
+def test_blocks_that_share_a_tile_cover_k_and_run_at_once(tmp_path):
+    """Over all numbers of stages, tiles and columns; a short K is not shared, a long one is."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "flare_b200", "csrc")
+    src, exe = tmp_path / "probe.cpp", tmp_path / "probe"
+    src.write_text("""#include <cstdio>
+#include "product_plan.h"
+using namespace flare;
+int main() {
+    const int columns[] = {1, 4, 16, 24, 64}, most[] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+    for (int all = 1; all <= 600; ++all)
+        for (long long tiles = 1; tiles <= 200; ++tiles)
+            for (int c : columns)
+                for (int plain = 0; plain <= (c <= 16); ++plain) {
+                    const int S = parts_of_k(all, tiles, c, plain), per = part_of_k(all, S);
+                    if (S < 1 || S > 8 || (S > 1 && tiles > most[S]) || (long long)S * per < all || (S > 1 && per % 2)) {
+                        std::printf("%d stages, %lld tiles, %d columns: %d parts of %d;", all, tiles, c, S, per);
+                        return 1;
+                    }
+                }
+    std::printf("%d %d %d %d", parts_of_k(4, 8, 64, false), parts_of_k(2, 32, 4, true), parts_of_k(16, 32, 4, true),
+                parts_of_k(32, 8, 64, false));
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-I", csrc, str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout == "1 1 4 8", out.stdout
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stages", [2, 6, 7, 10, 14, 16, 18, 26])
+@pytest.mark.parametrize("n", [65, 1900, 2600, 3300])
+@pytest.mark.parametrize("m", [2, 40])
+def test_product_of_parts_of_k_is_exact(m, n, stages):
+    """1 to 8 blocks share a tile, some without a stage of their own; K ends inside one.  Small whole numbers, so equality."""
+    g = torch.Generator().manual_seed(stages)
+    k = 256 * stages - 37
+    a, b = (torch.randint(-2, 3, (r, k), generator=g).float() for r in (m, n))
+    for t in (a, b):
+        t[:, ::32] = 4.0  # every block's scale is 1
+    want = a @ b.T  # sums below 2^24
+    w = microscale.quantize(b.to(DEV))
+    for x in (a.to(DEV), microscale.quantize(a.to(DEV))):
+        assert torch.equal(microscale.product(x, w, dtype=F32, check=True).cpu(), want)
