@@ -113,6 +113,16 @@ inline bool overlaps(const void *p, long long p_bytes, const void *q, long long 
     return p && q && p_bytes > 0 && q_bytes > 0 && a < b + (uintptr_t)q_bytes && b < a + (uintptr_t)p_bytes;
 }
 
+// The same for a stretch and `rows` rows of row_bytes, `stride` bytes apart.
+inline bool overlaps_rows(const void *p, long long p_bytes, const void *q, long long rows, long long row_bytes, long long stride) {
+    if (rows <= 0 || stride == 0) return overlaps(p, p_bytes, q, rows > 0 ? row_bytes : 0);
+    if (stride < 0) return overlaps_rows(p, p_bytes, static_cast<const char *>(q) + (rows - 1) * stride, rows, row_bytes, -stride);
+    // the first row that ends behind the stretch's start
+    const long long before = (long long)(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(q)) - row_bytes;
+    const long long row = before < 0 ? 0 : before / stride + 1;
+    return row < rows && overlaps(p, p_bytes, static_cast<const char *>(q) + row * stride, row_bytes);
+}
+
 // 2^(byte - 127); byte 255 stands for NaN
 __device__ __forceinline__ float micro_scale(unsigned byte) {
     if (byte == 0) return __uint_as_float(0x00400000u);

@@ -761,19 +761,30 @@ int rec_check(const flare_recurrence_args *a, bool backward, const char *what) {
     const long long gate = std::max(std::abs(a->gate_t), std::abs(a->dgate_t)) * type_size(a->gate_type);
     const long long rest = std::max({std::abs(a->x_t), std::abs(a->h_t), std::abs(a->dh_t), std::abs(a->dx_t)}) * type_size(a->x_type);
     OPS_CHECK(gate < 0x7fffffffll && rest < 0x7fffffffll, "%s: steps %lld bytes apart, less than 2^31 needed", what, std::max(gate, rest));
-    OPS_CHECK(a->offsets_type == FLARE_I32 || a->offsets_type == FLARE_I64, "%s: unknown offsets type %d", what, a->offsets_type);
     const bool some = a->seqs > 0, data = (some || a->offsets) && a->steps > 0;
     OPS_CHECK(!data || (a->gate && a->x), "%s: NULL gate or x", what);
     const long long ends = 4 * a->seqs * a->width;
     if (!backward) {
         OPS_CHECK(!some || a->last, "%s: NULL last", what);
         OPS_CHECK(a->last == a->state || !overlaps(a->last, ends, a->state, ends), "%s: last overlaps state", what);
+        // a step's caller chooses where the new state goes; element for element it may take an input's place, as each
+        // thread reads all of its own before it writes
+        if (a->steps == 1 && !a->offsets && a->last) {
+            auto apart = [&](const void *p, long long stride, int width, int type) {
+                const int size = type_size(type);
+                return (p == a->last && type == FLARE_F32 && width == a->width && (stride == width || a->seqs == 1)) ||
+                       !overlaps_rows(a->last, ends, p, a->seqs, (long long)width * size, stride * size);
+            };
+            OPS_CHECK(apart(a->x, a->x_s, a->width, a->x_type), "%s: last overlaps x", what);
+            OPS_CHECK(apart(a->gate, a->gate_s, a->groups, a->gate_type), "%s: last overlaps gate", what);
+        }
     } else {
         OPS_CHECK(a->dstate == a->dlast || !overlaps(a->dstate, ends, a->dlast, ends), "%s: dstate overlaps dlast", what);
         const bool spans = some && a->steps > SPAN;
         OPS_CHECK(!data || (a->dgate && a->dx), "%s: NULL gradient", what);
         OPS_CHECK(!spans || a->saved, "%s: NULL saved", what);
     }
+    OPS_CHECK(a->offsets_type == FLARE_I32 || a->offsets_type == FLARE_I64, "%s: unknown offsets type %d", what, a->offsets_type);
     return FLARE_OK;
 }
 

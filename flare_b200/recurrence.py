@@ -145,8 +145,8 @@ def step(gate, x, state, out=None):
     """One step for every sequence, for a caller that keeps the state: out = gate * state + x, f32 (sequences, width),
     written in place of `state` unless another tensor is given; returns it in x's type (a new tensor).
 
-    x: (sequences, width) f32, f16 or bf16; gate: (sequences, groups), of x's type or f32.  out is state itself or overlaps
-    none of the inputs.
+    x: (sequences, width) f32, f16 or bf16; gate: (sequences, groups), of x's type or f32.  What is written may be one of
+    the inputs, element for element, and overlaps them in no other way (FlareError).
     """
     lib = _lib.load()
     _ops.need(x, "x", _FLOATS)

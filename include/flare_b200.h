@@ -410,7 +410,8 @@ int flare_lookup_backward(const flare_lookup_grad_args *a, void *stream);
  * Backward reads gate, x, state, saved, dh (NULL: 0) and dlast (NULL: 0) and writes dgate, dx and, if not
  * NULL, dstate.  workspace: flare_recurrence_workspace bytes of these arguments, 16-byte aligned, contents irrelevant.
  * What is written overlaps nothing that is read and nothing else that is written, except that last may be state
- * and dstate may be dlast (a state kept in place); where they overlap in part the call is refused.
+ * and dstate may be dlast (a state kept in place), and with a single step last may be x or gate, element for
+ * element; where these overlap otherwise the call is refused.
  * A product of gates over a stretch of steps has to stay within the range of a float.  seqs * width and steps are
  * below 2^30, the steps of a tensor less than 2^31 bytes apart.
  */

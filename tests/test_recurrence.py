@@ -321,3 +321,48 @@ def test_c_entry_keeps_a_state_in_place(shape):
     dg, dx, ends = torch.empty_like(c["gate"]), torch.empty_like(c["x"]), c["dlast"].clone()
     call(lib.flare_recurrence_backward, 1, state=c["state"], saved=saved, dh=c["dh"], dlast=ends, dstate=ends, dgate=dg, dx=dx)
     assert torch.equal(dg, want[0]) and torch.equal(dx, want[1]) and torch.equal(ends, want[2])
+
+
+def test_c_entry_refuses_a_step_over_part_of_its_inputs():
+    """Addresses only: whatever is not refused is not run."""
+    lib = _lib.load()
+    B, D, at = 4, 10, 1 << 20  # last: 160 bytes from `at`
+
+    def why(gate=at - 4096, gate_s=2, groups=2, gate_type=0, x=at + 4096, x_s=D, x_type=0, state=at + 65536):
+        a = _lib.RecurrenceArgs(gate=gate, x=x, state=state, last=at, seqs=B, steps=1, gate_s=gate_s, x_s=x_s, width=D, groups=groups,
+                                gate_type=gate_type, x_type=x_type, offsets_type=7)  # the check behind these
+        assert lib.flare_recurrence_forward(ctypes.byref(a), None) == 1
+        return lib.flare_last_error().decode().split(": ")[1]
+
+    free = "unknown offsets type 7"
+    for kw, want in ((dict(), free), (dict(state=at), free), (dict(state=at + 4), "last overlaps state"), (dict(x=at), free),
+                     (dict(x=at, x_s=12), "last overlaps x"), (dict(x=at + 4), "last overlaps x"), (dict(x=at + 160), free),
+                     (dict(x=at - 160), free), (dict(x=at - 156), "last overlaps x"), (dict(x=at, x_type=1), "last overlaps x"),
+                     (dict(x=at - 40, x_s=50), free), (dict(x=at - 40, x_s=49), "last overlaps x"), (dict(x=at - 36, x_s=0), "last overlaps x"),
+                     (dict(x=at - 40, x_s=0), free), (dict(gate=at), "last overlaps gate"), (dict(gate=at, groups=D, gate_s=D), free),
+                     (dict(gate=at - 4 * 8, gate_s=2), free), (dict(gate=at - 4 * 8, gate_s=3), "last overlaps gate")):
+        assert why(**kw) == want, kw
+
+
+@pytest.mark.gpu
+def test_step_writes_over_an_input_only_as_a_whole():
+    g = torch.Generator().manual_seed(3)
+    buf, gate = torch.randn(200, generator=g).to(DEV), torch.rand(4, 2, generator=g).to(DEV)
+    state, x = buf[:40].view(4, 10), buf[100:140].view(4, 10)
+    for o in (buf[1:41].view(4, 10), buf[30:70].view(4, 10)):
+        with pytest.raises(_lib.FlareError, match="last overlaps state"):
+            recurrence.step(gate, x, state, out=o)
+    with pytest.raises(_lib.FlareError, match="last overlaps x"):
+        recurrence.step(gate, x, state, out=buf[90:130].view(4, 10))
+    with pytest.raises(_lib.FlareError, match="last overlaps x"):
+        recurrence.step(gate, buf[5:45].view(4, 10), state)
+    with pytest.raises(_lib.FlareError, match="last overlaps gate"):
+        recurrence.step(buf[160:168].view(4, 2), x, state, out=buf[160:].view(4, 10))
+    for gt in (gate, torch.rand(4, 10, generator=g).to(DEV)):
+        want = recurrence.step(gt, x, state, out=torch.empty_like(state))
+        for into in ("state", "x", "gate"):
+            t = dict(gate=gt.clone(), x=x.clone(), state=state.clone())
+            if t[into].shape == state.shape:
+                assert torch.equal(recurrence.step(**t, out=t[into]), want) and torch.equal(t[into], want)
+    twice = state.clone()
+    assert torch.equal(recurrence.step(gate, twice, twice), recurrence.step(gate, state, state, out=torch.empty_like(state)))
