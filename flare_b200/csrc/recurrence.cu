@@ -723,7 +723,9 @@ int run_recurrence(const flare_recurrence_args *in, bool backward, cudaStream_t 
         plain.tiles = (a.units + 31) / 32;
         const dim3 sgrid((plain.tiles + at_once - 1) / at_once, (unsigned)p.splits);
         if (!backward) {
-            if (p.splits > 1) recurrence_split_kernel<false, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
+            // 8 channels a lane take 300,000 channels, which leave nothing to split
+            if constexpr (VE < 8)
+                if (p.splits > 1) recurrence_split_kernel<false, T, GT, VE, SH><<<sgrid, 32 * WARPS, buffers, st>>>(plain);
             recurrence_forward_kernel<T, GT, VE, SH><<<grid, 32 * WARPS, buffers, st>>>(a);
             return;
         }
