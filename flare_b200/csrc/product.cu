@@ -898,7 +898,8 @@ int run_product(const flare_product_args *in, cudaStream_t st) {
     if (bn < a.q && tiles(192) >= SMS) bn = 192;
     while (bn > 64 && tiles(bn) < SMS) bn /= 2;
     // and then parts of K
-    const int split = parts_of_k((in->k + KSTAGE - 1) / KSTAGE, tiles(bn), (int)std::min<long long>(a.q, bn), in->x != nullptr);
+    const int split = parts_of_k((in->k + KSTAGE - 1) / KSTAGE, tiles(bn), (int)std::min<long long>(a.q, bn), in->x != nullptr,
+                                 a.swap ? Store::columns : a.vec ? Store::rows_of_16 : Store::rows);
     // whole 128-byte pieces of output rows go by TMA
     a.bulk = !a.swap && split == 1 && a.vec && bn * size >= 128;
     e = matrix_map(&pm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pc, a.p, 16ll * a.blocks, 16ll * a.blocks, PT);

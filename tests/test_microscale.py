@@ -264,29 +264,32 @@ def test_blocks_that_share_a_tile_cover_k_and_run_at_once(tmp_path):
 using namespace flare;
 int main() {
     const int columns[] = {1, 4, 16, 24, 64}, most[] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
-    for (int all = 1; all <= 600; ++all)
+    for (int all = 1; all <= 300; ++all)
         for (long long tiles = 1; tiles <= 200; ++tiles)
             for (int c : columns)
-                for (int plain = 0; plain <= (c <= 16); ++plain) {
-                    const int S = parts_of_k(all, tiles, c, plain), per = part_of_k(all, S);
-                    if (S < 1 || S > 8 || (S > 1 && tiles > most[S]) || (long long)S * per < all || (S > 1 && per % 2)) {
-                        std::printf("%d stages, %lld tiles, %d columns: %d parts of %d;", all, tiles, c, S, per);
+                for (int way = 0; way < (c <= 16 ? 6 : 3); ++way) {
+                    const bool plain = way > 2;
+                    const int S = parts_of_k(all, tiles, c, plain, (Store)(way % 3)), per = part_of_k(all, S);
+                    const bool once = S == 1 || tiles <= most[S] || (!plain && per == 2 && tiles * S <= 148);
+                    if (S < 1 || S > 8 || !once || (long long)S * per < all || (S > 1 && per % 2)) {
+                        std::printf("%d stages, %lld tiles, %d columns, way %d: %d parts of %d;", all, tiles, c, way, S, per);
                         return 1;
                     }
                 }
-    std::printf("%d %d %d %d", parts_of_k(4, 8, 64, false), parts_of_k(2, 32, 4, true), parts_of_k(16, 32, 4, true),
-                parts_of_k(32, 8, 64, false));
+    std::printf("%d %d %d %d %d", parts_of_k(4, 8, 64, false, Store::columns), parts_of_k(2, 32, 4, true, Store::columns),
+                parts_of_k(16, 32, 4, true, Store::columns), parts_of_k(32, 8, 64, false, Store::columns),
+                parts_of_k(32, 16, 64, false, Store::rows_of_16));
 }
 """)
     subprocess.run(["g++", "-std=c++17", "-I", csrc, str(src), "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True)
-    assert out.returncode == 0 and out.stdout == "1 1 4 8", out.stdout
+    assert out.returncode == 0 and out.stdout == "1 1 4 8 6", out.stdout
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("stages", [2, 6, 7, 10, 14, 16, 18, 26])
 @pytest.mark.parametrize("n", [65, 1900, 2600, 3300])
-@pytest.mark.parametrize("m", [2, 40])
+@pytest.mark.parametrize("m", [2, 40, 61])
 def test_product_of_parts_of_k_is_exact(m, n, stages):
     """1 to 8 blocks share a tile, some without a stage of their own; K ends inside one.  Small whole numbers, so equality."""
     g = torch.Generator().manual_seed(stages)
@@ -298,3 +301,4 @@ def test_product_of_parts_of_k_is_exact(m, n, stages):
     w = microscale.quantize(b.to(DEV))
     for x in (a.to(DEV), microscale.quantize(a.to(DEV))):
         assert torch.equal(microscale.product(x, w, dtype=F32, check=True).cpu(), want)
+    assert torch.equal(microscale.product(w, x, dtype=F32, check=True).cpu(), want.T)  # the tiles' rows are the output's
