@@ -1,5 +1,5 @@
-// ops.cuh -- shared by the operators outside the render path (lookup.cu, recurrence.cu, micro.cu): element
-// types, vector loads and stores through 32-bit floats, argument checks.
+// ops.cuh -- shared by the operators outside the render path (lookup.cu, recurrence.cu, micro.cu, product.cu): element
+// types, vector loads and stores through 32-bit floats, the 4-bit format, argument checks.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

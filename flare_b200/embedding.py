@@ -69,7 +69,8 @@ def lookup_backward(dout, table, idx, weight=None, scale=1.0, need_table=True, n
     idx's shape), each None where it is not asked for (need_weight: by default whether there is a weight).
 
     dout: idx.shape + (width,), f32, f16 or bf16, of any type whatever the table's.  The entries of a row are added in
-    ascending order in 32 bits, so results repeat bit for bit; rows that no entry names get zeros.  A Micro4 table
+    32 bits in an order that the sizes fix (ascending within stretches of 32 to 256 sorted entries, whose sums are then
+    added), so results repeat bit for bit; rows that no entry names get zeros.  A Micro4 table
     has no gradient: ValueError.
     """
     lib = _lib.load()

@@ -1,8 +1,9 @@
 """Matrices held in 4 bits an element with a power-of-two scale per 32 (microscaled 4-bit floats), and their product.
 
-A 96-wide f16 descriptor takes 192 of the 312 bytes that a hit reads; held here it takes 52.  `quantize` makes a `Micro4`
-from a tensor, `Micro4.dequantize` and `embedding.lookup` read it back, the renderer's inference methods take one as
-`conditioning_variable`, and `product` multiplies two of them on the tensor cores.  Inference only: none of them has a
+A 96-wide f16 descriptor takes 192 bytes; held here it takes 52, in memory and in each row that `embedding.lookup` reads.
+`quantize` makes a `Micro4` from a tensor, `Micro4.dequantize` reads it back, and `product` multiplies two of them on the
+tensor cores.  The renderer's inference methods take one as `conditioning_variable` too, but expand the whole table to f16 at
+every call (a pass over it and as much memory again while the call runs): for many frames `dequantize` it once.  Inference only: none of them has a
 gradient.  No reference counterpart.
 """
 from __future__ import annotations

@@ -95,8 +95,10 @@ def scan(gate, x, state=None, offsets=None, reverse=False, states=True, training
     With offsets (sequences + 1,) int32 or int64, non-decreasing, x is (rows, width) and gate (rows, groups), and
     sequence s is rows offsets[s] to offsets[s + 1]; it may be empty.  Rows of no sequence get zeros.
     h: every state, of x's shape and type (None if not states); last: the final states (sequences, width) f32; saved:
-    what scan_backward needs (None if not training).  The recurrence runs in 32 bits, h is rounded once; a product of
-    gates over any stretch of steps has to stay within the range of a float.  A tensor's steps are less than 2 GB apart
+    what scan_backward needs (None if not training).  The recurrence runs in 32 bits, h is rounded once.  Time is
+    cut into stretches, and the product of a stretch's gates is a float: where it is too small, the state that enters the
+    stretch counts as 0 behind it; where it is too large (gates above 1), a state other than 0 gives infinity or NaN behind it
+    even if single steps would stay finite.  A tensor's steps are less than 2 GB apart
     (FlareError).
     """
     lib = _lib.load()

@@ -12,7 +12,8 @@ Differences from the reference, by design:
   * arguments are checked (CUDA, contiguous, dtype, shapes); violations raise ValueError instead of
     corrupting memory;
   * failures raise FlareError (a RuntimeError) carrying the library's message instead of `throw 0`;
-  * the methods that compute no gradient also take the descriptors as a 4-bit `microscale.Micro4`;
+  * the methods that compute no gradient also take the descriptors as a 4-bit `microscale.Micro4`, which each call
+    expands to f16 first (a pass over the table, and its f16 size in memory while the call runs);
   * the work runs on torch.cuda.current_stream() of the renderer's device without a host sync per
     pass beyond reading the active-ray count.
 """

@@ -412,7 +412,9 @@ int flare_lookup_backward(const flare_lookup_grad_args *a, void *stream);
  * What is written overlaps nothing that is read and nothing else that is written, except that last may be state
  * and dstate may be dlast (a state kept in place), and with a single step last may be x or gate, element for
  * element; where these overlap otherwise the call is refused.
- * A product of gates over a stretch of steps has to stay within the range of a float.  seqs * width and steps are
+ * Time is cut into stretches, and the product of a stretch's gates is a float: where it is too small, the state that
+ * enters the stretch counts as 0 behind it; where it is too large (gates above 1), a state other than 0 gives
+ * infinity or NaN behind it even if single steps would stay finite.  seqs * width and steps are
  * below 2^30, the steps of a tensor less than 2^31 bytes apart.
  */
 #define FLARE_RECURRENCE_SPAN 16
