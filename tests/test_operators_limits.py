@@ -102,6 +102,25 @@ def test_product_past_2_to_the_31_outputs():
         assert torch.equal(out[s].float(), a[s] @ b.T)  # whole numbers below 100
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [4000, 16_384, 16_385, 70_000])
+@pytest.mark.parametrize("rows", [1, 5, 1023, 1024, 2 ** 20 + 5, embedding.MAX_ROWS])
+def test_lookup_gradient_of_every_number_of_digits(rows, n):
+    """Row numbers of 1 to 31 bits, up to the most rows there may be."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    idx = torch.randint(0, rows, (n,), device=DEV, generator=g)
+    idx[::7], idx[1::7], idx[3] = rows - 1, 0, -1
+    idx[5::50] = rows  # no row
+    dout = torch.randint(-3, 4, (n, 1), device=DEV, generator=g).float()
+    dt, _ = embedding.lookup_backward(dout, torch.empty(rows, 1, dtype=F16, device=DEV), idx)
+    some = (idx >= 0) & (idx < rows)
+    named, inverse = idx[some].unique(return_inverse=True)
+    want = torch.zeros(named.numel(), 1, device=DEV).index_add_(0, inverse, dout[some])
+    assert torch.equal(dt[named], want)
+    dt[named] = 0
+    assert not dt.any()
+
+
 FIRST = """
 import torch
 from flare_b200 import embedding, microscale, recurrence
